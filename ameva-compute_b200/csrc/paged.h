@@ -1,0 +1,19 @@
+// Launchers of the paged KV cache's attention kernels (paged.cuh), called by the launchers of their entry points (paged_attn.cu).
+#pragma once
+#include "paged.cuh"
+
+namespace amv {
+namespace paged {
+
+// Maps of the cache for boxes of `tokens` tokens x 64 columns of one head and page; false where no map expresses the strides.
+struct Maps {
+    CUtensorMap k, v;
+};
+
+constexpr uint32_t kDecRows = 16;                        // paged_attn.cu: rows per tile
+constexpr uint32_t kTcRows = 256, kTcKeys = 128;         // paged_tc.cu: rows and keys per tile
+
+bool launch_tc(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t head_dim, uint32_t ctas);
+
+}  // namespace paged
+}  // namespace amv

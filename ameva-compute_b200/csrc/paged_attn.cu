@@ -1,0 +1,650 @@
+// Attention over a paged KV cache (paged.cuh): ameva_paged_attn, and ameva_paged_prefix_attn for a batch that shares the pages of a
+// long prefix. Here: the kernel for few rows per sequence (tokens, drafts), the merge kernel and the launchers; many rows per
+// sequence (prompts, the prefix of a batch) run in paged_tc.cu.
+//
+// paged_rows_kernel: W + 1 warps. The last one streams key tiles (16 W keys, K and V) through a ring in shared memory with TMA, a box
+// of up to 64 columns x one page each, and runs ahead across the pieces of the CTA's stretch, so that the reads never pause. Each of
+// the others takes 16 keys of every tile for the tile's 16 rows: both products on mma.sync (f16 in, f32 out), an online softmax per row
+// to base 2, the scores' accumulators reused as the A operand of the second product. At the end of a piece the warps are joined through
+// shared memory. P: for an f32 result as an f16 value and its remainder (rounded once, 2^-12 of every probability would show there), for
+// an f16 result rounded once (2^-12 against the 2^-12 of the result itself, averaged over the keys).
+#include <cstring>
+
+#include "paged.h"
+#include "sync_ptx.cuh"
+#include "tcgen05_ptx.cuh"
+#include "tensor_map.h"
+
+namespace amv {
+namespace paged {
+
+using namespace ptx;
+
+template <int D>
+struct Rows {
+    static constexpr uint32_t W = D == 256 ? 4 : 8, KEYS = 16 * W, ATOMS = D / 64;
+    static constexpr uint32_t TILE = KEYS * D * 2u, STAGE = 2u * TILE, STAGES = D == 64 ? 6 : 3;
+    static constexpr uint32_t MERGE = (W / 2) * 8u * (D + 4u) * 4u;   // half the warps' results for eight rows
+    static constexpr uint32_t STATE = W * kDecRows * 2u * 4u;
+    static constexpr uint32_t FIXED = 1024u + STAGES * STAGE + MERGE + STATE + 128u + 16u * STAGES;
+    static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at));
+}
+// D (16 x 8, f32) += A (16 x 16, f16) * B (16 x 8, f16)
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t halves(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map),
+        "r"(bar), "r"(column), "r"(token), "r"(head), "r"(page)
+        : "memory");
+}
+template <uint32_t THREADS>
+__device__ __forceinline__ void worker_sync() {   // the warps that multiply, not the one that loads
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
+
+// TOP: every row tile has at most eight rows (the upper half of the MMA tile), so the lower half's work is left out.
+template <int D, bool TOP, bool EXACT>
+__global__ void __launch_bounds__((Rows<D>::W + 1) * 32, 1)
+paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args pc) {
+    using L = Rows<D>;
+    constexpr uint32_t W = L::W, KEYS = L::KEYS, A = L::ATOMS, C = D / 32, H = TOP ? 1 : 2;
+    constexpr int KS = D / 16, NT = D / 8;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    float* s_merge = reinterpret_cast<float*>(base + L::STAGES * L::STAGE);        // [W / 2][8][D + 4]
+    float* s_m = s_merge + L::MERGE / 4u;                                          // [W][16] maxima
+    float* s_l = s_m + W * kDecRows;                                               // [W][16] sums
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + W * kDecRows);              // full, empty
+    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 2u * L::STAGES);
+    uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                       // [W + 1]
+    uint32_t* s_bad = s_warp + W + 1u;                                             // per stage: 16-key blocks whose page is none
+    uint32_t* s_pref = s_bad + L::STAGES;
+    const uint32_t full = smem_u32(bars), empty = full + 8u * L::STAGES;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < L::STAGES; ++s) {
+            mbar_init(full + 8u * s, 1u);
+            mbar_init(empty + 8u * s, W);
+        }
+        ctl->abort = 0u;
+        fence_barrier_init();
+    }
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t total = build_line<kDecRows, KEYS, W + 1u>(pc, s_pref, s_warp);   // (its barriers publish the ones above)
+    const Stretch st = my_stretch(total);
+    Walk<kDecRows, KEYS> walk(st);
+    const uint32_t P = 1u << pc.page_log2, box = P < KEYS ? P : KEYS;
+    Ring ring(L::STAGES);
+    bool ok = true;
+
+    if (warp == W) {   // ---- loads ----
+        uint32_t issued = 0;
+        while (ok && walk.next(pc, s_pref)) {
+            const Piece& p = walk.p;
+            const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + kDecRows, p.R) - 1u).hi;
+            for (uint32_t i = p.a; i < p.b; ++i) {
+                const uint32_t key0 = (p.first + i) * KEYS;
+                ok = mbar_wait(empty + 8u * ring.idx, ring.phase ^ 1u, ctl, pc.status, 0xC00u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                // boxes of the tile: the first lanes look their pages up; those that hold a key somebody sees are loaded
+                const uint32_t boxes = KEYS / box, b0 = key0 + lane * box;
+                int32_t page = -1;
+                bool want = lane < boxes && b0 < hi && b0 + box > lo;
+                if (want) page = page_of(pc, p.q, b0);
+                const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0), load = __ballot_sync(0xffffffffu, want && page >= 0);
+                uint32_t bad = 0;
+                if (none) {   // as 16-key blocks
+                    for (uint32_t j = 0; j < W; ++j) bad |= (none >> (16u * j / box) & 1u) << j;
+                    if (lane == 0u) refuse(pc, __popc(none));
+                }
+                const uint32_t stage = smem_u32(base) + ring.idx * L::STAGE, bar = full + 8u * ring.idx;
+                if (lane == 0u) {
+                    s_bad[ring.idx] = bad;
+                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(load) * box * D * 2u * 2u);
+                }
+                __syncwarp();
+                for (uint32_t j = lane; j < boxes * A * 2u; j += 32u) {
+                    const uint32_t b = j % boxes, a = j / boxes % A, kv = j / (boxes * A);
+                    if (!(load >> b & 1u)) continue;
+                    const int32_t pg = page_of(pc, p.q, key0 + b * box);   // (just read: from L1)
+                    tma_page(stage + kv * L::TILE + a * (KEYS * 128u) + b * box * 128u, kv ? &v_map : &k_map, bar, (int)(64u * a),
+                             (int)((key0 + b * box) & (P - 1u)), (int)p.hkv, pg);
+                }
+                ++issued;
+                ring.advance();
+            }
+        }
+        if (ctl->abort) {   // copies already requested finish before the CTA leaves
+            for (uint32_t i = issued > L::STAGES ? issued - L::STAGES : 0u; i < issued; ++i)
+                mbar_wait(full + 8u * (i % L::STAGES), (i / L::STAGES) & 1u, ctl, pc.status, 0xC10u);
+        }
+        return;
+    }
+
+    // ---- products ----
+    const uint32_t g = lane >> 2, t4 = lane & 3u;
+    const uint32_t lm_row = 16u * warp + (lane & 7u) + ((lane >> 4) << 3), lm_hi = (lane >> 3) & 1u;   // K: key in the tile, upper eight columns
+    const uint32_t lv_row = 16u * warp + (lane & 7u) + (((lane >> 3) & 1u) << 3), lv_nt = lane >> 4;    // V: key in the tile, second n-tile
+    uint32_t done = st.begin;
+    bool cut = false;
+    while (walk.next(pc, s_pref)) {
+        const Piece& p = walk.p;
+        const uint32_t rows = min(kDecRows, p.R - p.r0);
+        const uint32_t lo_all = row_span(pc, p.q, p.r0).lo, hi_all = row_span(pc, p.q, p.r0 + rows - 1u).hi;     // keys that some row sees
+        const uint32_t lo_both = row_span(pc, p.q, p.r0 + rows - 1u).lo, hi_both = row_span(pc, p.q, p.r0).hi;   // keys that every row sees
+        Span span[2];
+        uint32_t qa[KS][4];
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h) {
+            const uint32_t r = p.r0 + g + 8u * h;
+            const bool valid = h < H && g + 8u * h < rows;
+            span[h] = valid ? row_span(pc, p.q, r) : Span{0u, 0u};
+            const __half* qrow = pc.q + (uint64_t)(p.q.tok0 + (valid ? r / pc.G : 0u)) * pc.q_s + (uint64_t)(p.hkv * pc.G + (valid ? r % pc.G : 0u)) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint32_t c = 16u * ks + 2u * t4;
+                qa[ks][h] = valid ? *reinterpret_cast<const uint32_t*>(qrow + c) : 0u;
+                qa[ks][2u + h] = valid ? *reinterpret_cast<const uint32_t*>(qrow + c + 8u) : 0u;
+            }
+        }
+        float oc[NT][4], m_run[2] = {neg_inf(), neg_inf()}, l_run[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) oc[nt][j] = 0.0f;
+
+        for (uint32_t i = p.a; i < p.b; ++i) {
+            const uint32_t key0 = (p.first + i) * KEYS + 16u * warp;
+            ok = ok && mbar_wait(full + 8u * ring.idx, ring.phase, ctl, pc.status, 0xC20u);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;   // (the pieces are walked to the end all the same: the warps meet at their barriers)
+            const uint32_t tk = smem_u32(base) + ring.idx * L::STAGE, tv = tk + L::TILE;
+            const bool seen = key0 < hi_all && key0 + 16u > lo_all && !(s_bad[ring.idx] >> warp & 1u);
+            if (seen) {
+                float sc[2][4];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sc[nt][j] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint32_t piece = 2u * (ks & 3) + lm_hi;
+                    uint32_t b[4];
+                    ldsm_x4(b, tk + (ks >> 2) * (KEYS * 128u) + lm_row * 128u + ((piece ^ (lm_row & 7u)) << 4));
+                    mma16816(sc[0], qa[ks], b[0], b[1]);
+                    mma16816(sc[1], qa[ks], b[2], b[3]);
+                }
+                // V rows behind the last key are whatever the page holds there: probabilities of zero do not hide a NaN
+                if (key0 + 16u > hi_all) {
+                    const uint32_t from = hi_all - key0;   // 1 .. 15
+                    for (uint32_t j = lane; j < (16u - from) * (D / 8u); j += 32u) {
+                        const uint32_t r = 16u * warp + from + j / (D / 8u), c = j % (D / 8u);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tv + (c >> 3) * (KEYS * 128u) + r * 128u + ((c & 7u) << 4)),
+                                     "r"(0u)
+                                     : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (before TMA writes there again)
+                    __syncwarp();
+                }
+                const bool plain = key0 >= lo_both && key0 + 16u <= hi_both;
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (uint32_t h = 0; h < H; ++h) {
+                    float x[2][2], mx = neg_inf();
+#pragma unroll
+                    for (uint32_t nt = 0; nt < 2u; ++nt)
+#pragma unroll
+                        for (uint32_t j = 0; j < 2u; ++j) {
+                            const uint32_t key = key0 + 8u * nt + 2u * t4 + j;
+                            const float v = score2(pc, sc[nt][2u * h + j]);
+                            x[nt][j] = plain || (key >= span[h].lo && key < span[h].hi) ? v : neg_inf();
+                            mx = fmaxf(mx, x[nt][j]);
+                        }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float m_new = fmaxf(m_run[h], mx);
+                    if (__any_sync(0xffffffffu, m_new != m_run[h])) {
+                        const float f = weight(m_run[h], m_new);
+                        l_run[h] *= f;
+                        m_run[h] = m_new;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            oc[nt][2u * h] *= f;
+                            oc[nt][2u * h + 1u] *= f;
+                        }
+                    }
+                    const float ref = m_new == neg_inf() ? 0.0f : m_new;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (uint32_t nt = 0; nt < 2u; ++nt) {
+                        const float p0 = ex2(x[nt][0] - ref), p1 = ex2(x[nt][1] - ref);
+                        sum += p0 + p1;
+                        const __half2 hi2 = __floats2half2_rn(p0, p1);
+                        ph[2u * nt + h] = *reinterpret_cast<const uint32_t*>(&hi2);
+                        if (EXACT) {
+                            const float2 f2 = __half22float2(hi2);
+                            pl[2u * nt + h] = halves(p0 - f2.x, p1 - f2.y);
+                        }
+                    }
+                    l_run[h] += sum;   // (this lane's keys; the four lanes of a row are added at the end)
+                }
+                if (TOP) ph[1] = ph[3] = pl[1] = pl[3] = 0u;
+#pragma unroll
+                for (int np = 0; np < NT / 2; ++np) {   // columns 16 np .. 16 np + 15
+                    const uint32_t piece = 2u * (np & 3) + lv_nt;
+                    uint32_t b[4];
+                    ldsm_x4_trans(b, tv + (np >> 2) * (KEYS * 128u) + lv_row * 128u + ((piece ^ (lv_row & 7u)) << 4));
+                    mma16816(oc[2 * np], ph, b[0], b[1]);
+                    mma16816(oc[2 * np + 1], ph, b[2], b[3]);
+                    if (EXACT) {
+                        mma16816(oc[2 * np], pl, b[0], b[1]);
+                        mma16816(oc[2 * np + 1], pl, b[2], b[3]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0u) mbar_arrive(empty + 8u * ring.idx);
+            ring.advance();
+        }
+        done += p.b - p.a;
+
+        // ---- the warps' results as one: maxima, then eight rows at a time through shared memory ----
+        const bool whole = p.a == 0u && p.b == p.n;
+        float* slot = pc.slots + (uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * kDecRows * (D + 4u);
+#pragma unroll
+        for (uint32_t h = 0; h < H; ++h) {
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+            if (t4 == 0u) {
+                s_m[warp * kDecRows + g + 8u * h] = m_run[h];
+                s_l[warp * kDecRows + g + 8u * h] = l_run[h];
+            }
+        }
+        worker_sync<W * 32u>();
+#pragma unroll
+        for (uint32_t h = 0; h < H; ++h) {
+            if (h * 8u >= rows) break;
+            float mx = neg_inf();
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w * kDecRows + g + 8u * h]);
+            const float f = weight(m_run[h], mx);
+            float* mine = s_merge + ((warp & (W / 2u - 1u)) * 8u + g) * (D + 4u);
+            if (warp >= W / 2u) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    *reinterpret_cast<float2*>(mine + 8 * nt + 2 * t4) =
+                        f == 0.0f ? make_float2(0.f, 0.f) : make_float2(oc[nt][2u * h] * f, oc[nt][2u * h + 1u] * f);
+            }
+            worker_sync<W * 32u>();
+            if (warp < W / 2u) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float2* at = reinterpret_cast<float2*>(mine + 8 * nt + 2 * t4);
+                    const float2 x = *at;
+                    *at = f == 0.0f ? x : make_float2(fmaf(oc[nt][2u * h], f, x.x), fmaf(oc[nt][2u * h + 1u], f, x.y));
+                }
+            }
+            worker_sync<W * 32u>();
+            for (uint32_t i = warp; i < 8u; i += W) {   // a warp per row
+                const uint32_t r = 8u * h + i;
+                if (r >= rows || !ok) break;
+                float m = neg_inf(), l = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, s_m[w * kDecRows + r]);
+#pragma unroll
+                for (uint32_t w = 0; w < W; ++w) l = fmaf(s_l[w * kDecRows + r], weight(s_m[w * kDecRows + r], m), l);
+                float o[C], check = 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < W / 2u; ++w)
+#pragma unroll
+                    for (uint32_t c = 0; c < C; ++c) o[c] += s_merge[(w * 8u + i) * (D + 4u) + C * lane + c];
+#pragma unroll
+                for (uint32_t c = 0; c < C; ++c) check = fmaf(o[c], 0.0f, check);
+                const uint32_t row = p.r0 + r, token = p.q.tok0 + row / pc.G, head = p.hkv * pc.G + row % pc.G;
+                // (a sum that is not finite says that the scores are not: the row is NaN either way)
+                if (__any_sync(0xffffffffu, check != 0.0f) && l - l == 0.0f) {
+                    const Span s = row_span(pc, p.q, row);
+                    const uint32_t from = max(s.lo, (p.first + p.a) * KEYS), to = min(s.hi, (p.first + p.b) * KEYS);
+                    seen_keys_row<C>(pc, p.q, p.hkv, pc.q + (uint64_t)token * pc.q_s + (uint64_t)head * D, from, to, m == neg_inf() ? 0.0f : m, o);
+                }
+                if (whole) {
+                    finish_row<C>(pc, token, head, m, l, o);
+                } else {
+                    float* to = slot + (uint64_t)r * (D + 4u);
+                    if (lane == 0u) *reinterpret_cast<float2*>(to) = make_float2(m, l);
+#pragma unroll
+                    for (uint32_t c = 0; c < C; c += 2u) *reinterpret_cast<float2*>(to + 4u + C * lane + c) = make_float2(o[c], o[c + 1u]);
+                }
+            }
+            worker_sync<W * 32u>();   // (the memory is written again)
+        }
+        if (p.a == 0u && p.b < p.n) {
+            cut = true;
+            if (threadIdx.x == 0u) note_cut(pc, st, p, rows, done);
+        }
+    }
+    if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[2u * blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// Joins the cut row tiles: CTA x of the kernel in front whose last row tile goes on elsewhere has noted it; its parts lie in slot
+// 2 x + 1 and in slots 2 y of the CTAs behind. A warp per row where there are few parts, otherwise the warps share a row's parts.
+constexpr uint32_t kMergeWarps = 8;
+template <uint32_t C>
+__device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_t tile_rows, uint32_t chunk, uint32_t chunks) {
+    constexpr uint32_t D = 32u * C, ROW = D + 4u;
+    const uint4 note = pc.cut[2u * cta];
+    const uint32_t parts = note.x, tok0 = note.y, r0 = note.z, rows = note.w;
+    if (parts == 0u) return;
+    const uint32_t hkv = pc.cut[2u * cta + 1u].x;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    __shared__ float s_ml[kMergeWarps][2], s_o[kMergeWarps][D];
+    const bool shared = parts > 8u;   // the warps share the parts of a row
+    const uint32_t stride = shared ? chunks : chunks * kMergeWarps;
+    for (uint32_t r = shared ? chunk : chunk * kMergeWarps + warp; r < rows; r += stride) {
+        auto part = [&](uint32_t i) { return pc.slots + ((uint64_t)(i == 0u ? 2u * cta + 1u : 2u * (cta + i)) * tile_rows + r) * ROW; };
+        const uint32_t begin = shared ? warp : 0u, step = shared ? kMergeWarps : 1u;
+        float m = neg_inf();
+        for (uint32_t i = begin; i < parts; i += step) m = fmaxf(m, part(i)[0]);
+        float l = 0.0f, o[C];
+#pragma unroll
+        for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = begin; i < parts; i += step) {
+            const float* x = part(i);
+            const float f = weight(x[0], m);
+            l = fmaf(x[1], f, l);
+#pragma unroll
+            for (uint32_t c = 0; c < C; ++c) o[c] += f != 0.0f ? x[4u + C * lane + c] * f : 0.0f;
+        }
+        if (shared) {
+            if (lane == 0u) {
+                s_ml[warp][0] = m;
+                s_ml[warp][1] = l;
+            }
+#pragma unroll
+            for (uint32_t c = 0; c < C; ++c) s_o[warp][C * lane + c] = o[c];
+            __syncthreads();
+            if (warp == 0u) {
+                m = neg_inf();
+                for (uint32_t w = 0; w < kMergeWarps; ++w) m = fmaxf(m, s_ml[w][0]);
+                l = 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
+                for (uint32_t w = 0; w < kMergeWarps; ++w) {
+                    const float f = weight(s_ml[w][0], m);
+                    l = fmaf(s_ml[w][1], f, l);
+#pragma unroll
+                    for (uint32_t c = 0; c < C; ++c) o[c] += f != 0.0f ? s_o[w][C * lane + c] * f : 0.0f;
+                }
+            }
+            __syncthreads();
+            if (warp != 0u) continue;
+        }
+        const uint32_t row = r0 + r;
+        finish_row<C>(pc, tok0 + row / pc.G, hkv * pc.G + row % pc.G, m, l, o);
+    }
+}
+// CTAs 0 .. n_first - 1 join the tiles of `a`, the others those of `b`.
+template <uint32_t C>
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ Args a, const __grid_constant__ Args b, uint32_t n_first,
+                                                                       uint32_t rows_a, uint32_t rows_b) {
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.x < n_first) merge_tile<C>(a, blockIdx.x, rows_a, blockIdx.y, gridDim.y);
+    else merge_tile<C>(b, blockIdx.x - n_first, rows_b, blockIdx.y, gridDim.y);
+}
+
+template <int D, bool TOP, bool EXACT>
+static bool launch_rows_t(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
+    if (!ensure_dynamic_smem<paged_rows_kernel<D, TOP, EXACT>>((int)Rows<D>::smem(kMaxSeqs))) return false;
+    launch_pdl(paged_rows_kernel<D, TOP, EXACT>, dim3(ctas), dim3((Rows<D>::W + 1) * 32), Rows<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k,
+               maps.v, pc);
+    return true;
+}
+template <int D>
+static bool launch_rows_d(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
+    const bool top = (uint64_t)pc.max_q * pc.G <= 8u, exact = pc.out != OUT_F16;
+    return top ? (exact ? launch_rows_t<D, true, true>(a, pc, maps, ctas) : launch_rows_t<D, true, false>(a, pc, maps, ctas))
+               : (exact ? launch_rows_t<D, false, true>(a, pc, maps, ctas) : launch_rows_t<D, false, false>(a, pc, maps, ctas));
+}
+static bool launch_rows(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t D, uint32_t ctas) {
+    return D == 64u ? launch_rows_d<64>(a, pc, maps, ctas) : D == 128u ? launch_rows_d<128>(a, pc, maps, ctas) : launch_rows_d<256>(a, pc, maps, ctas);
+}
+
+static bool launch_merge(const LaunchArgs& a, const Args& x, const Args& y, uint32_t D, uint32_t n_x, uint32_t n_y, uint32_t rows_x, uint32_t rows_y) {
+    const dim3 grid(n_x + n_y, 4), block(kMergeWarps * 32);
+    if (D == 64u) launch_pdl(paged_merge_kernel<2>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
+    else if (D == 128u) launch_pdl(paged_merge_kernel<4>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
+    else launch_pdl(paged_merge_kernel<8>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
+    return true;
+}
+
+// [pages][heads][tokens][D] f16 with the caller's strides, boxes of `tokens` x 64 columns
+static bool encode_cache(tc::EncodeTiledFn enc, CUtensorMap* map, const void* ptr, const Args& pc, uint32_t D, uint32_t tokens) {
+    const uint32_t P = 1u << pc.page_log2;
+    const cuuint64_t dims[4] = {D, P, pc.n_head_kv, pc.n_pages};
+    // (the stride of a dimension of one element is never used, but has to be a valid one)
+    const cuuint64_t strides[3] = {2ull * pc.c_ts, pc.n_head_kv > 1u ? 2ull * pc.c_hs : 2ull * D, pc.n_pages > 1u ? 2ull * pc.c_ps : 2ull * D};
+    const cuuint32_t box[4] = {64, tokens, 1, 1}, estr[4] = {1, 1, 1, 1};
+    if (!strides[0] || !strides[1] || !strides[2]) return false;
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static float word_f(uint32_t u) {
+    float f;
+    memcpy(&f, &u, 4);
+    return f;
+}
+static bool meet(const LaunchArgs& a, uint32_t i, uint32_t j) {
+    const uintptr_t p = (uintptr_t)a.ptr[i], q = (uintptr_t)a.ptr[j];
+    return p < q + a.range[j] && q < p + a.range[i];
+}
+
+// What both entry points' arguments have in common: the first 18 push words and bindings 0 .. 8.
+static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
+    const uint32_t* w = a.push;
+    memset(&pc, 0, sizeof(pc));
+    D = w[0];
+    pc.n_head = w[1];
+    pc.n_head_kv = w[2];
+    pc.n_seqs = w[3];
+    pc.rows = w[4];
+    pc.max_q = w[5];
+    pc.max_kv = w[6];
+    const uint32_t P = w[7];
+    pc.n_pages = w[8];
+    pc.table_stride = w[9];
+    pc.c_ps = w[10];
+    pc.c_ts = w[11];
+    pc.c_hs = w[12];
+    pc.q_s = w[13];
+    pc.dst_s = w[14];
+    pc.out = w[15];
+    pc.scale = word_f(w[16]);
+    pc.softcap = word_f(w[17]);
+    pc.scale2 = pc.scale * kLog2e;
+    if (!D || !pc.n_head || !pc.n_head_kv || pc.n_head % pc.n_head_kv || !pc.n_seqs || !pc.rows || !pc.max_q || !pc.max_kv || !P || (P & (P - 1u)) ||
+        !pc.n_pages || !pc.table_stride || pc.out > OUT_F16 || !(pc.softcap >= 0.0f) || pc.scale != pc.scale)
+        return AC_ERR_KERNEL_ARG_INVALID;
+    pc.G = pc.n_head / pc.n_head_kv;
+    if ((D != 64u && D != 128u && D != 256u) || P < 16u || P > 1024u) return AC_ERR_FEATURE_NOT_SUPPORTED;
+    for (pc.page_log2 = 0; (1u << pc.page_log2) < P; ++pc.page_log2) {}
+    if (pc.n_seqs > kMaxSeqs || pc.n_head > 65535u || pc.rows > 0x7FFFFFFFu || pc.max_kv > 0x7FFFFFFFu - 1024u || pc.n_pages > 0x7FFFFFFFu ||
+        (uint64_t)pc.rows * pc.n_head > 0x7FFFFFFFull || (uint64_t)pc.table_stride * P > 0x7FFFFFFFull)
+        return AC_ERR_INVALID_SHAPE;
+    if (pc.max_q > pc.rows) pc.max_q = pc.rows;
+    if (((pc.c_ps | pc.c_ts | pc.c_hs | pc.q_s) & 7u) || (pc.dst_s & (pc.out == OUT_F16 ? 7u : 3u))) return AC_ERR_BUFFER_ALIGNMENT_INVALID;
+    for (uint32_t i : {0u, 1u, 2u, 6u, 7u})
+        if ((uintptr_t)a.ptr[i] & 15u) return AC_ERR_BUFFER_ALIGNMENT_INVALID;
+    for (uint32_t i : {3u, 4u, 5u, 8u})
+        if ((uintptr_t)a.ptr[i] & 3u) return AC_ERR_BUFFER_ALIGNMENT_INVALID;
+    const uint64_t last = pc.rows - 1u, width = (uint64_t)pc.n_head * D, esize = pc.out == OUT_F16 ? 2u : 4u;
+    const uint64_t cache = ((uint64_t)(pc.n_pages - 1u) * pc.c_ps + (uint64_t)(P - 1u) * pc.c_ts + (uint64_t)(pc.n_head_kv - 1u) * pc.c_hs + D) * 2u;
+    if (a.range[0] < (last * pc.q_s + width) * 2u || a.range[1] < cache || a.range[2] < cache ||
+        a.range[3] < (uint64_t)pc.n_seqs * pc.table_stride * 4u || a.range[4] < ((uint64_t)pc.n_seqs + 1u) * 4u || a.range[5] < (uint64_t)pc.n_seqs * 4u ||
+        a.range[6] < (last * pc.dst_s + width) * esize || a.range[8] < 8u)
+        return AC_ERR_INVALID_BUFFER_SIZE;
+    for (uint32_t o : {6u, 7u, 8u})   // what is written meets nothing else
+        for (uint32_t i = 0; i < a.binding_count; ++i)
+            if (i != o && meet(a, o, i)) return AC_ERR_KERNEL_ARG_INVALID;
+    pc.q = (const __half*)a.ptr[0];
+    pc.k = (const __half*)a.ptr[1];
+    pc.v = (const __half*)a.ptr[2];
+    pc.table = (const int32_t*)a.ptr[3];
+    pc.q_start = (const int32_t*)a.ptr[4];
+    pc.kv_len = (const int32_t*)a.ptr[5];
+    pc.dst = a.ptr[6];
+    pc.refused = (uint32_t*)a.ptr[8];
+    pc.status = a.status;
+    return AC_SUCCESS;
+}
+
+// Which kernel a sequence of R rows per KV head runs in: up to kFewRows in paged_rows_kernel, more in paged_tc.cu's (D 64, 128).
+constexpr uint32_t kFewRows = 64;
+
+struct Scratch {   // taken from the front
+    uint8_t* at;
+    uint64_t left;
+    void* take(uint64_t bytes) {
+        bytes = (bytes + 255u) & ~255ull;
+        if (bytes > left) return nullptr;
+        void* p = at;
+        at += bytes;
+        left -= bytes;
+        return p;
+    }
+};
+// CTAs for a kernel whose cut tiles take 2 * tile_bytes of scratch each: as many as the SMs, fewer where the scratch holds no more
+static uint32_t ctas_for(uint64_t room, uint64_t tile_bytes, uint32_t sms) {
+    const uint64_t n = room > 1024u ? (room - 1024u) / (2u * tile_bytes + 32u) : 0u;
+    return n < 1u ? 1u : n > sms ? sms : (uint32_t)n;
+}
+
+// One attention over one set of keys: the sequences of few rows, those of many, and the join of what both cut.
+static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t max_rows, Scratch scratch, const Maps& rows_maps, const Maps& tc_maps) {
+    const uint32_t sms = a.sm_count > 0 ? (uint32_t)a.sm_count : 148u;
+    const bool both = D <= 128u && max_rows > kFewRows;
+    const uint64_t row = (D + 4u) * 4u;
+    Args few = pc, many = pc;
+    few.min_rows = 1u;
+    few.max_rows = both ? kFewRows : 0xFFFFFFFFu;
+    many.min_rows = pc.prefix ? 1u : kFewRows + 1u;   // (a prefix has one number of rows, and one kernel)
+    many.max_rows = 0xFFFFFFFFu;
+    const bool use_few = !both || !pc.prefix, use_many = both;
+    // the line's length in 32 bits
+    const uint32_t keys = D == 256u ? 64u : 128u;
+    const uint64_t few_rows = both ? kFewRows : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs, tiles = ((uint64_t)pc.max_kv + keys - 1u) / keys + 1u;
+    if (use_few && seqs * pc.n_head_kv * ((few_rows + 15u) / 16u) * tiles > 0xFFFFFFFFull) return AC_ERR_INVALID_SHAPE;
+    if (use_many && seqs * pc.n_head_kv * ((max_rows + kTcRows - 1u) / kTcRows) * tiles > 0xFFFFFFFFull) return AC_ERR_INVALID_SHAPE;
+    uint32_t n_few = 0, n_many = 0;
+    if (use_few) {
+        n_few = ctas_for(use_many ? scratch.left / 8u : scratch.left, kDecRows * row, sms);
+        few.cut = (uint4*)scratch.take(n_few * 32ull);
+        few.slots = (float*)scratch.take(n_few > 1u ? 2ull * n_few * kDecRows * row : 0u);
+        if (!few.cut || !few.slots) n_few = 1u, few.cut = nullptr, few.slots = nullptr;
+    }
+    if (use_many) {
+        n_many = ctas_for(scratch.left, kTcRows * row, sms);
+        many.cut = (uint4*)scratch.take(n_many * 32ull);
+        many.slots = (float*)scratch.take(n_many > 1u ? 2ull * n_many * kTcRows * row : 0u);
+        if (!many.cut || !many.slots) n_many = 1u, many.cut = nullptr, many.slots = nullptr;
+    }
+    if (use_many && !launch_tc(a, many, tc_maps, D, n_many)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
+    if (use_few && !launch_rows(a, few, rows_maps, D, n_few)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
+    const uint32_t merge_few = n_few > 1u ? n_few : 0u, merge_many = n_many > 1u ? n_many : 0u;
+    if (merge_few + merge_many && !launch_merge(a, few, many, D, merge_few, merge_many, kDecRows, kTcRows)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
+    return check_launch();
+}
+
+static AcResult cache_maps(const LaunchArgs& a, const Args& pc, uint32_t D, Maps& rows_maps, Maps& tc_maps) {
+    tc::EncodeTiledFn enc = tc::encode_fn();
+    const uint32_t P = 1u << pc.page_log2, keys = D == 256u ? 64u : 128u, rows_box = P < keys ? P : keys, tc_box = P < kTcKeys ? P : kTcKeys;
+    if (!enc) return AC_ERR_DRIVER_SYMBOL_MISSING;
+    const bool ok = encode_cache(enc, &rows_maps.k, a.ptr[1], pc, D, rows_box) && encode_cache(enc, &rows_maps.v, a.ptr[2], pc, D, rows_box) &&
+                    encode_cache(enc, &tc_maps.k, a.ptr[1], pc, D, tc_box) && encode_cache(enc, &tc_maps.v, a.ptr[2], pc, D, tc_box);
+    return ok ? AC_SUCCESS : AC_ERR_INVALID_SHAPE;
+}
+
+}  // namespace paged
+
+// ameva_paged_attn: bindings 0 q f16, 1 k cache f16, 2 v cache f16, 3 table i32 [n_seqs][table_stride], 4 q_start i32 [n_seqs + 1],
+// 5 kv_len i32 [n_seqs], 6 dst f32 or f16, 7 scratch, 8 status (two words: count of refused entries, lowest node).
+// push: D (64, 128, 256), n_head, n_head_kv, n_seqs (<= 4095), rows of q and dst, most rows of a sequence, most keys of one, page size
+// (a power of two, 16 .. 1024), pages, table stride, cache strides of page, token and head, row strides of q and dst (in elements),
+// dst is f16, scale, softcap (0: none), window (0: none; otherwise a query sees that many keys, its own the last), node.
+// Query j of a sequence's n stands at place kv_len - n + j and sees the keys up to there; one that sees none is zero. Rows behind the
+// last sequence are left as they are. Sequences whose numbers do not fit the buffers or the announced maxima are left out, keys on
+// pages that are none of the cache's are not seen; both are counted. The results do not depend on the scratch's contents, and with the
+// same scratch size and maxima not on the run; a larger scratch (up to 2 x SMs x 272 rows) allows more CTAs.
+AcResult launch_paged_attn(const LaunchArgs& a) {
+    using namespace paged;
+    Args pc;
+    uint32_t D;
+    AcResult rc = read_args(a, pc, D);
+    if (rc != AC_SUCCESS) return rc;
+    pc.window = a.push[18];
+    pc.node = a.push[19];
+    Maps rows_maps, tc_maps;
+    rc = cache_maps(a, pc, D, rows_maps, tc_maps);
+    if (rc != AC_SUCCESS) return rc;
+    return launch_set(a, pc, D, (uint64_t)pc.max_q * pc.G, {(uint8_t*)a.ptr[7], a.range[7]}, rows_maps, tc_maps);
+}
+
+// ameva_paged_prefix_attn: the same for sequences that share a prefix, whose pages are read once for all of them. Binding 9: prefix i32
+// [1 + pages], its number of keys and its pages; kv_len and the tables are those of the sequences' own keys behind it. push words 18, 19:
+// most keys of the prefix, node; no window. The scratch holds rows x n_head x (D + 4) floats at least.
+AcResult launch_paged_prefix_attn(const LaunchArgs& a) {
+    using namespace paged;
+    Args pc;
+    uint32_t D;
+    AcResult rc = read_args(a, pc, D);
+    if (rc != AC_SUCCESS) return rc;
+    const uint32_t max_prefix = a.push[18];
+    pc.node = a.push[19];
+    if (!max_prefix) return AC_ERR_KERNEL_ARG_INVALID;
+    if (max_prefix > 0x7FFFFFFFu - 1024u) return AC_ERR_INVALID_SHAPE;
+    if ((uintptr_t)a.ptr[9] & 3u) return AC_ERR_BUFFER_ALIGNMENT_INVALID;
+    if (a.range[9] < 4u + 4ull * (((uint64_t)max_prefix + (1u << pc.page_log2) - 1u) >> pc.page_log2)) return AC_ERR_INVALID_BUFFER_SIZE;
+    Maps rows_maps, tc_maps;
+    rc = cache_maps(a, pc, D, rows_maps, tc_maps);
+    if (rc != AC_SUCCESS) return rc;
+    Scratch scratch = {(uint8_t*)a.ptr[7], a.range[7]};
+    float* own = (float*)scratch.take((uint64_t)pc.rows * pc.n_head * (D + 4u) * 4u);
+    if (!own) return AC_ERR_INVALID_BUFFER_SIZE;
+    Args first = pc;   // the sequences' own keys
+    first.dst = own;
+    first.out = OUT_PARTS;
+    rc = launch_set(a, first, D, (uint64_t)pc.max_q * pc.G, scratch, rows_maps, tc_maps);
+    if (rc != AC_SUCCESS) return rc;
+    pc.extra = own;    // the prefix, for all rows at once, with those taken in
+    pc.prefix = (const int32_t*)a.ptr[9];
+    pc.max_own_q = pc.max_q;
+    pc.max_own_kv = pc.max_kv;
+    pc.max_q = pc.rows;
+    pc.max_kv = max_prefix;
+    return launch_set(a, pc, D, (uint64_t)pc.rows * pc.G, scratch, rows_maps, tc_maps);
+}
+
+}  // namespace amv

@@ -1,0 +1,516 @@
+// Attention over a paged KV cache for many rows per sequence (prompts, the shared prefix of a batch; D 64, 128) on the 5th-generation
+// tensor cores. Arguments, rows and the line of work: paged.cuh; launchers: paged_attn.cu.
+//
+// A CTA (one per SM) takes row tiles of 256 rows, two groups of 128, and walks key tiles of 128 for both:
+//   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 128 scores from tensor memory, online softmax to base 2, write P
+//                    over the scores as f16 (and, for a 32-bit result, what that rounding left beside it). The accumulator is rescaled
+//                    only when a row's maximum has grown by more than 2^kGrowth since its last rescale. They also bring Q of the next
+//                    piece into shared memory while the last P V runs, and write the piece's results.
+//   warp 8           issues the MMAs: S = Q K^T (both in shared memory), O += P V (P in tensor memory, V MN-major): P V of a group and
+//                    its next S leave together, so that the tensor core works on one group while the other's softmax runs
+//   warp 9           streams K and V tiles with TMA, a box of 64 columns x one page each
+// Tensor memory: two S / P of 128 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
+// steps of 16 keys that none sees; V rows behind the last key are zeroed before they are multiplied (a page holds anything there).
+// Every wait on a barrier is bounded (sync_ptx.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
+#include <cstring>
+
+#include "paged.h"
+#include "sync_ptx.cuh"
+#include "tcgen05_ptx.cuh"
+
+namespace amv {
+namespace paged {
+
+using namespace ptx;
+using namespace tc;
+
+constexpr uint32_t kGroupRows = 128, kWarpMma = 8, kWarpLoad = 9, kTcThreads = 320, kTmemCols = 512, kBadRing = 8;
+constexpr float kGrowth = 7.0f;   // probabilities stay below 2^7
+
+template <int D>
+struct Tc {
+    static constexpr uint32_t A = D / 64, STAGES = D == 64 ? 4 : 2;
+    static constexpr uint32_t Q = A * kGroupRows * 128u, TILE = A * kTcKeys * 128u;
+    static constexpr uint32_t FIXED = 1024u + 2u * Q + 2u * STAGES * TILE + 512u;
+    static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
+};
+
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map),
+        "r"(bar), "r"(column), "r"(token), "r"(head), "r"(page)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31, %32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+        "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Descriptor of a V tile as the B operand with its columns (N) contiguous: 64-column groups of the 128-byte swizzle
+// kTcKeys * 128 bytes apart (leading offset), groups of eight keys 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t v_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(kTcKeys * 128u >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// A group's share of a piece: its rows, the keys any of them sees and those all of them see, its key tiles [t0, t1).
+struct Group {
+    uint32_t r0, rows, lo, hi, lo_all, hi_all, t0, t1;
+};
+__device__ __forceinline__ Group group_of(const Args& pc, const Piece& p, uint32_t g) {
+    Group x;
+    x.r0 = p.r0 + g * kGroupRows;
+    x.rows = p.R > x.r0 ? min(kGroupRows, p.R - x.r0) : 0u;
+    x.lo = x.hi = x.lo_all = x.hi_all = x.t0 = x.t1 = 0u;
+    if (x.rows) {
+        const Span a = row_span(pc, p.q, x.r0), b = row_span(pc, p.q, x.r0 + x.rows - 1u);
+        x.lo = a.lo;
+        x.hi = b.hi;
+        x.lo_all = b.lo;
+        x.hi_all = a.hi;
+        x.t0 = max(p.first + p.a, x.lo / kTcKeys);
+        x.t1 = x.hi > x.lo ? min(p.first + p.b, (x.hi + kTcKeys - 1u) / kTcKeys) : x.t0;
+        if (x.t1 < x.t0) x.t1 = x.t0;
+    }
+    return x;
+}
+
+template <int D, bool EXACT>
+__global__ void __launch_bounds__(kTcThreads, 1)
+paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args pc) {
+    using L = Tc<D>;
+    constexpr uint32_t A = L::A, ST = L::STAGES, C = D / 32;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t *sQ = base, *sK = sQ + 2u * L::Q, *sV = sK + ST * L::TILE;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * L::TILE);
+    const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST,
+                   q_full = v_empty + 8u * ST, s_full = q_full + 16u, p_full = s_full + 16u, pv_done = p_full + 16u, drain = pv_done + 16u;
+    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 4u * ST + 9u);
+    uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                   // [10]
+    volatile uint32_t* s_bad = s_warp + kTcThreads / 32u;                      // 16-key steps whose page is none, of the last key tiles
+    uint32_t* s_pref = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + 512u);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < ST; ++s) {
+            mbar_init(k_full + 8u * s, 1u);
+            mbar_init(k_empty + 8u * s, 1u);
+            mbar_init(v_full + 8u * s, 1u);
+            mbar_init(v_empty + 8u * s, 1u);
+        }
+        for (uint32_t g = 0; g < 2u; ++g) {
+            mbar_init(q_full + 8u * g, 4u);
+            mbar_init(s_full + 8u * g, 1u);
+            mbar_init(p_full + 8u * g, 4u);
+            mbar_init(pv_done + 8u * g, 1u);
+        }
+        mbar_init(drain, 1u);
+        ctl->abort = 0u;
+        fence_barrier_init();
+    }
+    // boxes that no row needs are not loaded: their steps are not multiplied, but a zero is a better guest than a NaN
+    for (uint32_t i = threadIdx.x; i < 2u * ST * L::TILE / 16u; i += kTcThreads) reinterpret_cast<uint4*>(sK)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (warp == kWarpMma) tmem_alloc<false>(smem_u32(&ctl->tmem_base), kTmemCols);
+    fence_async_smem();
+    pdl_wait();
+    tc_fence_before();
+    const uint32_t total = build_line<kTcRows, kTcKeys, kTcThreads / 32u>(pc, s_pref, s_warp);   // (its barriers publish the above)
+    tc_fence_after();
+    pdl_trigger();   // not before the tensor memory is this CTA's
+    const uint32_t tmem = ctl->tmem_base;
+    const Stretch st = my_stretch(total);
+    Walk<kTcRows, kTcKeys> walk(st);
+    const uint32_t P = 1u << pc.page_log2, box = P < kTcKeys ? P : kTcKeys, boxes = kTcKeys / box;
+    bool ok = true;
+
+    if (warp == kWarpLoad) {
+        Ring kr(ST), vr(ST);
+        uint32_t tiles = 0;     // of this CTA so far
+        uint32_t k_issued = 0, v_issued = 0;
+        while (ok && walk.next(pc, s_pref)) {
+            const Piece& p = walk.p;
+            const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + kTcRows, p.R) - 1u).hi;
+            for (uint32_t i = p.a; i < p.b; ++i, ++tiles) {
+                const uint32_t key0 = (p.first + i) * kTcKeys, b0 = key0 + lane * box;
+                int32_t page = -1;
+                const bool want = lane < boxes && b0 < hi && b0 + box > lo;
+                if (want) page = page_of(pc, p.q, b0);
+                const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0), load = __ballot_sync(0xffffffffu, want && page >= 0);
+                uint32_t bad = 0;
+                if (none) {
+                    for (uint32_t j = 0; j < kTcKeys / 16u; ++j) bad |= (none >> (16u * j / box) & 1u) << j;
+                    if (lane == 0u) refuse(pc, __popc(none));
+                }
+                const uint32_t bytes = (uint32_t)__popc(load) * box * 128u * A;
+                for (uint32_t kv = 0; kv < 2u; ++kv) {
+                    Ring& r = kv ? vr : kr;
+                    const uint32_t full = (kv ? v_full : k_full) + 8u * r.idx, empty = (kv ? v_empty : k_empty) + 8u * r.idx;
+                    ok = mbar_wait(empty, r.phase ^ 1u, ctl, pc.status, kv ? 0xD10u : 0xD00u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0u) {
+                        if (!kv) s_bad[tiles & (kBadRing - 1u)] = bad;
+                        mbar_arrive_expect_tx(full, bytes);
+                    }
+                    __syncwarp();
+                    const uint32_t stage = smem_u32((kv ? sV : sK) + r.idx * L::TILE);
+                    if (lane < boxes && (load >> lane & 1u))
+                        for (uint32_t a = 0; a < A; ++a)
+                            tma_box(stage + a * (kTcKeys * 128u) + lane * box * 128u, kv ? &v_map : &k_map, full, (int)(64u * a), (int)(b0 & (P - 1u)),
+                                    (int)p.hkv, page);
+                    if (kv) ++v_issued;
+                    else ++k_issued;
+                    r.advance();
+                }
+                if (!ok) break;
+            }
+        }
+        if (ctl->abort) {   // copies already requested finish before the CTA leaves
+            for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) mbar_wait(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
+            for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) mbar_wait(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
+        }
+    } else if (warp == kWarpMma) {
+        const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
+        Ring kr(ST), vr(ST);
+        uint32_t tiles = 0, q_uses[2] = {0u, 0u}, p_uses[2] = {0u, 0u};
+        while (ok && walk.next(pc, s_pref)) {
+            const Piece& p = walk.p;
+            const Group grp[2] = {group_of(pc, p, 0u), group_of(pc, p, 1u)};
+            const uint32_t hi_all = max(grp[0].hi, grp[1].hi), T0 = p.first + p.a, T1 = p.first + p.b;
+            bool started[2] = {false, false};
+            // step u: P V of key tile u - 1 and S of key tile u, group by group
+            for (uint32_t u = T0; u <= T1 && ok; ++u) {
+                bool have_k = false, have_v = false;
+                uint32_t steps = 0xFFu;   // 16-key steps of tile u - 1 whose pages are there
+                if (u > T0) steps = ~s_bad[(tiles + (u - 1u - T0)) & (kBadRing - 1u)];
+#pragma unroll
+                for (uint32_t g = 0; g < 2u; ++g) {
+                    const Group& x = grp[g];
+                    if (u > T0 && u - 1u >= x.t0 && u - 1u < x.t1) {
+                        const uint32_t key0 = (u - 1u) * kTcKeys;
+                        if (!have_v) {
+                            ok = ok && mbar_wait<false>(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
+                            have_v = true;
+                            if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
+                                const uint32_t from = hi_all - key0, n = (16u - (from & 15u)) & 15u;
+                                for (uint32_t j = lane; j < n * (D / 8u); j += 32u) {
+                                    const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
+                                    *reinterpret_cast<uint4*>(sV + vr.idx * L::TILE + (c >> 3) * (kTcKeys * 128u) + r * 128u + ((c & 7u) << 4)) =
+                                        make_uint4(0u, 0u, 0u, 0u);
+                                }
+                                fence_async_smem();
+                                __syncwarp();
+                            }
+                        }
+                        ok = ok && mbar_wait<false>(p_full + 8u * g, p_uses[g] & 1u, ctl, pc.status, 0xD50u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        ++p_uses[g];
+                        tc_fence_after();
+                        const uint32_t s0 = x.lo > key0 ? (x.lo - key0) / 16u : 0u, s1 = (min(x.hi - key0, kTcKeys) + 15u) / 16u;
+                        if (lane == 0u) {
+                            const uint64_t dv = v_desc(smem_u32(sV + vr.idx * L::TILE));
+                            uint32_t acc = started[g];
+#pragma unroll
+                            for (uint32_t k = 0; k < kTcKeys / 16u; ++k) {   // 16 keys: 8 columns of P, two groups of eight V rows
+                                if (k < s0 || k >= s1 || !(steps >> k & 1u)) continue;
+                                const uint32_t ta = tmem + g * kTcKeys + 8u * k, to = tmem + 2u * kTcKeys + g * D;
+                                umma_ts<false, false>(to, ta, dv + 128u * k, idesc_o, acc);
+                                if (EXACT) umma_ts<false, false>(to, ta + 64u, dv + 128u * k, idesc_o, 1u);
+                                acc = 1u;
+                            }
+                            started[g] = acc;
+                            if (u == x.t1) umma_commit<false>(pv_done + 8u * g);
+                        }
+                    }
+                    if (u < T1 && u >= x.t0 && u < x.t1) {
+                        if (!have_k) ok = ok && mbar_wait<false>(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
+                        have_k = true;
+                        if (u == x.t0) {
+                            ok = ok && mbar_wait<false>(q_full + 8u * g, q_uses[g] & 1u, ctl, pc.status, 0xD70u);
+                            ++q_uses[g];
+                        }
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (lane == 0u) {
+#pragma unroll
+                            for (uint32_t a = 0; a < A; ++a) {
+                                const uint64_t da = make_smem_desc(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)));
+                                const uint64_t db = make_smem_desc(smem_u32(sK + kr.idx * L::TILE + a * (kTcKeys * 128u)));
+#pragma unroll
+                                for (uint32_t k = 0; k < 4u; ++k)
+                                    umma_ss_f16(tmem + g * kTcKeys, da + 2u * k, db + 2u * k, idesc_s, (uint32_t)((a | k) != 0u));
+                            }
+                            umma_commit<false>(s_full + 8u * g);
+                        }
+                    }
+                }
+                if (!ok) break;
+                if (u > T0) {   // (a tile that neither group sees is given back, too)
+                    if (!have_v) ok = mbar_wait<false>(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD80u);
+                    if (lane == 0u) umma_commit<false>(v_empty + 8u * vr.idx);
+                    vr.advance();
+                }
+                if (u < T1) {
+                    if (!have_k) ok = ok && mbar_wait<false>(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD90u);
+                    if (lane == 0u) umma_commit<false>(k_empty + 8u * kr.idx);
+                    kr.advance();
+                }
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            tiles += p.b - p.a;
+        }
+        if (ctl->abort && lane == 0u) {   // MMAs already issued finish before the CTA leaves
+            umma_commit<false>(drain);
+            for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain, 0u); ++spins) __nanosleep(64);
+        }
+    } else {
+        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, ts = tmem + lanes + g * kTcKeys, to = tmem + lanes + 2u * kTcKeys + g * D;
+        uint32_t s_uses = 0, pv_uses = 0, tiles = 0, at = st.begin;
+        bool cut = false;
+        // Q rows of a piece into the K-major 128-byte swizzle, a warp its own 32 rows, idle rows zero
+        auto load_q = [&](const Piece& p, const Group& x) {
+            constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
+#pragma unroll 8
+            for (uint32_t i = 0; i < 32u / PER; ++i) {
+                const uint32_t r = (warp & 3u) * 32u + i * PER + lane / PIECES, c = lane % PIECES, row = x.r0 + r;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (r < x.rows)
+                    v = *reinterpret_cast<const uint4*>(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.hkv * pc.G + row % pc.G) * D + 8u * c);
+                *reinterpret_cast<uint4*>(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u) + r * 128u + (((c & 7u) ^ (r & 7u)) << 4)) = v;
+            }
+            fence_async_smem();   // the MMAs read Q through the async proxy
+            __syncwarp();
+            if (lane == 0u) mbar_arrive(q_full + 8u * g);
+        };
+        bool have = walk.next(pc, s_pref);
+        Group x = {};
+        if (have) {
+            x = group_of(pc, walk.p, g);
+            if (x.t1 > x.t0) load_q(walk.p, x);
+        }
+        while (have) {
+            const Piece p = walk.p;
+            const uint32_t my = threadIdx.x & 127u, row = x.r0 + my;
+            const bool valid = my < x.rows;
+            const Span span = valid ? row_span(pc, p.q, row) : Span{0u, 0u};
+            float m_run = neg_inf(), l_run = 0.0f;
+            for (uint32_t t = x.t0; t < x.t1; ++t) {
+                const uint32_t key0 = t * kTcKeys;
+                ok = ok && mbar_wait(s_full + 8u * g, s_uses & 1u, ctl, pc.status, 0xDA0u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ++s_uses;
+                tc_fence_after();
+                const uint32_t gone = s_bad[(tiles + (t - p.first - p.a)) & (kBadRing - 1u)];
+                float s[kTcKeys];
+#pragma unroll
+                for (uint32_t c = 0; c < kTcKeys; c += 32u) tmem_ld32_async(ts + c, reinterpret_cast<uint32_t*>(s) + c);
+                tmem_wait_ld();
+                // the same for every thread of the group
+                const bool plain = gone == 0u && key0 >= x.lo_all && key0 + kTcKeys <= x.hi_all && pc.softcap == 0.0f && pc.scale2 > 0.0f;
+                float mx = neg_inf();
+                if (plain) {
+                    float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+                    for (uint32_t k = 0; k < kTcKeys; ++k) m4[k & 3u] = fmaxf(m4[k & 3u], s[k]);
+                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * pc.scale2;
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < kTcKeys; ++k) {
+                        const uint32_t key = key0 + k;
+                        s[k] = key >= span.lo && key < span.hi && !(gone >> (k >> 4) & 1u) ? score2(pc, s[k]) : neg_inf();
+                        mx = fmaxf(mx, s[k]);
+                    }
+                }
+                const bool grow = mx > m_run + kGrowth || (m_run == neg_inf() && mx != neg_inf());
+                if (__any_sync(0xffffffffu, grow)) {   // (no P V of this group is on its way: S of this tile was issued behind the last)
+                    const float f = !grow ? 1.0f : weight(m_run, mx);
+                    if (grow) m_run = mx;
+                    l_run *= f;
+                    if (t != x.t0) {
+#pragma unroll 1
+                        for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
+                            uint32_t v[32];
+                            tmem_ld32_async(to + c, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                            tmem_st32_async(to + c, v);
+                        }
+                    }
+                }
+                const float ref = m_run == neg_inf() ? 0.0f : m_run, mul = plain ? pc.scale2 : 1.0f;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t half = 0; half < 2u; ++half) {
+                    uint32_t ph[32], pl[32];
+#pragma unroll
+                    for (uint32_t k = 0; k < 32u; ++k) {
+                        const float s0 = s[64u * half + 2u * k], s1 = s[64u * half + 2u * k + 1u];
+                        // (the difference by one rounding where the scores are scaled here, of rounded scores otherwise)
+                        const float p0 = ex2(plain ? fmaf(s0, mul, -ref) : s0 - ref), p1 = ex2(plain ? fmaf(s1, mul, -ref) : s1 - ref);
+                        sum[(2u * k) & 3u] += p0;
+                        sum[(2u * k + 1u) & 3u] += p1;
+                        const __half2 h = __floats2half2_rn(p0, p1);
+                        ph[k] = *reinterpret_cast<const uint32_t*>(&h);
+                        if (EXACT) {
+                            const float2 f2 = __half22float2(h);
+                            const __half2 low = __floats2half2_rn(p0 - f2.x, p1 - f2.y);
+                            pl[k] = *reinterpret_cast<const uint32_t*>(&low);
+                        }
+                    }
+                    tmem_st32_async(ts + 32u * half, ph);   // over this tile's scores
+                    if (EXACT) tmem_st32_async(ts + 64u + 32u * half, pl);
+                }
+                l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(p_full + 8u * g);
+            }
+            // Q of the next piece: S of this one's last tile has been read, so its Q is free
+            const Group cur = x;
+            have = walk.next(pc, s_pref);
+            if (have) {
+                x = group_of(pc, walk.p, g);
+                if (ok && x.t1 > x.t0) load_q(walk.p, x);
+            }
+            // ---- results of this piece ----
+            const bool some = cur.t1 > cur.t0, whole = p.a == 0u && p.b == p.n;
+            if (some) {
+                ok = ok && mbar_wait(pv_done + 8u * g, pv_uses & 1u, ctl, pc.status, 0xDB0u) && !ctl->abort;
+                ++pv_uses;
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            tiles += p.b - p.a;
+            at += p.b - p.a;
+            if (cur.rows) {
+                const uint32_t token = p.q.tok0 + row / pc.G, head = p.hkv * pc.G + row % pc.G;
+                float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * kTcRows + (cur.r0 - p.r0)) * (D + 4u);
+                const bool parts = !whole || pc.out == OUT_PARTS;
+                float own = 1.0f, other = 0.0f;      // factors of the values here and of those over other keys
+                const float* extra = nullptr;
+                void* dst = nullptr;
+                if (valid) {
+                    if (parts) {
+                        float* r = whole ? reinterpret_cast<float*>(pc.dst) + dst_row(pc, token, head, D) : slot + (uint64_t)my * (D + 4u);
+                        *reinterpret_cast<float2*>(r) = make_float2(m_run, l_run);
+                        dst = r + 4;
+                    } else {
+                        float l = l_run, f = 1.0f;
+                        if (pc.extra) {
+                            extra = pc.extra + ((uint64_t)token * pc.n_head + head) * (D + 4u);
+                            const float2 ml = *reinterpret_cast<const float2*>(extra);
+                            const float top = fmaxf(m_run, ml.x);
+                            f = weight(m_run, top);
+                            other = weight(ml.x, top);
+                            l = l * f + ml.y * other;
+                            if (other == 0.0f) extra = nullptr;
+                        }
+                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                        own = f * inv;
+                        other *= inv;
+                        const uint64_t e = dst_row(pc, token, head, D);
+                        dst = pc.out == OUT_F16 ? (void*)(reinterpret_cast<__half*>(pc.dst) + e) : (void*)(reinterpret_cast<float*>(pc.dst) + e);
+                    }
+                }
+                const bool nothing = l_run == 0.0f;   // nothing was accumulated, or only what zeros made
+                float check = 0.0f;
+#pragma unroll 1
+                for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
+                    uint32_t v[32];
+                    if (some) {
+                        tmem_ld32_async(to + c, v);
+                        tmem_wait_ld();
+                    }
+                    float y[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float o = nothing || !some ? 0.0f : __uint_as_float(v[j]);
+                        check = fmaf(o, 0.0f, check);
+                        y[j] = own == 0.0f ? 0.0f : o * own;
+                    }
+                    if (valid) {
+                        if (extra) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const float4 e = *reinterpret_cast<const float4*>(extra + 4u + c + j);
+                                y[j] = fmaf(e.x, other, y[j]);
+                                y[j + 1] = fmaf(e.y, other, y[j + 1]);
+                                y[j + 2] = fmaf(e.z, other, y[j + 2]);
+                                y[j + 3] = fmaf(e.w, other, y[j + 3]);
+                            }
+                        }
+                        if (!parts && pc.out == OUT_F16) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 8) {
+                                uint4 h;
+                                __half2 h2[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) h2[k] = __floats2half2_rn(y[j + 2 * k], y[j + 2 * k + 1]);
+                                memcpy(&h, h2, 16);
+                                *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(dst) + c + j) = h;
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4)
+                                *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + c + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                        }
+                    }
+                }
+                __syncwarp();
+                // rows that are not finite although their sum is: over the keys they see, by the whole warp
+                for (uint32_t again = __ballot_sync(0xffffffffu, valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
+                    const int i = __ffs(again) - 1;
+                    const uint32_t r = cur.r0 + (warp & 3u) * 32u + (uint32_t)i, tk = p.q.tok0 + r / pc.G, hd = p.hkv * pc.G + r % pc.G;
+                    const float m = __shfl_sync(0xffffffffu, m_run, i), l = __shfl_sync(0xffffffffu, l_run, i);
+                    const Span sp = row_span(pc, p.q, r);
+                    float o[C];
+                    seen_keys_row<C>(pc, p.q, p.hkv, pc.q + (uint64_t)tk * pc.q_s + (uint64_t)hd * D, max(sp.lo, (p.first + p.a) * kTcKeys),
+                                     min(sp.hi, (p.first + p.b) * kTcKeys), m == neg_inf() ? 0.0f : m, o);
+                    if (whole) {
+                        finish_row<C>(pc, tk, hd, m, l, o);
+                    } else {
+                        float* to_row = slot + (uint64_t)(r - cur.r0) * (D + 4u) + 4u + C * lane;
+#pragma unroll
+                        for (uint32_t c = 0; c < C; ++c) to_row[c] = o[c];
+                    }
+                }
+            }
+            if (p.a == 0u && p.b < p.n) {
+                cut = true;
+                if (threadIdx.x == 0u) note_cut(pc, st, p, min(kTcRows, p.R - p.r0), at);
+            }
+            tc_fence_before();   // (the next P V overwrites the accumulator behind an arrival of this thread)
+        }
+        if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[2u * blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kWarpMma) tmem_dealloc<false>(tmem, kTmemCols);
+}
+
+template <int D, bool EXACT>
+static bool launch_tc_t(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
+    if (!ensure_dynamic_smem<paged_tc_kernel<D, EXACT>>((int)Tc<D>::smem(kMaxSeqs))) return false;
+    launch_pdl(paged_tc_kernel<D, EXACT>, dim3(ctas), dim3(kTcThreads), Tc<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, pc);
+    return true;
+}
+
+bool launch_tc(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t head_dim, uint32_t ctas) {
+    const bool exact = pc.out != OUT_F16;
+    return head_dim == 64u ? (exact ? launch_tc_t<64, true>(a, pc, maps, ctas) : launch_tc_t<64, false>(a, pc, maps, ctas))
+                           : (exact ? launch_tc_t<128, true>(a, pc, maps, ctas) : launch_tc_t<128, false>(a, pc, maps, ctas));
+}
+
+}  // namespace paged
+}  // namespace amv
