@@ -411,7 +411,7 @@ def test_serving_steps_replayed(ctx):
         batch = ctx.batch(8)
         paged.record_append(batch, cache, seqs, b["q"], b["k"], b["v"], b["qr"], b["status"], heads=H, rope=paged.Rope(D, theta))
         paged.record_attention(batch, cache, seqs, b["qr"], b["out"], b["scratch"], b["status"], heads=H, scale=D ** -0.5)
-        paged.record_prefix_attention(batch, cache, seqs, b["qr"], b["out_p"], b["scratch"], b["status"], prefix=b["prefix"], max_prefix=64,
+        paged.record_prefix_attention(batch, cache, seqs, b["qr"], b["out_p"], b["scratch"], b["status"], prefix=b["prefix"], max_prefix=48,
                                       heads=H, scale=D ** -0.5, f16_out=True)
         batch.instantiate()
         return b, batch
