@@ -41,7 +41,7 @@ struct Args {
     uint32_t n_head, n_head_kv, G;
     uint32_t c_ps, c_ts, c_hs;  // cache strides in elements: page, token, head
     uint32_t q_s, dst_s, out, node, window, min_rows, max_rows;   // a launch serves the sequences of min_rows .. max_rows rows
-    float scale, softcap, scale2;                                 // scale2: scale * log2(e)
+    float scale, softcap, scale2, cap_in, cap_out;                // scale2: scale * log2(e); 2 log2(e) scale / softcap, softcap * log2(e)
 };
 
 struct Seq {

@@ -348,7 +348,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 }
 
 // Joins the cut row tiles: CTA x of the kernel in front whose last row tile goes on elsewhere has noted it; its parts lie in slot
-// 2 x + 1 and in slots 2 y of the CTAs behind. A warp per row where there are few parts, otherwise the warps share a row's parts.
+// 2 x + 1 and in slots 2 y of the CTAs behind. SHARE warps take the parts of a row in turn, the more the more parts there are; the
+// CTAs of one x share the rows.
 constexpr uint32_t kMergeWarps = 8;
 template <uint32_t C>
 __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_t tile_rows, uint32_t chunk, uint32_t chunks) {
@@ -359,25 +360,50 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
     const uint32_t hkv = pc.cut[2u * cta + 1u].x;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     __shared__ float s_ml[kMergeWarps][2], s_o[kMergeWarps][D];
-    const bool shared = parts > 8u;   // the warps share the parts of a row
-    const uint32_t stride = shared ? chunks : chunks * kMergeWarps;
-    for (uint32_t r = shared ? chunk : chunk * kMergeWarps + warp; r < rows; r += stride) {
-        auto part = [&](uint32_t i) { return pc.slots + ((uint64_t)(i == 0u ? 2u * cta + 1u : 2u * (cta + i)) * tile_rows + r) * ROW; };
-        const uint32_t begin = shared ? warp : 0u, step = shared ? kMergeWarps : 1u;
-        float m = neg_inf();
-        for (uint32_t i = begin; i < parts; i += step) m = fmaxf(m, part(i)[0]);
-        float l = 0.0f, o[C];
+    const uint32_t share = parts <= 8u ? 1u : parts <= 16u ? 2u : parts <= 32u ? 4u : kMergeWarps, at_once = kMergeWarps / share;
+    const uint32_t begin = warp % share;
+    for (uint32_t base = chunk * at_once; base < rows; base += chunks * at_once) {
+        const uint32_t r = base + warp / share;
+        float m = neg_inf(), l = 0.0f, o[C];
 #pragma unroll
         for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
-#pragma unroll 4
-        for (uint32_t i = begin; i < parts; i += step) {
-            const float* x = part(i);
-            const float f = weight(x[0], m);
-            l = fmaf(x[1], f, l);
+        if (r < rows) {
+            auto part = [&](uint32_t i) { return pc.slots + ((uint64_t)(i == 0u ? 2u * cta + 1u : 2u * (cta + i)) * tile_rows + r) * ROW; };
+            float x[8][C], ml[8][2];   // eight parts on their way together
+            for (uint32_t i0 = begin; i0 < parts; i0 += 8u * share) {
+                float top = m;
 #pragma unroll
-            for (uint32_t c = 0; c < C; ++c) o[c] += f != 0.0f ? x[4u + C * lane + c] * f : 0.0f;
+                for (uint32_t j = 0; j < 8u; ++j) {
+                    const uint32_t i = i0 + j * share;
+                    const bool have = i < parts;
+                    const float* p = part(have ? i : begin);
+                    const float2 v = *reinterpret_cast<const float2*>(p);
+                    ml[j][0] = have ? v.x : neg_inf();
+                    ml[j][1] = have ? v.y : 0.0f;
+#pragma unroll
+                    for (uint32_t c = 0; c < C; c += 2u) {
+                        const float2 y = *reinterpret_cast<const float2*>(p + 4u + C * lane + c);
+                        x[j][c] = y.x;
+                        x[j][c + 1u] = y.y;
+                    }
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) top = fmaxf(top, ml[j][0]);
+                const float f0 = weight(m, top);
+                m = top;
+                l *= f0;
+#pragma unroll
+                for (uint32_t c = 0; c < C; ++c) o[c] *= f0;
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) {
+                    const float f = weight(ml[j][0], top);
+                    l = fmaf(ml[j][1], f, l);
+#pragma unroll
+                    for (uint32_t c = 0; c < C; ++c) o[c] += f != 0.0f ? x[j][c] * f : 0.0f;
+                }
+            }
         }
-        if (shared) {
+        if (share > 1u) {
             if (lane == 0u) {
                 s_ml[warp][0] = m;
                 s_ml[warp][1] = l;
@@ -385,13 +411,13 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
 #pragma unroll
             for (uint32_t c = 0; c < C; ++c) s_o[warp][C * lane + c] = o[c];
             __syncthreads();
-            if (warp == 0u) {
+            if (begin == 0u && r < rows) {
                 m = neg_inf();
-                for (uint32_t w = 0; w < kMergeWarps; ++w) m = fmaxf(m, s_ml[w][0]);
+                for (uint32_t w = warp; w < warp + share; ++w) m = fmaxf(m, s_ml[w][0]);
                 l = 0.0f;
 #pragma unroll
                 for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
-                for (uint32_t w = 0; w < kMergeWarps; ++w) {
+                for (uint32_t w = warp; w < warp + share; ++w) {
                     const float f = weight(s_ml[w][0], m);
                     l = fmaf(s_ml[w][1], f, l);
 #pragma unroll
@@ -399,10 +425,12 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
                 }
             }
             __syncthreads();
-            if (warp != 0u) continue;
+            if (begin != 0u) continue;
         }
-        const uint32_t row = r0 + r;
-        finish_row<C>(pc, tok0 + row / pc.G, hkv * pc.G + row % pc.G, m, l, o);
+        if (r < rows) {
+            const uint32_t row = r0 + r;
+            finish_row<C>(pc, tok0 + row / pc.G, hkv * pc.G + row % pc.G, m, l, o);
+        }
     }
 }
 // CTAs 0 .. n_first - 1 join the tiles of `a`, the others those of `b`.
@@ -433,7 +461,7 @@ static bool launch_rows(const LaunchArgs& a, const Args& pc, const Maps& maps, u
 }
 
 static bool launch_merge(const LaunchArgs& a, const Args& x, const Args& y, uint32_t D, uint32_t n_x, uint32_t n_y, uint32_t rows_x, uint32_t rows_y) {
-    const dim3 grid(n_x + n_y, 4), block(kMergeWarps * 32);
+    const dim3 grid(n_x + n_y, n_y ? 16 : 4), block(kMergeWarps * 32);
     if (D == 64u) launch_pdl(paged_merge_kernel<2>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
     else if (D == 128u) launch_pdl(paged_merge_kernel<4>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
     else launch_pdl(paged_merge_kernel<8>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
@@ -485,6 +513,10 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
     pc.scale = word_f(w[16]);
     pc.softcap = word_f(w[17]);
     pc.scale2 = pc.scale * kLog2e;
+    if (pc.softcap > 0.0f) {
+        pc.cap_in = 2.0f * kLog2e * pc.scale / pc.softcap;
+        pc.cap_out = pc.softcap * kLog2e;
+    }
     if (!D || !pc.n_head || !pc.n_head_kv || pc.n_head % pc.n_head_kv || !pc.n_seqs || !pc.rows || !pc.max_q || !pc.max_kv || !P || (P & (P - 1u)) ||
         !pc.n_pages || !pc.table_stride || pc.out > OUT_F16 || !(pc.softcap >= 0.0f) || pc.scale != pc.scale)
         return AC_ERR_KERNEL_ARG_INVALID;

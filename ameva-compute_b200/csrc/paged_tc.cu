@@ -4,11 +4,11 @@
 // A CTA (one per SM) takes row tiles of 256 rows, two groups of 128, and walks key tiles of 128 for both:
 //   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 128 scores from tensor memory, online softmax to base 2, write P
 //                    over the scores as f16 (and, for a 32-bit result, what that rounding left beside it). The accumulator is rescaled
-//                    only when a row's maximum has grown by more than 2^kGrowth since its last rescale. They also bring Q of the next
-//                    piece into shared memory while the last P V runs, and write the piece's results.
+//                    only when a row's maximum has grown by more than 2^kGrowth since its last rescale. They write the piece's results.
 //   warp 8           issues the MMAs: S = Q K^T (both in shared memory), O += P V (P in tensor memory, V MN-major): P V of a group and
 //                    its next S leave together, so that the tensor core works on one group while the other's softmax runs
 //   warp 9           streams K and V tiles with TMA, a box of 64 columns x one page each
+//   warps 10, 11     bring the Q rows of group 0 and 1 in, those of the next piece as soon as the last S of this one has read them
 // Tensor memory: two S / P of 128 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
 // steps of 16 keys that none sees; V rows behind the last key are zeroed before they are multiplied (a page holds anything there).
 // Every wait on a barrier is bounded (sync_ptx.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
@@ -24,7 +24,9 @@ namespace paged {
 using namespace ptx;
 using namespace tc;
 
-constexpr uint32_t kGroupRows = 128, kWarpMma = 8, kWarpLoad = 9, kTcThreads = 320, kTmemCols = 512, kBadRing = 8;
+constexpr uint32_t kGroupRows = 128, kWarpMma = 8, kWarpLoad = 9, kWarpQ = 10, kTcThreads = 384, kTmemCols = 512, kBadRing = 8;
+// Registers a thread after the split: 256 x 200 + 128 x 104 = 384 x 168, what the block is launched with.
+constexpr uint32_t kSoftmaxRegs = 200, kOtherRegs = 104;
 constexpr float kGrowth = 7.0f;   // probabilities stay below 2^7
 
 template <int D>
@@ -35,21 +37,67 @@ struct Tc {
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
 
+// mbar_wait (sync_ptx.cuh) without a call: the registers of a warp whose share setmaxnreg has changed leave no room for a callee's.
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, Ctl* ctl, uint32_t* status, uint32_t tag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!mbar_try_wait(bar, parity)) {
+        if (ctl->abort) return false;
+        if (clock64() - t0 > kWaitCycles) {
+            ctl->abort = 1u;
+            if (atomicCAS(status, DEV_STATUS_OK, DEV_STATUS_WAIT_TIMEOUT) == DEV_STATUS_OK) status[1] = tag;
+            return false;
+        }
+    }
+    return true;
+}
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int page) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map),
         "r"(bar), "r"(column), "r"(token), "r"(head), "r"(page)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t* v) {
+__device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t* v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-        "%30, %31, %32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
-        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-        "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+        "r"(v[14]), "r"(v[15])
         : "memory");
+}
+// two f32 in one register pair: one instruction for both
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// score2 (paged.cuh) from 1 - 2 / (1 + e^2y) = tanh(y): tanhf, 128 times over, leaves no registers for the scores. Its absolute error of
+// 2^-22 is, times a cap of 30, 7e-6 of a score (a 32-bit score of 30 has a spacing of 2e-6).
+__device__ __forceinline__ float capped(const Args& pc, float s) {
+    if (pc.softcap == 0.0f) return s * pc.scale2;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s * pc.cap_in)));
+    return fmaf(-2.0f * pc.cap_out, r, pc.cap_out);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Descriptor of a V tile as the B operand with its columns (N) contiguous: 64-column groups of the 128-byte swizzle
@@ -90,9 +138,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     uint8_t *sQ = base, *sK = sQ + 2u * L::Q, *sV = sK + ST * L::TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * L::TILE);
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST,
-                   q_full = v_empty + 8u * ST, s_full = q_full + 16u, p_full = s_full + 16u, pv_done = p_full + 16u, drain = pv_done + 16u;
-    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 4u * ST + 9u);
-    uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                   // [10]
+                   q_full = v_empty + 8u * ST, s_full = q_full + 16u, p_full = s_full + 16u, pv_done = p_full + 16u, q_empty = pv_done + 16u, drain = q_empty + 16u;
+    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 4u * ST + 11u);
+    uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                   // [12]
     volatile uint32_t* s_bad = s_warp + kTcThreads / 32u;                      // 16-key steps whose page is none, of the last key tiles
     uint32_t* s_pref = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + 512u);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -104,7 +152,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             mbar_init(v_empty + 8u * s, 1u);
         }
         for (uint32_t g = 0; g < 2u; ++g) {
-            mbar_init(q_full + 8u * g, 4u);
+            mbar_init(q_full + 8u * g, 1u);
+            mbar_init(q_empty + 8u * g, 1u);
             mbar_init(s_full + 8u * g, 1u);
             mbar_init(p_full + 8u * g, 4u);
             mbar_init(pv_done + 8u * g, 1u);
@@ -128,6 +177,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     const uint32_t P = 1u << pc.page_log2, box = P < kTcKeys ? P : kTcKeys, boxes = kTcKeys / box;
     bool ok = true;
 
+    if (warp >= kWarpMma) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kWarpLoad) {
         Ring kr(ST), vr(ST);
         uint32_t tiles = 0;     // of this CTA so far
@@ -150,7 +201,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 for (uint32_t kv = 0; kv < 2u; ++kv) {
                     Ring& r = kv ? vr : kr;
                     const uint32_t full = (kv ? v_full : k_full) + 8u * r.idx, empty = (kv ? v_empty : k_empty) + 8u * r.idx;
-                    ok = mbar_wait(empty, r.phase ^ 1u, ctl, pc.status, kv ? 0xD10u : 0xD00u);
+                    ok = wait_on(empty, r.phase ^ 1u, ctl, pc.status, kv ? 0xD10u : 0xD00u);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (lane == 0u) {
@@ -171,8 +222,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             }
         }
         if (ctl->abort) {   // copies already requested finish before the CTA leaves
-            for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) mbar_wait(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
-            for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) mbar_wait(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
+            for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) wait_on(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
+            for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) wait_on(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
         }
     } else if (warp == kWarpMma) {
         const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
@@ -194,7 +245,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (u > T0 && u - 1u >= x.t0 && u - 1u < x.t1) {
                         const uint32_t key0 = (u - 1u) * kTcKeys;
                         if (!have_v) {
-                            ok = ok && mbar_wait<false>(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
+                            ok = ok && wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
                             have_v = true;
                             if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
                                 const uint32_t from = hi_all - key0, n = (16u - (from & 15u)) & 15u;
@@ -207,7 +258,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                 __syncwarp();
                             }
                         }
-                        ok = ok && mbar_wait<false>(p_full + 8u * g, p_uses[g] & 1u, ctl, pc.status, 0xD50u);
+                        ok = ok && wait_on(p_full + 8u * g, p_uses[g] & 1u, ctl, pc.status, 0xD50u);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         ++p_uses[g];
@@ -229,10 +280,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         }
                     }
                     if (u < T1 && u >= x.t0 && u < x.t1) {
-                        if (!have_k) ok = ok && mbar_wait<false>(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
+                        if (!have_k) ok = ok && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
                         have_k = true;
                         if (u == x.t0) {
-                            ok = ok && mbar_wait<false>(q_full + 8u * g, q_uses[g] & 1u, ctl, pc.status, 0xD70u);
+                            ok = ok && wait_on(q_full + 8u * g, q_uses[g] & 1u, ctl, pc.status, 0xD70u);
                             ++q_uses[g];
                         }
                         ok = __all_sync(0xffffffffu, ok);
@@ -248,17 +299,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                     umma_ss_f16(tmem + g * kTcKeys, da + 2u * k, db + 2u * k, idesc_s, (uint32_t)((a | k) != 0u));
                             }
                             umma_commit<false>(s_full + 8u * g);
+                            if (u + 1u == x.t1) umma_commit<false>(q_empty + 8u * g);
                         }
                     }
                 }
                 if (!ok) break;
                 if (u > T0) {   // (a tile that neither group sees is given back, too)
-                    if (!have_v) ok = mbar_wait<false>(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD80u);
+                    if (!have_v) ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD80u);
                     if (lane == 0u) umma_commit<false>(v_empty + 8u * vr.idx);
                     vr.advance();
                 }
                 if (u < T1) {
-                    if (!have_k) ok = ok && mbar_wait<false>(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD90u);
+                    if (!have_k) ok = ok && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD90u);
                     if (lane == 0u) umma_commit<false>(k_empty + 8u * kr.idx);
                     kr.advance();
                 }
@@ -270,40 +322,51 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             umma_commit<false>(drain);
             for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain, 0u); ++spins) __nanosleep(64);
         }
-    } else {
-        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, ts = tmem + lanes + g * kTcKeys, to = tmem + lanes + 2u * kTcKeys + g * D;
-        uint32_t s_uses = 0, pv_uses = 0, tiles = 0, at = st.begin;
-        bool cut = false;
-        // Q rows of a piece into the K-major 128-byte swizzle, a warp its own 32 rows, idle rows zero
-        auto load_q = [&](const Piece& p, const Group& x) {
+    } else if (warp >= kWarpQ) {
+        // Q rows of a group into the K-major 128-byte swizzle, idle rows zero
+        const uint32_t g = warp - kWarpQ;
+        uint32_t uses = 0;
+        while (ok && walk.next(pc, s_pref)) {
+            const Piece& p = walk.p;
+            const Group x = group_of(pc, p, g);
+            if (x.t1 <= x.t0) continue;
+            if (uses) ok = wait_on(q_empty + 8u * g, (uses - 1u) & 1u, ctl, pc.status, 0xDC0u);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ++uses;
             constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
-#pragma unroll 8
-            for (uint32_t i = 0; i < 32u / PER; ++i) {
-                const uint32_t r = (warp & 3u) * 32u + i * PER + lane / PIECES, c = lane % PIECES, row = x.r0 + r;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t c = lane % PIECES, at = smem_u32(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u));
+#pragma unroll 4
+            for (uint32_t i = 0; i < kGroupRows / PER; ++i) {
+                const uint32_t r = i * PER + lane / PIECES, row = x.r0 + r, to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
                 if (r < x.rows)
-                    v = *reinterpret_cast<const uint4*>(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.hkv * pc.G + row % pc.G) * D + 8u * c);
-                *reinterpret_cast<uint4*>(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u) + r * 128u + (((c & 7u) ^ (r & 7u)) << 4)) = v;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to),
+                                 "l"(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.hkv * pc.G + row % pc.G) * D + 8u * c)
+                                 : "memory");
+                else
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0u) : "memory");
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();   // the MMAs read Q through the async proxy
             __syncwarp();
             if (lane == 0u) mbar_arrive(q_full + 8u * g);
-        };
-        bool have = walk.next(pc, s_pref);
-        Group x = {};
-        if (have) {
-            x = group_of(pc, walk.p, g);
-            if (x.t1 > x.t0) load_q(walk.p, x);
         }
-        while (have) {
-            const Piece p = walk.p;
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, ts = tmem + lanes + g * kTcKeys, to = tmem + lanes + 2u * kTcKeys + g * D;
+        uint32_t s_uses = 0, pv_uses = 0, tiles = 0, at = st.begin;
+        bool cut = false;
+        while (walk.next(pc, s_pref)) {
+            const Piece& p = walk.p;
+            const Group x = group_of(pc, p, g);
             const uint32_t my = threadIdx.x & 127u, row = x.r0 + my;
             const bool valid = my < x.rows;
             const Span span = valid ? row_span(pc, p.q, row) : Span{0u, 0u};
             float m_run = neg_inf(), l_run = 0.0f;
             for (uint32_t t = x.t0; t < x.t1; ++t) {
                 const uint32_t key0 = t * kTcKeys;
-                ok = ok && mbar_wait(s_full + 8u * g, s_uses & 1u, ctl, pc.status, 0xDA0u);
+                ok = ok && wait_on(s_full + 8u * g, s_uses & 1u, ctl, pc.status, 0xDA0u);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 ++s_uses;
@@ -319,13 +382,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 if (plain) {
                     float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-                    for (uint32_t k = 0; k < kTcKeys; ++k) m4[k & 3u] = fmaxf(m4[k & 3u], s[k]);
+                    for (uint32_t k = 0; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
                     mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * pc.scale2;
                 } else {
 #pragma unroll
                     for (uint32_t k = 0; k < kTcKeys; ++k) {
                         const uint32_t key = key0 + k;
-                        s[k] = key >= span.lo && key < span.hi && !(gone >> (k >> 4) & 1u) ? score2(pc, s[k]) : neg_inf();
+                        s[k] = key >= span.lo && key < span.hi && !(gone >> (k >> 4) & 1u) ? capped(pc, s[k]) : neg_inf();
                         mx = fmaxf(mx, s[k]);
                     }
                 }
@@ -336,28 +399,26 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     l_run *= f;
                     if (t != x.t0) {
 #pragma unroll 1
-                        for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
-                            uint32_t v[32];
-                            tmem_ld32_async(to + c, v);
-                            tmem_wait_ld();
+                        for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {   // (the scores stay in registers meanwhile)
+                            uint32_t v[16];
+                            tmem_ld16(to + c, v);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-                            tmem_st32_async(to + c, v);
+                            for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                            tmem_st16_async(to + c, v);
                         }
                     }
                 }
                 const float ref = m_run == neg_inf() ? 0.0f : m_run, mul = plain ? pc.scale2 : 1.0f;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t mul2 = pack2(mul, mul), ref2 = pack2(-ref, -ref);
+                uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-                for (uint32_t half = 0; half < 2u; ++half) {
-                    uint32_t ph[32], pl[32];
+                for (uint32_t part = 0; part < 4u; ++part) {
+                    uint32_t ph[16], pl[16];
 #pragma unroll
-                    for (uint32_t k = 0; k < 32u; ++k) {
-                        const float s0 = s[64u * half + 2u * k], s1 = s[64u * half + 2u * k + 1u];
-                        // (the difference by one rounding where the scores are scaled here, of rounded scores otherwise)
-                        const float p0 = ex2(plain ? fmaf(s0, mul, -ref) : s0 - ref), p1 = ex2(plain ? fmaf(s1, mul, -ref) : s1 - ref);
-                        sum[(2u * k) & 3u] += p0;
-                        sum[(2u * k + 1u) & 3u] += p1;
+                    for (uint32_t k = 0; k < 16u; ++k) {
+                        const float2 e = unpack2(fma2(pack2(s[32u * part + 2u * k], s[32u * part + 2u * k + 1u]), mul2, ref2));
+                        const float p0 = ex2(e.x), p1 = ex2(e.y);
+                        sum2[k & 1u] = add2(sum2[k & 1u], pack2(p0, p1));
                         const __half2 h = __floats2half2_rn(p0, p1);
                         ph[k] = *reinterpret_cast<const uint32_t*>(&h);
                         if (EXACT) {
@@ -366,26 +427,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                             pl[k] = *reinterpret_cast<const uint32_t*>(&low);
                         }
                     }
-                    tmem_st32_async(ts + 32u * half, ph);   // over this tile's scores
-                    if (EXACT) tmem_st32_async(ts + 64u + 32u * half, pl);
+                    tmem_st16_async(ts + 16u * part, ph);   // over this tile's scores
+                    if (EXACT) tmem_st16_async(ts + 64u + 16u * part, pl);
                 }
-                l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const float2 sums = unpack2(add2(sum2[0], sum2[1]));
+                l_run += sums.x + sums.y;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(p_full + 8u * g);
             }
-            // Q of the next piece: S of this one's last tile has been read, so its Q is free
-            const Group cur = x;
-            have = walk.next(pc, s_pref);
-            if (have) {
-                x = group_of(pc, walk.p, g);
-                if (ok && x.t1 > x.t0) load_q(walk.p, x);
-            }
             // ---- results of this piece ----
-            const bool some = cur.t1 > cur.t0, whole = p.a == 0u && p.b == p.n;
+            const bool some = x.t1 > x.t0, whole = p.a == 0u && p.b == p.n;
             if (some) {
-                ok = ok && mbar_wait(pv_done + 8u * g, pv_uses & 1u, ctl, pc.status, 0xDB0u) && !ctl->abort;
+                ok = ok && wait_on(pv_done + 8u * g, pv_uses & 1u, ctl, pc.status, 0xDB0u) && !ctl->abort;
                 ++pv_uses;
             }
             ok = __all_sync(0xffffffffu, ok);
@@ -393,9 +448,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             tc_fence_after();
             tiles += p.b - p.a;
             at += p.b - p.a;
-            if (cur.rows) {
+            if (x.rows) {
                 const uint32_t token = p.q.tok0 + row / pc.G, head = p.hkv * pc.G + row % pc.G;
-                float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * kTcRows + (cur.r0 - p.r0)) * (D + 4u);
+                float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * kTcRows + (x.r0 - p.r0)) * (D + 4u);
                 const bool parts = !whole || pc.out == OUT_PARTS;
                 float own = 1.0f, other = 0.0f;      // factors of the values here and of those over other keys
                 const float* extra = nullptr;
@@ -471,7 +526,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 // rows that are not finite although their sum is: over the keys they see, by the whole warp
                 for (uint32_t again = __ballot_sync(0xffffffffu, valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
                     const int i = __ffs(again) - 1;
-                    const uint32_t r = cur.r0 + (warp & 3u) * 32u + (uint32_t)i, tk = p.q.tok0 + r / pc.G, hd = p.hkv * pc.G + r % pc.G;
+                    const uint32_t r = x.r0 + (warp & 3u) * 32u + (uint32_t)i, tk = p.q.tok0 + r / pc.G, hd = p.hkv * pc.G + r % pc.G;
                     const float m = __shfl_sync(0xffffffffu, m_run, i), l = __shfl_sync(0xffffffffu, l_run, i);
                     const Span sp = row_span(pc, p.q, r);
                     float o[C];
@@ -480,7 +535,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (whole) {
                         finish_row<C>(pc, tk, hd, m, l, o);
                     } else {
-                        float* to_row = slot + (uint64_t)(r - cur.r0) * (D + 4u) + 4u + C * lane;
+                        float* to_row = slot + (uint64_t)(r - x.r0) * (D + 4u) + 4u + C * lane;
 #pragma unroll
                         for (uint32_t c = 0; c < C; ++c) to_row[c] = o[c];
                     }
