@@ -99,6 +99,28 @@ __device__ __forceinline__ float capped(const Args& pc, float s) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s * pc.cap_in)));
     return fmaf(-2.0f * pc.cap_out, r, pc.cap_out);
 }
+// The MMAs and commits of a converged warp, issued by one lane, the same every time, without a branch around them: what a branch that
+// only one lane takes computes is not uniform to the compiler, and every descriptor then takes a detour of some 100 clocks.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Descriptor of a V tile as the B operand with its columns (N) contiguous: 64-column groups of the 128-byte swizzle
 // kTcKeys * 128 bytes apart (leading offset), groups of eight keys 1024 bytes apart (stride offset).
@@ -233,12 +255,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const Piece& p = walk.p;
             const Group grp[2] = {group_of(pc, p, 0u), group_of(pc, p, 1u)};
             const uint32_t hi_all = max(grp[0].hi, grp[1].hi), T0 = p.first + p.a, T1 = p.first + p.b;
-            bool started[2] = {false, false};
+            uint32_t started[2] = {0u, 0u};
             // step u: P V of key tile u - 1 and S of key tile u, group by group
             for (uint32_t u = T0; u <= T1 && ok; ++u) {
                 bool have_k = false, have_v = false;
                 uint32_t steps = 0xFFu;   // 16-key steps of tile u - 1 whose pages are there
-                if (u > T0) steps = ~s_bad[(tiles + (u - 1u - T0)) & (kBadRing - 1u)];
+                if (u > T0) steps = ~s_bad[(tiles + (u - 1u - T0)) & (kBadRing - 1u)] & 0xFFu;
 #pragma unroll
                 for (uint32_t g = 0; g < 2u; ++g) {
                     const Group& x = grp[g];
@@ -247,7 +269,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         if (!have_v) {
                             ok = ok && wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
                             have_v = true;
-                            if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
+                            if (ok && hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
                                 const uint32_t from = hi_all - key0, n = (16u - (from & 15u)) & 15u;
                                 for (uint32_t j = lane; j < n * (D / 8u); j += 32u) {
                                     const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
@@ -264,20 +286,27 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         ++p_uses[g];
                         tc_fence_after();
                         const uint32_t s0 = x.lo > key0 ? (x.lo - key0) / 16u : 0u, s1 = (min(x.hi - key0, kTcKeys) + 15u) / 16u;
-                        if (lane == 0u) {
-                            const uint64_t dv = v_desc(smem_u32(sV + vr.idx * L::TILE));
-                            uint32_t acc = started[g];
+                        const uint64_t dv = v_desc(smem_u32(sV + vr.idx * L::TILE));
+                        const uint32_t ta = tmem + g * kTcKeys, to = tmem + 2u * kTcKeys + g * D;
+                        // 16 keys a step: 8 columns of P, two groups of eight V rows
+                        if (s0 == 0u && s1 == kTcKeys / 16u && steps == 0xFFu) {
 #pragma unroll
-                            for (uint32_t k = 0; k < kTcKeys / 16u; ++k) {   // 16 keys: 8 columns of P, two groups of eight V rows
-                                if (k < s0 || k >= s1 || !(steps >> k & 1u)) continue;
-                                const uint32_t ta = tmem + g * kTcKeys + 8u * k, to = tmem + 2u * kTcKeys + g * D;
-                                umma_ts<false, false>(to, ta, dv + 128u * k, idesc_o, acc);
-                                if (EXACT) umma_ts<false, false>(to, ta + 64u, dv + 128u * k, idesc_o, 1u);
-                                acc = 1u;
+                            for (uint32_t k = 0; k < kTcKeys / 16u; ++k) mma_ts(to, ta + 8u * k, dv + 128u * k, idesc_o, k ? 1u : started[g]);
+                            if (EXACT) {
+#pragma unroll
+                                for (uint32_t k = 0; k < kTcKeys / 16u; ++k) mma_ts(to, ta + 64u + 8u * k, dv + 128u * k, idesc_o, 1u);
                             }
-                            started[g] = acc;
-                            if (u == x.t1) umma_commit<false>(pv_done + 8u * g);
+                            started[g] = 1u;
+                        } else {
+#pragma unroll 1
+                            for (uint32_t k = s0; k < s1; ++k) {
+                                if (!(steps >> k & 1u)) continue;
+                                mma_ts(to, ta + 8u * k, dv + 128u * k, idesc_o, started[g]);
+                                if (EXACT) mma_ts(to, ta + 64u + 8u * k, dv + 128u * k, idesc_o, 1u);
+                                started[g] = 1u;
+                            }
                         }
+                        if (u == x.t1) commit(pv_done + 8u * g);
                     }
                     if (u < T1 && u >= x.t0 && u < x.t1) {
                         if (!have_k) ok = ok && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
@@ -289,37 +318,35 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         tc_fence_after();
-                        if (lane == 0u) {
 #pragma unroll
-                            for (uint32_t a = 0; a < A; ++a) {
-                                const uint64_t da = make_smem_desc(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)));
-                                const uint64_t db = make_smem_desc(smem_u32(sK + kr.idx * L::TILE + a * (kTcKeys * 128u)));
+                        for (uint32_t a = 0; a < A; ++a) {
+                            const uint64_t da = make_smem_desc(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)));
+                            const uint64_t db = make_smem_desc(smem_u32(sK + kr.idx * L::TILE + a * (kTcKeys * 128u)));
 #pragma unroll
-                                for (uint32_t k = 0; k < 4u; ++k)
-                                    umma_ss_f16(tmem + g * kTcKeys, da + 2u * k, db + 2u * k, idesc_s, (uint32_t)((a | k) != 0u));
-                            }
-                            umma_commit<false>(s_full + 8u * g);
-                            if (u + 1u == x.t1) umma_commit<false>(q_empty + 8u * g);
+                            for (uint32_t k = 0; k < 4u; ++k)
+                                mma_ss(tmem + g * kTcKeys, da + 2u * k, db + 2u * k, idesc_s, (uint32_t)((a | k) != 0u));
                         }
+                        commit(s_full + 8u * g);
+                        if (u + 1u == x.t1) commit(q_empty + 8u * g);
                     }
                 }
                 if (!ok) break;
                 if (u > T0) {   // (a tile that neither group sees is given back, too)
                     if (!have_v) ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD80u);
-                    if (lane == 0u) umma_commit<false>(v_empty + 8u * vr.idx);
+                    commit(v_empty + 8u * vr.idx);
                     vr.advance();
                 }
                 if (u < T1) {
                     if (!have_k) ok = ok && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD90u);
-                    if (lane == 0u) umma_commit<false>(k_empty + 8u * kr.idx);
+                    commit(k_empty + 8u * kr.idx);
                     kr.advance();
                 }
-                ok = __all_sync(0xffffffffu, ok);
             }
+            ok = __all_sync(0xffffffffu, ok);
             tiles += p.b - p.a;
         }
-        if (ctl->abort && lane == 0u) {   // MMAs already issued finish before the CTA leaves
-            umma_commit<false>(drain);
+        if (__any_sync(0xffffffffu, ctl->abort != 0u)) {   // MMAs already issued finish before the CTA leaves
+            commit(drain);
             for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain, 0u); ++spins) __nanosleep(64);
         }
     } else if (warp >= kWarpQ) {
@@ -372,26 +399,30 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 ++s_uses;
                 tc_fence_after();
                 const uint32_t gone = s_bad[(tiles + (t - p.first - p.a)) & (kBadRing - 1u)];
-                float s[kTcKeys];
+                // the same for every thread of the group
+                const bool plain = gone == 0u && key0 >= x.lo_all && key0 + kTcKeys <= x.hi_all && pc.softcap == 0.0f && pc.scale2 > 0.0f;
+                if (!plain) {   // hidden keys and the cap, on the scores where they are: few tiles, so few registers rather than few steps
+#pragma unroll 1
+                    for (uint32_t c = 0; c < kTcKeys; c += 16u) {
+                        uint32_t v[16];
+                        tmem_ld16(ts + c, v);
+#pragma unroll
+                        for (uint32_t k = 0; k < 16u; ++k) {
+                            const uint32_t key = key0 + c + k;
+                            const bool seen = key >= span.lo && key < span.hi && !(gone >> (c >> 4) & 1u);
+                            v[k] = __float_as_uint(seen ? capped(pc, __uint_as_float(v[k])) : neg_inf());
+                        }
+                        tmem_st16_async(ts + c, v);
+                    }
+                    tmem_wait_st();
+                }
+                float s[kTcKeys], m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
                 for (uint32_t c = 0; c < kTcKeys; c += 32u) tmem_ld32_async(ts + c, reinterpret_cast<uint32_t*>(s) + c);
                 tmem_wait_ld();
-                // the same for every thread of the group
-                const bool plain = gone == 0u && key0 >= x.lo_all && key0 + kTcKeys <= x.hi_all && pc.softcap == 0.0f && pc.scale2 > 0.0f;
-                float mx = neg_inf();
-                if (plain) {
-                    float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-                    for (uint32_t k = 0; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
-                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * pc.scale2;
-                } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < kTcKeys; ++k) {
-                        const uint32_t key = key0 + k;
-                        s[k] = key >= span.lo && key < span.hi && !(gone >> (k >> 4) & 1u) ? capped(pc, s[k]) : neg_inf();
-                        mx = fmaxf(mx, s[k]);
-                    }
-                }
+                for (uint32_t k = 0; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
+                const float mul = plain ? pc.scale2 : 1.0f, mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
                 const bool grow = mx > m_run + kGrowth || (m_run == neg_inf() && mx != neg_inf());
                 if (__any_sync(0xffffffffu, grow)) {   // (no P V of this group is on its way: S of this tile was issued behind the last)
                     const float f = !grow ? 1.0f : weight(m_run, mx);
@@ -408,7 +439,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         }
                     }
                 }
-                const float ref = m_run == neg_inf() ? 0.0f : m_run, mul = plain ? pc.scale2 : 1.0f;
+                const float ref = m_run == neg_inf() ? 0.0f : m_run;
                 const uint64_t mul2 = pack2(mul, mul), ref2 = pack2(-ref, -ref);
                 uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
