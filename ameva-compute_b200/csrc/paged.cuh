@@ -7,11 +7,12 @@
 // a batch is one more sequence, of all rows, every one of which sees all of its keys.
 //
 // The G query heads that share a KV head make R = n * G rows per sequence and KV head (row r: query r / G, head r % G), dealt in
-// tiles of ROWS; a row tile walks the key tiles (KEYS keys each) that any of its rows sees. All (sequence, KV head, row tile, key
-// tile) in this order form one line, and every CTA takes an equal stretch of it: no CTA has more than one tile more than another,
-// whatever the lengths are. A row tile that lies in one stretch is finished there; one that is cut leaves a maximum, a sum and
-// weighted values per row and CTA (at most two per CTA: its first and its last piece), which the merge kernel joins. The line's
-// length is only known on the device: every CTA forms the same sums over the sequences.
+// tiles of ROWS; a row tile walks the key tiles (2^keys_log2 keys each) that any of its rows sees, for the HB KV heads of a group at
+// once. All (sequence, head group, row tile, key tile) in this order form one line, and every CTA takes an equal stretch of it,
+// whatever the lengths are. What a row tile costs beside its key tiles counts as `over` tiles behind its last. A row tile that lies in one
+// stretch is finished there; one that is cut leaves a maximum, a sum and weighted values per row and CTA (at most two per CTA: its
+// first and its last piece), which the merge kernel joins. The line's length is only known on the device: every CTA forms the same
+// sums over the sequences.
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -33,6 +34,7 @@ struct Args {
     void* dst;
     float* slots;               // results of cut row tiles: slot 2 c (a tile begun elsewhere), 2 c + 1 (one that goes on elsewhere)
     uint4* cut;                 // per CTA two words of four: what the merge kernel needs of a cut row tile
+    uint32_t HB, groups, keys_log2, over;   // KV heads of a group, groups, the line's tiles and its allowance per row tile
     const float* extra;         // results over other keys of the same rows that the final ones take in (the layout of OUT_PARTS)
     uint32_t* refused;          // the caller's status words: count of refused entries, lowest node
     uint32_t* status;           // the context's
@@ -87,17 +89,16 @@ __device__ __forceinline__ Span row_span(const Args& pc, const Seq& q, uint32_t 
     return {pc.window && hi > pc.window ? hi - pc.window : 0u, hi};
 }
 // The first key tile of rows r0 .. r1 and how many there are: at least one, so that rows that see nothing are written, too.
-template <uint32_t KEYS>
 __device__ __forceinline__ void tile_range(const Args& pc, const Seq& q, uint32_t r0, uint32_t r1, uint32_t& first, uint32_t& count) {
     const uint32_t lo = row_span(pc, q, r0).lo, hi = row_span(pc, q, r1).hi;
-    first = lo / KEYS;
-    count = hi > lo ? (hi + KEYS - 1u) / KEYS - first : 1u;
+    first = lo >> pc.keys_log2;
+    count = hi > lo ? ((hi + (1u << pc.keys_log2) - 1u) >> pc.keys_log2) - first : 1u;
 }
 
 __device__ __forceinline__ bool served(const Args& pc, uint32_t R) { return R >= pc.min_rows && R <= pc.max_rows && R != 0u; }
 
 // The line: s_pref[s] = tiles in front of sequence s (s_pref[n] = all of them). WARPS warps, all threads; ends with a barrier.
-template <uint32_t ROWS, uint32_t KEYS, uint32_t WARPS>
+template <uint32_t ROWS, uint32_t WARPS>
 __device__ __forceinline__ uint32_t build_line(const Args& pc, uint32_t* s_pref, uint32_t* s_warp) {
     const uint32_t n = pc.prefix ? 1u : pc.n_seqs;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -121,16 +122,16 @@ __device__ __forceinline__ uint32_t build_line(const Args& pc, uint32_t* s_pref,
             uint32_t tiles = 0, first, count;
             if (served(pc, R) && whole) {
                 if (pc.prefix) {
-                    tile_range<KEYS>(pc, q, 0u, 0u, first, count);
-                    tiles = count * ((R + ROWS - 1u) / ROWS);
+                    tile_range(pc, q, 0u, 0u, first, count);
+                    tiles = (count + pc.over) * ((R + ROWS - 1u) / ROWS);
                 } else {
                     for (uint32_t r = 0; r < R; r += ROWS) {
-                        tile_range<KEYS>(pc, q, r, min(r + ROWS, R) - 1u, first, count);
-                        tiles += count;
+                        tile_range(pc, q, r, min(r + ROWS, R) - 1u, first, count);
+                        tiles += count + pc.over;
                     }
                 }
             }
-            s_pref[s] = tiles * pc.n_head_kv;
+            s_pref[s] = tiles * pc.groups;
         }
     } else {
         for (uint32_t s = warp; s < n; s += WARPS) {
@@ -139,11 +140,11 @@ __device__ __forceinline__ uint32_t build_line(const Args& pc, uint32_t* s_pref,
             uint32_t tiles = 0, first, count;
             if (served(pc, R))
                 for (uint32_t r = lane * ROWS; r < R; r += 32u * ROWS) {
-                    tile_range<KEYS>(pc, q, r, min(r + ROWS, R) - 1u, first, count);
-                    tiles += count;
+                    tile_range(pc, q, r, min(r + ROWS, R) - 1u, first, count);
+                    tiles += count + pc.over;
                 }
             tiles = (uint32_t)warp_sum_i((int)tiles);
-            if (lane == 0u) s_pref[s] = tiles * pc.n_head_kv;
+            if (lane == 0u) s_pref[s] = tiles * pc.groups;
         }
     }
     __syncthreads();
@@ -195,77 +196,80 @@ __device__ __forceinline__ uint32_t last_cta(const Stretch& x, uint32_t e) {
     return (uint32_t)(((uint64_t)e * x.ctas + x.total - 1u) / x.total) - 1u;
 }
 
-// The part of a row tile that a CTA works on: key tiles first + a .. first + b - 1 of its n.
+// The part of a row tile that a CTA works on: key tiles first + a .. first + b - 1 of its n; `begin`: the row tile's place in the line.
 struct Piece {
-    uint32_t seq, hkv, r0, R, first, a, b, n;
+    uint32_t seq, group, r0, R, first, a, b, n, begin;
     Seq q;
 };
 // Walks a stretch piece by piece; a whole warp, all lanes with the same values.
-template <uint32_t ROWS, uint32_t KEYS>
+template <uint32_t ROWS>
 struct Walk {
     uint32_t t, end, seq;
     Piece p;
     __device__ __forceinline__ Walk(const Stretch& x) : t(x.begin), end(x.end), seq(0xFFFFFFFFu) {}
     __device__ __forceinline__ bool next(const Args& pc, const uint32_t* s_pref) {
-        if (t >= end) return false;
-        if (seq == 0xFFFFFFFFu || t >= s_pref[seq + 1u]) {   // the sequence that tile t belongs to
-            uint32_t lo = 0, hi = pc.prefix ? 1u : pc.n_seqs;   // s_pref[lo] <= t < s_pref[hi]
-            while (hi - lo > 1u) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (s_pref[mid] <= t) lo = mid;
-                else hi = mid;
+        while (t < end) {
+            if (seq == 0xFFFFFFFFu || t >= s_pref[seq + 1u]) {   // the sequence that place t belongs to
+                uint32_t lo = 0, hi = pc.prefix ? 1u : pc.n_seqs;   // s_pref[lo] <= t < s_pref[hi]
+                while (hi - lo > 1u) {
+                    const uint32_t mid = (lo + hi) >> 1;
+                    if (s_pref[mid] <= t) lo = mid;
+                    else hi = mid;
+                }
+                seq = p.seq = lo;
+                p.q = load_seq(pc, lo);
+                p.R = p.q.n_q * pc.G;
             }
-            seq = p.seq = lo;
-            p.q = load_seq(pc, lo);
-            p.R = p.q.n_q * pc.G;
-        }
-        const uint32_t at = t - s_pref[seq], per_head = (s_pref[seq + 1u] - s_pref[seq]) / pc.n_head_kv;
-        p.hkv = at / per_head;
-        uint32_t rem = at - p.hkv * per_head;
-        // the row tile: the prefix's have the same number of key tiles, the others are counted 32 at a time
-        if (pc.prefix) {
-            tile_range<KEYS>(pc, p.q, 0u, 0u, p.first, p.n);
-            const uint32_t i = rem / p.n;
-            p.r0 = i * ROWS;
-            rem -= i * p.n;
-        } else {
-            const uint32_t lane = threadIdx.x & 31u;
-            for (uint32_t base = 0;; base += 32u * ROWS) {
-                const uint32_t r = base + lane * ROWS;
-                uint32_t first = 0, count = 0;
-                if (r < p.R) tile_range<KEYS>(pc, p.q, r, min(r + ROWS, p.R) - 1u, first, count);
-                uint32_t incl = count;
+            const uint32_t at = t - s_pref[seq], per_group = (s_pref[seq + 1u] - s_pref[seq]) / pc.groups;
+            p.group = at / per_group;
+            uint32_t rem = at - p.group * per_group;
+            if (pc.prefix || p.R <= ROWS) {   // row tiles with the same number of key tiles, or a single one
+                tile_range(pc, p.q, 0u, p.R <= ROWS ? p.R - 1u : 0u, p.first, p.n);
+                const uint32_t i = rem / (p.n + pc.over);
+                p.r0 = i * ROWS;
+                rem -= i * (p.n + pc.over);
+            } else {                          // counted 32 at a time
+                const uint32_t lane = threadIdx.x & 31u;
+                for (uint32_t base = 0;; base += 32u * ROWS) {
+                    const uint32_t r = base + lane * ROWS;
+                    uint32_t first = 0, count = 0;
+                    if (r < p.R) tile_range(pc, p.q, r, min(r + ROWS, p.R) - 1u, first, count);
+                    const uint32_t len = r < p.R ? count + pc.over : 0u;
+                    uint32_t incl = len;
 #pragma unroll
-                for (uint32_t o = 1; o < 32u; o <<= 1) {
-                    const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += up;
+                    for (uint32_t o = 1; o < 32u; o <<= 1) {
+                        const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= o) incl += up;
+                    }
+                    const uint32_t hit = __ballot_sync(0xffffffffu, incl > rem);
+                    if (hit == 0u && base + 32u * ROWS < p.R) {
+                        rem -= __shfl_sync(0xffffffffu, incl, 31);
+                        continue;
+                    }
+                    const int from = hit ? __ffs(hit) - 1 : 0;   // (hit is never empty in the last round)
+                    p.first = __shfl_sync(0xffffffffu, first, from);
+                    p.n = __shfl_sync(0xffffffffu, count, from);
+                    p.r0 = base + (uint32_t)from * ROWS;
+                    rem -= __shfl_sync(0xffffffffu, incl - len, from);
+                    break;
                 }
-                const uint32_t hit = __ballot_sync(0xffffffffu, incl > rem);
-                if (hit == 0u && base + 32u * ROWS < p.R) {
-                    rem -= __shfl_sync(0xffffffffu, incl, 31);
-                    continue;
-                }
-                const int from = hit ? __ffs(hit) - 1 : 0;   // (hit is never empty in the last round)
-                p.first = __shfl_sync(0xffffffffu, first, from);
-                p.n = __shfl_sync(0xffffffffu, count, from);
-                p.r0 = base + (uint32_t)from * ROWS;
-                rem -= __shfl_sync(0xffffffffu, incl - count, from);
-                break;
             }
+            const uint32_t step = min(p.n + pc.over - rem, end - t);
+            p.begin = t - rem;
+            p.a = min(rem, p.n);
+            p.b = min(p.n, rem + step);
+            t += step;
+            if (p.b > p.a) return true;
         }
-        p.a = rem;
-        p.b = min(p.n, rem + (end - t));
-        t += p.b - p.a;
-        return true;
+        return false;
     }
 };
 
-// Notes for the merge kernel what the CTA's last piece leaves: parts == 0 where that is nothing. `whole`: tiles of the line up to
-// the end of the row tile.
-__device__ __forceinline__ void note_cut(const Args& pc, const Stretch& x, const Piece& p, uint32_t rows, uint32_t piece_end) {
-    const uint32_t last = last_cta(x, piece_end + (p.n - p.b));
+// Notes for the merge kernel what the CTA's last piece leaves (the first word 0: nothing).
+__device__ __forceinline__ void note_cut(const Args& pc, const Stretch& x, const Piece& p, uint32_t rows) {
+    const uint32_t last = last_cta(x, p.begin + p.n);
     pc.cut[2u * blockIdx.x] = make_uint4(last - blockIdx.x + 1u, p.q.tok0, p.r0, rows);
-    pc.cut[2u * blockIdx.x + 1u] = make_uint4(p.hkv, 0u, 0u, 0u);
+    pc.cut[2u * blockIdx.x + 1u] = make_uint4(p.group, 0u, 0u, 0u);
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -5,7 +5,7 @@
 namespace amv {
 namespace paged {
 
-// Maps of the cache for boxes of `tokens` tokens x 64 columns of one head and page; false where no map expresses the strides.
+// Maps of the cache for boxes of 64 columns x tokens x heads of one page.
 struct Maps {
     CUtensorMap k, v;
 };

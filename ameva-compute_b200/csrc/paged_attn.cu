@@ -2,12 +2,16 @@
 // long prefix. Here: the kernel for few rows per sequence (tokens, drafts), the merge kernel and the launchers; many rows per
 // sequence (prompts, the prefix of a batch) run in paged_tc.cu.
 //
-// paged_rows_kernel: W + 1 warps. The last one streams key tiles (16 W keys, K and V) through a ring in shared memory with TMA, a box
-// of up to 64 columns x one page each, and runs ahead across the pieces of the CTA's stretch, so that the reads never pause. Each of
-// the others takes 16 keys of every tile for the tile's 16 rows: both products on mma.sync (f16 in, f32 out), an online softmax per row
-// to base 2, the scores' accumulators reused as the A operand of the second product. At the end of a piece the warps are joined through
-// shared memory. P: for an f32 result as an f16 value and its remainder (rounded once, 2^-12 of every probability would show there), for
-// an f16 result rounded once (2^-12 against the 2^-12 of the result itself, averaged over the keys).
+// paged_rows_kernel: W + 1 warps. The last one streams key tiles (KB blocks of 16 keys of HB KV heads, K and V) through a ring in shared
+// memory with TMA, a box of 64 columns x 16 keys x HB heads each, and runs ahead across the pieces of the CTA's stretch, so that the
+// reads never pause. Each of the others takes one head and one block of 16 keys of every tile for the tile's 16 rows: both products on
+// mma.sync (f16 in, f32 out), an online softmax per row to base 2, the scores' accumulators reused as the A operand of the second
+// product. With W = HB (eight KV heads, say) a warp owns its head's rows from the first key to the last and the warps never meet; with
+// fewer heads the KB warps of a head are joined pairwise through shared memory at the end of a piece. All heads of a block of keys are
+// read together because in a cache with a token's heads beside one another they are one run of memory: a head at a time (a warp per
+// 16 keys of a tile of 128) took 195 us for 96 sequences of 20 to 8192 keys, 8 KV heads of 128, 160 k keys, as against 100 us for the
+// bytes, and 8 us per (sequence, head). P: for an f32 result as an f16 value and its remainder (rounded once, 2^-12 of every probability
+// would show there), for an f16 result rounded once (2^-12 against the 2^-12 of the result itself, averaged over the keys).
 #include <cstring>
 
 #include "paged.h"
@@ -22,13 +26,15 @@ using namespace ptx;
 
 template <int D>
 struct Rows {
-    static constexpr uint32_t W = D == 256 ? 4 : 8, KEYS = 16 * W, ATOMS = D / 64;
-    static constexpr uint32_t TILE = KEYS * D * 2u, STAGE = 2u * TILE, STAGES = D == 64 ? 6 : 3;
-    static constexpr uint32_t MERGE = (W / 2) * 8u * (D + 4u) * 4u;   // half the warps' results for eight rows
-    static constexpr uint32_t STATE = W * kDecRows * 2u * 4u;
-    static constexpr uint32_t FIXED = 1024u + STAGES * STAGE + MERGE + STATE + 128u + 16u * STAGES;
+    static constexpr uint32_t W = D == 256 ? 4 : 8, ATOMS = D / 64, MAX_STAGES = 8;
+    static constexpr uint32_t BLOCK = 16u * D * 2u;                    // K or V of one head and 16 keys
+    static constexpr uint32_t RING = 3u * 2u * 8u * 16u * 128u * 2u;   // 192 KB
+    static constexpr uint32_t MERGE = (W / 2) * 8u * (D + 4u) * 4u;    // half the warps' results for eight rows
+    static constexpr uint32_t FIXED = 1024u + RING + MERGE + 128u + 16u * MAX_STAGES;
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
+// How W warps share HB heads: blocks of 16 keys per tile, a power of two
+__host__ __device__ constexpr uint32_t blocks_of(uint32_t W, uint32_t HB) { return W >= 8u * HB ? 8u : W >= 4u * HB ? 4u : W >= 2u * HB ? 2u : 1u; }
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
@@ -59,27 +65,64 @@ __device__ __forceinline__ void worker_sync() {   // the warps that multiply, no
     asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
+// Result of a row whose columns 8 nt + 2 t4 + {0, 1} the four lanes of its MMA fragment hold: as finish_row (paged.cuh).
+template <int NT>
+__device__ __forceinline__ void finish_fragment(const Args& pc, uint32_t token, uint32_t head, uint32_t t4, float m, float l, const float (&oc)[NT][4],
+                                                uint32_t h) {
+    constexpr uint32_t D = 8u * NT;
+    const float* extra = nullptr;
+    float f = 1.0f, g = 0.0f;
+    if (pc.extra) {
+        extra = pc.extra + ((uint64_t)token * pc.n_head + head) * (D + 4u);
+        const float2 ml = *reinterpret_cast<const float2*>(extra);
+        const float top = fmaxf(m, ml.x);
+        f = weight(m, top);
+        g = weight(ml.x, top);
+        l = l * f + ml.y * g;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const uint64_t at = dst_row(pc, token, head, D) + 2u * t4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float2 y = make_float2(f != 0.0f ? oc[nt][2u * h] * f : 0.0f, f != 0.0f ? oc[nt][2u * h + 1u] * f : 0.0f);
+        if (extra && g != 0.0f) {
+            const float2 e = *reinterpret_cast<const float2*>(extra + 4u + 8u * nt + 2u * t4);
+            y.x = fmaf(e.x, g, y.x);
+            y.y = fmaf(e.y, g, y.y);
+        }
+        if (inv == 0.0f) y = make_float2(0.0f, 0.0f);
+        if (pc.out == OUT_F16) *reinterpret_cast<__half2*>(reinterpret_cast<__half*>(pc.dst) + at + 8u * nt) = __floats2half2_rn(y.x * inv, y.y * inv);
+        else *reinterpret_cast<float2*>(reinterpret_cast<float*>(pc.dst) + at + 8u * nt) = make_float2(y.x * inv, y.y * inv);
+    }
+}
+template <int NT>
+__device__ __forceinline__ void store_part(float* row, uint32_t t4, float m, float l, const float (&oc)[NT][4], uint32_t h) {
+    if (t4 == 0u) *reinterpret_cast<float2*>(row) = make_float2(m, l);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float2*>(row + 4u + 8u * nt + 2u * t4) = make_float2(oc[nt][2u * h], oc[nt][2u * h + 1u]);
+}
+
 // TOP: every row tile has at most eight rows (the upper half of the MMA tile), so the lower half's work is left out.
 template <int D, bool TOP, bool EXACT>
 __global__ void __launch_bounds__((Rows<D>::W + 1) * 32, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args pc) {
     using L = Rows<D>;
-    constexpr uint32_t W = L::W, KEYS = L::KEYS, A = L::ATOMS, C = D / 32, H = TOP ? 1 : 2;
+    constexpr uint32_t W = L::W, A = L::ATOMS, C = D / 32, H = TOP ? 1 : 2;
     constexpr int KS = D / 16, NT = D / 8;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    float* s_merge = reinterpret_cast<float*>(base + L::STAGES * L::STAGE);        // [W / 2][8][D + 4]
-    float* s_m = s_merge + L::MERGE / 4u;                                          // [W][16] maxima
-    float* s_l = s_m + W * kDecRows;                                               // [W][16] sums
-    uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + W * kDecRows);              // full, empty
-    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 2u * L::STAGES);
+    float* s_merge = reinterpret_cast<float*>(base + L::RING);                     // [W / 2][8][D + 4]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_merge + L::MERGE / 4u);         // full, empty
+    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 2u * L::MAX_STAGES);
     uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                       // [W + 1]
     uint32_t* s_bad = s_warp + W + 1u;                                             // per stage: 16-key blocks whose page is none
-    uint32_t* s_pref = s_bad + L::STAGES;
-    const uint32_t full = smem_u32(bars), empty = full + 8u * L::STAGES;
+    uint32_t* s_pref = s_bad + L::MAX_STAGES;
+    const uint32_t full = smem_u32(bars), empty = full + 8u * L::MAX_STAGES;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t HB = pc.HB, KB = 1u << (pc.keys_log2 - 4u);
+    const uint32_t half = KB * HB * L::BLOCK, stages = min(L::MAX_STAGES, L::RING / (2u * half));   // bytes of K (and of V) of a tile
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < L::STAGES; ++s) {
+        for (uint32_t s = 0; s < L::MAX_STAGES; ++s) {
             mbar_init(full + 8u * s, 1u);
             mbar_init(empty + 8u * s, W);
         }
@@ -88,82 +131,83 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     }
     pdl_trigger();
     pdl_wait();
-    const uint32_t total = build_line<kDecRows, KEYS, W + 1u>(pc, s_pref, s_warp);   // (its barriers publish the ones above)
+    const uint32_t total = build_line<kDecRows, W + 1u>(pc, s_pref, s_warp);   // (its barriers publish the ones above)
     const Stretch st = my_stretch(total);
-    Walk<kDecRows, KEYS> walk(st);
-    const uint32_t P = 1u << pc.page_log2, box = P < KEYS ? P : KEYS;
-    Ring ring(L::STAGES);
+    Walk<kDecRows> walk(st);
+    Ring ring(stages);
     bool ok = true;
 
     if (warp == W) {   // ---- loads ----
+        const uint32_t mask = (1u << pc.page_log2) - 1u;
         uint32_t issued = 0;
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
             const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + kDecRows, p.R) - 1u).hi;
             for (uint32_t i = p.a; i < p.b; ++i) {
-                const uint32_t key0 = (p.first + i) * KEYS;
+                const uint32_t key0 = (p.first + i) << pc.keys_log2;
+                // lane b < KB looks block b's page up; blocks that hold a key somebody sees are loaded, box j of 2 A KB by lane j
+                const uint32_t b = lane & (KB - 1u), b0 = key0 + 16u * b, j = lane / KB;
+                const bool want = b0 < hi && b0 + 16u > lo;
+                const int32_t page = want ? page_of(pc, p.q, b0) : -1;
                 ok = mbar_wait(empty + 8u * ring.idx, ring.phase ^ 1u, ctl, pc.status, 0xC00u);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                // boxes of the tile: the first lanes look their pages up; those that hold a key somebody sees are loaded
-                const uint32_t boxes = KEYS / box, b0 = key0 + lane * box;
-                int32_t page = -1;
-                bool want = lane < boxes && b0 < hi && b0 + box > lo;
-                if (want) page = page_of(pc, p.q, b0);
-                const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0), load = __ballot_sync(0xffffffffu, want && page >= 0);
-                uint32_t bad = 0;
-                if (none) {   // as 16-key blocks
-                    for (uint32_t j = 0; j < W; ++j) bad |= (none >> (16u * j / box) & 1u) << j;
-                    if (lane == 0u) refuse(pc, __popc(none));
-                }
-                const uint32_t stage = smem_u32(base) + ring.idx * L::STAGE, bar = full + 8u * ring.idx;
+                const uint32_t ours = KB == 32u ? 0xffffffffu : (1u << KB) - 1u;
+                const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0) & ours, load = __ballot_sync(0xffffffffu, page >= 0) & ours;
+                const uint32_t stage = smem_u32(base) + ring.idx * 2u * half, bar = full + 8u * ring.idx;
                 if (lane == 0u) {
-                    s_bad[ring.idx] = bad;
-                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(load) * box * D * 2u * 2u);
+                    if (none) refuse(pc, __popc(none));
+                    s_bad[ring.idx] = none;
+                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(load) * HB * L::BLOCK * 2u);
                 }
                 __syncwarp();
-                for (uint32_t j = lane; j < boxes * A * 2u; j += 32u) {
-                    const uint32_t b = j % boxes, a = j / boxes % A, kv = j / (boxes * A);
-                    if (!(load >> b & 1u)) continue;
-                    const int32_t pg = page_of(pc, p.q, key0 + b * box);   // (just read: from L1)
-                    tma_page(stage + kv * L::TILE + a * (KEYS * 128u) + b * box * 128u, kv ? &v_map : &k_map, bar, (int)(64u * a),
-                             (int)((key0 + b * box) & (P - 1u)), (int)p.hkv, pg);
+                for (uint32_t n = j; n < 2u * A; n += 32u / KB) {   // K and V, 64 columns each
+                    const uint32_t kv = n / A, a = n % A;
+                    if (page >= 0)
+                        tma_page(stage + kv * half + (b * A + a) * (HB * 2048u), kv ? &v_map : &k_map, bar, (int)(64u * a), (int)(b0 & mask),
+                                 (int)(p.group * HB), page);
                 }
                 ++issued;
                 ring.advance();
             }
         }
         if (ctl->abort) {   // copies already requested finish before the CTA leaves
-            for (uint32_t i = issued > L::STAGES ? issued - L::STAGES : 0u; i < issued; ++i)
-                mbar_wait(full + 8u * (i % L::STAGES), (i / L::STAGES) & 1u, ctl, pc.status, 0xC10u);
+            for (uint32_t i = issued > stages ? issued - stages : 0u; i < issued; ++i)
+                mbar_wait(full + 8u * (i % stages), (i / stages) & 1u, ctl, pc.status, 0xC10u);
         }
         return;
     }
 
-    // ---- products ----
+    // ---- products: head `hb` of the group, block `kb` of the tile ----
+    const uint32_t kb = warp / HB, hb = warp - kb * HB;
     const uint32_t g = lane >> 2, t4 = lane & 3u;
-    const uint32_t lm_row = 16u * warp + (lane & 7u) + ((lane >> 4) << 3), lm_hi = (lane >> 3) & 1u;   // K: key in the tile, upper eight columns
-    const uint32_t lv_row = 16u * warp + (lane & 7u) + (((lane >> 3) & 1u) << 3), lv_nt = lane >> 4;    // V: key in the tile, second n-tile
-    uint32_t done = st.begin;
+    const uint32_t lm_row = (lane & 7u) + ((lane >> 4) << 3), lm_hi = (lane >> 3) & 1u;   // K: key in the block, upper eight columns
+    const uint32_t lv_row = (lane & 7u) + (((lane >> 3) & 1u) << 3), lv_nt = lane >> 4;    // V: key in the block, second n-tile
     bool cut = false;
     while (walk.next(pc, s_pref)) {
         const Piece& p = walk.p;
+        const uint32_t hkv = p.group * HB + hb;
+        const bool mine = kb < KB && hkv < pc.n_head_kv;
         const uint32_t rows = min(kDecRows, p.R - p.r0);
         const uint32_t lo_all = row_span(pc, p.q, p.r0).lo, hi_all = row_span(pc, p.q, p.r0 + rows - 1u).hi;     // keys that some row sees
         const uint32_t lo_both = row_span(pc, p.q, p.r0 + rows - 1u).lo, hi_both = row_span(pc, p.q, p.r0).hi;   // keys that every row sees
         Span span[2];
+        uint32_t token[2], head[2];
+        bool valid[2];
         uint32_t qa[KS][4];
 #pragma unroll
         for (uint32_t h = 0; h < 2u; ++h) {
             const uint32_t r = p.r0 + g + 8u * h;
-            const bool valid = h < H && g + 8u * h < rows;
-            span[h] = valid ? row_span(pc, p.q, r) : Span{0u, 0u};
-            const __half* qrow = pc.q + (uint64_t)(p.q.tok0 + (valid ? r / pc.G : 0u)) * pc.q_s + (uint64_t)(p.hkv * pc.G + (valid ? r % pc.G : 0u)) * D;
+            valid[h] = mine && h < H && g + 8u * h < rows;
+            span[h] = valid[h] ? row_span(pc, p.q, r) : Span{0u, 0u};
+            token[h] = p.q.tok0 + (valid[h] ? r / pc.G : 0u);
+            head[h] = valid[h] ? hkv * pc.G + r % pc.G : 0u;
+            const __half* qrow = pc.q + (uint64_t)token[h] * pc.q_s + (uint64_t)head[h] * D;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const uint32_t c = 16u * ks + 2u * t4;
-                qa[ks][h] = valid ? *reinterpret_cast<const uint32_t*>(qrow + c) : 0u;
-                qa[ks][2u + h] = valid ? *reinterpret_cast<const uint32_t*>(qrow + c + 8u) : 0u;
+                qa[ks][h] = valid[h] ? *reinterpret_cast<const uint32_t*>(qrow + c) : 0u;
+                qa[ks][2u + h] = valid[h] ? *reinterpret_cast<const uint32_t*>(qrow + c + 8u) : 0u;
             }
         }
         float oc[NT][4], m_run[2] = {neg_inf(), neg_inf()}, l_run[2] = {0.0f, 0.0f};
@@ -173,12 +217,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             for (int j = 0; j < 4; ++j) oc[nt][j] = 0.0f;
 
         for (uint32_t i = p.a; i < p.b; ++i) {
-            const uint32_t key0 = (p.first + i) * KEYS + 16u * warp;
+            const uint32_t key0 = ((p.first + i) << pc.keys_log2) + 16u * kb;
             ok = ok && mbar_wait(full + 8u * ring.idx, ring.phase, ctl, pc.status, 0xC20u);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;   // (the pieces are walked to the end all the same: the warps meet at their barriers)
-            const uint32_t tk = smem_u32(base) + ring.idx * L::STAGE, tv = tk + L::TILE;
-            const bool seen = key0 < hi_all && key0 + 16u > lo_all && !(s_bad[ring.idx] >> warp & 1u);
+            // [block][64 columns][head][16 keys][128 bytes, swizzled]
+            const uint32_t tk = smem_u32(base) + ring.idx * 2u * half + kb * A * HB * 2048u + hb * 2048u, tv = tk + half, atom = HB * 2048u;
+            const bool seen = mine && key0 < hi_all && key0 + 16u > lo_all && !(s_bad[ring.idx] >> kb & 1u);
             if (seen) {
                 float sc[2][4];
 #pragma unroll
@@ -189,7 +234,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t piece = 2u * (ks & 3) + lm_hi;
                     uint32_t b[4];
-                    ldsm_x4(b, tk + (ks >> 2) * (KEYS * 128u) + lm_row * 128u + ((piece ^ (lm_row & 7u)) << 4));
+                    ldsm_x4(b, tk + (ks >> 2) * atom + lm_row * 128u + ((piece ^ (lm_row & 7u)) << 4));
                     mma16816(sc[0], qa[ks], b[0], b[1]);
                     mma16816(sc[1], qa[ks], b[2], b[3]);
                 }
@@ -197,10 +242,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                 if (key0 + 16u > hi_all) {
                     const uint32_t from = hi_all - key0;   // 1 .. 15
                     for (uint32_t j = lane; j < (16u - from) * (D / 8u); j += 32u) {
-                        const uint32_t r = 16u * warp + from + j / (D / 8u), c = j % (D / 8u);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tv + (c >> 3) * (KEYS * 128u) + r * 128u + ((c & 7u) << 4)),
-                                     "r"(0u)
-                                     : "memory");
+                        const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tv + (c >> 3) * atom + r * 128u + ((c & 7u) << 4)), "r"(0u) : "memory");
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (before TMA writes there again)
                     __syncwarp();
@@ -252,7 +295,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                 for (int np = 0; np < NT / 2; ++np) {   // columns 16 np .. 16 np + 15
                     const uint32_t piece = 2u * (np & 3) + lv_nt;
                     uint32_t b[4];
-                    ldsm_x4_trans(b, tv + (np >> 2) * (KEYS * 128u) + lv_row * 128u + ((piece ^ (lv_row & 7u)) << 4));
+                    ldsm_x4_trans(b, tv + (np >> 2) * atom + lv_row * 128u + ((piece ^ (lv_row & 7u)) << 4));
                     mma16816(oc[2 * np], ph, b[0], b[1]);
                     mma16816(oc[2 * np + 1], ph, b[2], b[3]);
                     if (EXACT) {
@@ -265,83 +308,75 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             if (lane == 0u) mbar_arrive(empty + 8u * ring.idx);
             ring.advance();
         }
-        done += p.b - p.a;
-
-        // ---- the warps' results as one: maxima, then eight rows at a time through shared memory ----
-        const bool whole = p.a == 0u && p.b == p.n;
-        float* slot = pc.slots + (uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * kDecRows * (D + 4u);
 #pragma unroll
         for (uint32_t h = 0; h < H; ++h) {
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
-            if (t4 == 0u) {
-                s_m[warp * kDecRows + g + 8u * h] = m_run[h];
-                s_l[warp * kDecRows + g + 8u * h] = l_run[h];
+        }
+        // ---- the warps of a head as one: the upper half of the blocks hands its rows to the lower, until one is left ----
+        for (uint32_t n = KB >> 1; n; n >>= 1) {
+#pragma unroll
+            for (uint32_t h = 0; h < H; ++h) {
+                if (h * 8u >= rows) break;
+                float* row = s_merge + (((kb & (n - 1u)) * HB + hb) * 8u + g) * (D + 4u);
+                worker_sync<W * 32u>();   // (the rows written before have been read)
+                if (mine && kb >= n && kb < 2u * n) store_part<NT>(row, t4, m_run[h], l_run[h], oc, h);
+                worker_sync<W * 32u>();
+                if (mine && kb < n) {
+                    const float2 ml = *reinterpret_cast<const float2*>(row);
+                    const float top = fmaxf(m_run[h], ml.x), f0 = weight(m_run[h], top), f1 = weight(ml.x, top);
+                    m_run[h] = top;
+                    l_run[h] = l_run[h] * f0 + ml.y * f1;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float2 y = *reinterpret_cast<const float2*>(row + 4u + 8u * nt + 2u * t4);
+                        oc[nt][2u * h] = (f0 != 0.0f ? oc[nt][2u * h] * f0 : 0.0f) + (f1 != 0.0f ? y.x * f1 : 0.0f);
+                        oc[nt][2u * h + 1u] = (f0 != 0.0f ? oc[nt][2u * h + 1u] * f0 : 0.0f) + (f1 != 0.0f ? y.y * f1 : 0.0f);
+                    }
+                }
             }
         }
-        worker_sync<W * 32u>();
+        // ---- results ----
+        if (mine && kb == 0u && ok) {
+            const bool whole = p.a == 0u && p.b == p.n;
+            float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * HB + hb) * kDecRows * (D + 4u);
 #pragma unroll
-        for (uint32_t h = 0; h < H; ++h) {
-            if (h * 8u >= rows) break;
-            float mx = neg_inf();
+            for (uint32_t h = 0; h < H; ++h) {
+                float check = 0.0f;   // NaN once a column is not finite
 #pragma unroll
-            for (uint32_t w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w * kDecRows + g + 8u * h]);
-            const float f = weight(m_run[h], mx);
-            float* mine = s_merge + ((warp & (W / 2u - 1u)) * 8u + g) * (D + 4u);
-            if (warp >= W / 2u) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    *reinterpret_cast<float2*>(mine + 8 * nt + 2 * t4) =
-                        f == 0.0f ? make_float2(0.f, 0.f) : make_float2(oc[nt][2u * h] * f, oc[nt][2u * h + 1u] * f);
-            }
-            worker_sync<W * 32u>();
-            if (warp < W / 2u) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float2* at = reinterpret_cast<float2*>(mine + 8 * nt + 2 * t4);
-                    const float2 x = *at;
-                    *at = f == 0.0f ? x : make_float2(fmaf(oc[nt][2u * h], f, x.x), fmaf(oc[nt][2u * h + 1u], f, x.y));
-                }
-            }
-            worker_sync<W * 32u>();
-            for (uint32_t i = warp; i < 8u; i += W) {   // a warp per row
-                const uint32_t r = 8u * h + i;
-                if (r >= rows || !ok) break;
-                float m = neg_inf(), l = 0.0f;
-#pragma unroll
-                for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, s_m[w * kDecRows + r]);
-#pragma unroll
-                for (uint32_t w = 0; w < W; ++w) l = fmaf(s_l[w * kDecRows + r], weight(s_m[w * kDecRows + r], m), l);
-                float o[C], check = 0.0f;
-#pragma unroll
-                for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
-#pragma unroll
-                for (uint32_t w = 0; w < W / 2u; ++w)
-#pragma unroll
-                    for (uint32_t c = 0; c < C; ++c) o[c] += s_merge[(w * 8u + i) * (D + 4u) + C * lane + c];
-#pragma unroll
-                for (uint32_t c = 0; c < C; ++c) check = fmaf(o[c], 0.0f, check);
-                const uint32_t row = p.r0 + r, token = p.q.tok0 + row / pc.G, head = p.hkv * pc.G + row % pc.G;
+                for (int nt = 0; nt < NT; ++nt) check = fmaf(oc[nt][2u * h], 0.0f, fmaf(oc[nt][2u * h + 1u], 0.0f, check));
+                check += __shfl_xor_sync(0xffffffffu, check, 1);
+                check += __shfl_xor_sync(0xffffffffu, check, 2);
                 // (a sum that is not finite says that the scores are not: the row is NaN either way)
-                if (__any_sync(0xffffffffu, check != 0.0f) && l - l == 0.0f) {
-                    const Span s = row_span(pc, p.q, row);
-                    const uint32_t from = max(s.lo, (p.first + p.a) * KEYS), to = min(s.hi, (p.first + p.b) * KEYS);
-                    seen_keys_row<C>(pc, p.q, p.hkv, pc.q + (uint64_t)token * pc.q_s + (uint64_t)head * D, from, to, m == neg_inf() ? 0.0f : m, o);
+                const bool again = valid[h] && check != 0.0f && l_run[h] - l_run[h] == 0.0f;
+                if (valid[h] && !again) {
+                    if (whole && pc.out != OUT_PARTS) finish_fragment<NT>(pc, token[h], head[h], t4, m_run[h], l_run[h], oc, h);
+                    else
+                        store_part<NT>(whole ? reinterpret_cast<float*>(pc.dst) + dst_row(pc, token[h], head[h], D) : slot + (uint64_t)(g + 8u * h) * (D + 4u),
+                                       t4, m_run[h], l_run[h], oc, h);
                 }
-                if (whole) {
-                    finish_row<C>(pc, token, head, m, l, o);
-                } else {
-                    float* to = slot + (uint64_t)r * (D + 4u);
-                    if (lane == 0u) *reinterpret_cast<float2*>(to) = make_float2(m, l);
+                for (uint32_t bad = __ballot_sync(0xffffffffu, again && t4 == 0u); bad; bad &= bad - 1u) {   // by the whole warp
+                    const int from = __ffs(bad) - 1;
+                    const uint32_t r = p.r0 + (uint32_t)from / 4u + 8u * h, tk = p.q.tok0 + r / pc.G, hd = hkv * pc.G + r % pc.G;
+                    const float m = __shfl_sync(0xffffffffu, m_run[h], from), l = __shfl_sync(0xffffffffu, l_run[h], from);
+                    const Span s = row_span(pc, p.q, r);
+                    float o[C];
+                    seen_keys_row<C>(pc, p.q, hkv, pc.q + (uint64_t)tk * pc.q_s + (uint64_t)hd * D, max(s.lo, (p.first + p.a) << pc.keys_log2),
+                                     min(s.hi, (p.first + p.b) << pc.keys_log2), m == neg_inf() ? 0.0f : m, o);
+                    if (whole) {
+                        finish_row<C>(pc, tk, hd, m, l, o);
+                    } else {
+                        float* to = slot + (uint64_t)(r - p.r0) * (D + 4u);
+                        if (lane == 0u) *reinterpret_cast<float2*>(to) = make_float2(m, l);
 #pragma unroll
-                    for (uint32_t c = 0; c < C; c += 2u) *reinterpret_cast<float2*>(to + 4u + C * lane + c) = make_float2(o[c], o[c + 1u]);
+                        for (uint32_t c = 0; c < C; ++c) to[4u + C * lane + c] = o[c];
+                    }
                 }
             }
-            worker_sync<W * 32u>();   // (the memory is written again)
         }
         if (p.a == 0u && p.b < p.n) {
             cut = true;
-            if (threadIdx.x == 0u) note_cut(pc, st, p, rows, done);
+            if (threadIdx.x == 0u) note_cut(pc, st, p, rows);
         }
     }
     if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[2u * blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
@@ -357,18 +392,18 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
     const uint4 note = pc.cut[2u * cta];
     const uint32_t parts = note.x, tok0 = note.y, r0 = note.z, rows = note.w;
     if (parts == 0u) return;
-    const uint32_t hkv = pc.cut[2u * cta + 1u].x;
+    const uint32_t hkv0 = pc.cut[2u * cta + 1u].x * pc.HB, all = min(pc.HB, pc.n_head_kv - hkv0) * rows;   // rows of every head
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     __shared__ float s_ml[kMergeWarps][2], s_o[kMergeWarps][D];
     const uint32_t share = parts <= 8u ? 1u : parts <= 16u ? 2u : parts <= 32u ? 4u : kMergeWarps, at_once = kMergeWarps / share;
     const uint32_t begin = warp % share;
-    for (uint32_t base = chunk * at_once; base < rows; base += chunks * at_once) {
-        const uint32_t r = base + warp / share;
+    for (uint32_t base = chunk * at_once; base < all; base += chunks * at_once) {
+        const uint32_t i_row = base + warp / share, hb = i_row / rows, r = i_row - hb * rows;
         float m = neg_inf(), l = 0.0f, o[C];
 #pragma unroll
         for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
-        if (r < rows) {
-            auto part = [&](uint32_t i) { return pc.slots + ((uint64_t)(i == 0u ? 2u * cta + 1u : 2u * (cta + i)) * tile_rows + r) * ROW; };
+        if (i_row < all) {
+            auto part = [&](uint32_t i) { return pc.slots + (((uint64_t)(i == 0u ? 2u * cta + 1u : 2u * (cta + i)) * pc.HB + hb) * tile_rows + r) * ROW; };
             float x[8][C], ml[8][2];   // eight parts on their way together
             for (uint32_t i0 = begin; i0 < parts; i0 += 8u * share) {
                 float top = m;
@@ -411,7 +446,7 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
 #pragma unroll
             for (uint32_t c = 0; c < C; ++c) s_o[warp][C * lane + c] = o[c];
             __syncthreads();
-            if (begin == 0u && r < rows) {
+            if (begin == 0u && i_row < all) {
                 m = neg_inf();
                 for (uint32_t w = warp; w < warp + share; ++w) m = fmaxf(m, s_ml[w][0]);
                 l = 0.0f;
@@ -427,9 +462,9 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
             __syncthreads();
             if (begin != 0u) continue;
         }
-        if (r < rows) {
+        if (i_row < all) {
             const uint32_t row = r0 + r;
-            finish_row<C>(pc, tok0 + row / pc.G, hkv * pc.G + row % pc.G, m, l, o);
+            finish_row<C>(pc, tok0 + row / pc.G, (hkv0 + hb) * pc.G + row % pc.G, m, l, o);
         }
     }
 }
@@ -461,20 +496,20 @@ static bool launch_rows(const LaunchArgs& a, const Args& pc, const Maps& maps, u
 }
 
 static bool launch_merge(const LaunchArgs& a, const Args& x, const Args& y, uint32_t D, uint32_t n_x, uint32_t n_y, uint32_t rows_x, uint32_t rows_y) {
-    const dim3 grid(n_x + n_y, n_y ? 16 : 4), block(kMergeWarps * 32);
+    const dim3 grid(n_x + n_y, 16), block(kMergeWarps * 32);
     if (D == 64u) launch_pdl(paged_merge_kernel<2>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
     else if (D == 128u) launch_pdl(paged_merge_kernel<4>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
     else launch_pdl(paged_merge_kernel<8>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
     return true;
 }
 
-// [pages][heads][tokens][D] f16 with the caller's strides, boxes of `tokens` x 64 columns
-static bool encode_cache(tc::EncodeTiledFn enc, CUtensorMap* map, const void* ptr, const Args& pc, uint32_t D, uint32_t tokens) {
+// [pages][heads][tokens][D] f16 with the caller's strides, boxes of 64 columns x `tokens` x `heads`
+static bool encode_cache(tc::EncodeTiledFn enc, CUtensorMap* map, const void* ptr, const Args& pc, uint32_t D, uint32_t tokens, uint32_t heads) {
     const uint32_t P = 1u << pc.page_log2;
     const cuuint64_t dims[4] = {D, P, pc.n_head_kv, pc.n_pages};
     // (the stride of a dimension of one element is never used, but has to be a valid one)
     const cuuint64_t strides[3] = {2ull * pc.c_ts, pc.n_head_kv > 1u ? 2ull * pc.c_hs : 2ull * D, pc.n_pages > 1u ? 2ull * pc.c_ps : 2ull * D};
-    const cuuint32_t box[4] = {64, tokens, 1, 1}, estr[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, tokens, heads, 1}, estr[4] = {1, 1, 1, 1};
     if (!strides[0] || !strides[1] || !strides[2]) return false;
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -555,6 +590,13 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
 
 // Which kernel a sequence of R rows per KV head runs in: up to kFewRows in paged_rows_kernel, more in paged_tc.cu's (D 64, 128).
 constexpr uint32_t kFewRows = 64;
+// What a row tile costs beside its key tiles, in key tiles (the line's allowance).
+constexpr uint32_t kFewOver = 2, kManyOver = 1;
+// KV heads that paged_rows_kernel takes at once: all of them where its warps suffice, otherwise equal groups
+static uint32_t few_heads(uint32_t D, uint32_t n_head_kv) {
+    const uint32_t W = D == 256u ? 4u : 8u, groups = (n_head_kv + W - 1u) / W;
+    return (n_head_kv + groups - 1u) / groups;
+}
 
 struct Scratch {   // taken from the front
     uint8_t* at;
@@ -585,16 +627,27 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
     many.min_rows = pc.prefix ? 1u : kFewRows + 1u;   // (a prefix has one number of rows, and one kernel)
     many.max_rows = 0xFFFFFFFFu;
     const bool use_few = !both || !pc.prefix, use_many = both;
+    few.HB = few_heads(D, pc.n_head_kv);
+    few.groups = (pc.n_head_kv + few.HB - 1u) / few.HB;
+    const uint32_t kb = blocks_of(D == 256u ? 4u : 8u, few.HB);
+    for (few.keys_log2 = 4u; (16u << (few.keys_log2 - 4u)) < 16u * kb; ++few.keys_log2) {}
+    few.over = kFewOver;
+    many.HB = 1u;
+    many.groups = pc.n_head_kv;
+    many.keys_log2 = 7u;
+    many.over = kManyOver;
     // the line's length in 32 bits
-    const uint32_t keys = D == 256u ? 64u : 128u;
-    const uint64_t few_rows = both ? kFewRows : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs, tiles = ((uint64_t)pc.max_kv + keys - 1u) / keys + 1u;
-    if (use_few && seqs * pc.n_head_kv * ((few_rows + 15u) / 16u) * tiles > 0xFFFFFFFFull) return AC_ERR_INVALID_SHAPE;
-    if (use_many && seqs * pc.n_head_kv * ((max_rows + kTcRows - 1u) / kTcRows) * tiles > 0xFFFFFFFFull) return AC_ERR_INVALID_SHAPE;
+    const uint64_t few_rows = both ? kFewRows : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs;
+    auto too_long = [&](const Args& x, uint64_t row_tiles) {
+        return seqs * x.groups * row_tiles * (((uint64_t)pc.max_kv >> x.keys_log2) + 2u + x.over) > 0xFFFFFFFFull;
+    };
+    if (use_few && too_long(few, (few_rows + kDecRows - 1u) / kDecRows)) return AC_ERR_INVALID_SHAPE;
+    if (use_many && too_long(many, (max_rows + kTcRows - 1u) / kTcRows)) return AC_ERR_INVALID_SHAPE;
     uint32_t n_few = 0, n_many = 0;
     if (use_few) {
-        n_few = ctas_for(use_many ? scratch.left / 8u : scratch.left, kDecRows * row, sms);
+        n_few = ctas_for(use_many ? scratch.left * few.HB / (few.HB + 16u) : scratch.left, few.HB * kDecRows * row, sms);
         few.cut = (uint4*)scratch.take(n_few * 32ull);
-        few.slots = (float*)scratch.take(n_few > 1u ? 2ull * n_few * kDecRows * row : 0u);
+        few.slots = (float*)scratch.take(n_few > 1u ? 2ull * n_few * few.HB * kDecRows * row : 0u);
         if (!few.cut || !few.slots) n_few = 1u, few.cut = nullptr, few.slots = nullptr;
     }
     if (use_many) {
@@ -612,10 +665,10 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
 
 static AcResult cache_maps(const LaunchArgs& a, const Args& pc, uint32_t D, Maps& rows_maps, Maps& tc_maps) {
     tc::EncodeTiledFn enc = tc::encode_fn();
-    const uint32_t P = 1u << pc.page_log2, keys = D == 256u ? 64u : 128u, rows_box = P < keys ? P : keys, tc_box = P < kTcKeys ? P : kTcKeys;
+    const uint32_t P = 1u << pc.page_log2, heads = few_heads(D, pc.n_head_kv), tc_box = P < kTcKeys ? P : kTcKeys;
     if (!enc) return AC_ERR_DRIVER_SYMBOL_MISSING;
-    const bool ok = encode_cache(enc, &rows_maps.k, a.ptr[1], pc, D, rows_box) && encode_cache(enc, &rows_maps.v, a.ptr[2], pc, D, rows_box) &&
-                    encode_cache(enc, &tc_maps.k, a.ptr[1], pc, D, tc_box) && encode_cache(enc, &tc_maps.v, a.ptr[2], pc, D, tc_box);
+    const bool ok = encode_cache(enc, &rows_maps.k, a.ptr[1], pc, D, 16u, heads) && encode_cache(enc, &rows_maps.v, a.ptr[2], pc, D, 16u, heads) &&
+                    encode_cache(enc, &tc_maps.k, a.ptr[1], pc, D, tc_box, 1u) && encode_cache(enc, &tc_maps.v, a.ptr[2], pc, D, tc_box, 1u);
     return ok ? AC_SUCCESS : AC_ERR_INVALID_SHAPE;
 }
 
@@ -629,7 +682,7 @@ static AcResult cache_maps(const LaunchArgs& a, const Args& pc, uint32_t D, Maps
 // Query j of a sequence's n stands at place kv_len - n + j and sees the keys up to there; one that sees none is zero. Rows behind the
 // last sequence are left as they are. Sequences whose numbers do not fit the buffers or the announced maxima are left out, keys on
 // pages that are none of the cache's are not seen; both are counted. The results do not depend on the scratch's contents, and with the
-// same scratch size and maxima not on the run; a larger scratch (up to 2 x SMs x 272 rows) allows more CTAs.
+// same scratch size and maxima not on the run; a larger scratch (up to 2 x SMs x 384 rows of D + 4 floats) allows more CTAs.
 AcResult launch_paged_attn(const LaunchArgs& a) {
     using namespace paged;
     Args pc;

@@ -190,12 +190,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     fence_async_smem();
     pdl_wait();
     tc_fence_before();
-    const uint32_t total = build_line<kTcRows, kTcKeys, kTcThreads / 32u>(pc, s_pref, s_warp);   // (its barriers publish the above)
+    const uint32_t total = build_line<kTcRows, kTcThreads / 32u>(pc, s_pref, s_warp);   // (its barriers publish the above)
     tc_fence_after();
     pdl_trigger();   // not before the tensor memory is this CTA's
     const uint32_t tmem = ctl->tmem_base;
     const Stretch st = my_stretch(total);
-    Walk<kTcRows, kTcKeys> walk(st);
+    Walk<kTcRows> walk(st);
     const uint32_t P = 1u << pc.page_log2, box = P < kTcKeys ? P : kTcKeys, boxes = kTcKeys / box;
     bool ok = true;
 
@@ -235,7 +235,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (lane < boxes && (load >> lane & 1u))
                         for (uint32_t a = 0; a < A; ++a)
                             tma_box(stage + a * (kTcKeys * 128u) + lane * box * 128u, kv ? &v_map : &k_map, full, (int)(64u * a), (int)(b0 & (P - 1u)),
-                                    (int)p.hkv, page);
+                                    (int)p.group, page);
                     if (kv) ++v_issued;
                     else ++k_issued;
                     r.advance();
@@ -368,7 +368,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 const uint32_t r = i * PER + lane / PIECES, row = x.r0 + r, to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
                 if (r < x.rows)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to),
-                                 "l"(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.hkv * pc.G + row % pc.G) * D + 8u * c)
+                                 "l"(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.group * pc.G + row % pc.G) * D + 8u * c)
                                  : "memory");
                 else
                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0u) : "memory");
@@ -382,7 +382,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, ts = tmem + lanes + g * kTcKeys, to = tmem + lanes + 2u * kTcKeys + g * D;
-        uint32_t s_uses = 0, pv_uses = 0, tiles = 0, at = st.begin;
+        uint32_t s_uses = 0, pv_uses = 0, tiles = 0;
         bool cut = false;
         while (walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
@@ -478,9 +478,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             if (!ok) break;
             tc_fence_after();
             tiles += p.b - p.a;
-            at += p.b - p.a;
             if (x.rows) {
-                const uint32_t token = p.q.tok0 + row / pc.G, head = p.hkv * pc.G + row % pc.G;
+                const uint32_t token = p.q.tok0 + row / pc.G, head = p.group * pc.G + row % pc.G;
                 float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * kTcRows + (x.r0 - p.r0)) * (D + 4u);
                 const bool parts = !whole || pc.out == OUT_PARTS;
                 float own = 1.0f, other = 0.0f;      // factors of the values here and of those over other keys
@@ -557,11 +556,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 // rows that are not finite although their sum is: over the keys they see, by the whole warp
                 for (uint32_t again = __ballot_sync(0xffffffffu, valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
                     const int i = __ffs(again) - 1;
-                    const uint32_t r = x.r0 + (warp & 3u) * 32u + (uint32_t)i, tk = p.q.tok0 + r / pc.G, hd = p.hkv * pc.G + r % pc.G;
+                    const uint32_t r = x.r0 + (warp & 3u) * 32u + (uint32_t)i, tk = p.q.tok0 + r / pc.G, hd = p.group * pc.G + r % pc.G;
                     const float m = __shfl_sync(0xffffffffu, m_run, i), l = __shfl_sync(0xffffffffu, l_run, i);
                     const Span sp = row_span(pc, p.q, r);
                     float o[C];
-                    seen_keys_row<C>(pc, p.q, p.hkv, pc.q + (uint64_t)tk * pc.q_s + (uint64_t)hd * D, max(sp.lo, (p.first + p.a) * kTcKeys),
+                    seen_keys_row<C>(pc, p.q, p.group, pc.q + (uint64_t)tk * pc.q_s + (uint64_t)hd * D, max(sp.lo, (p.first + p.a) * kTcKeys),
                                      min(sp.hi, (p.first + p.b) * kTcKeys), m == neg_inf() ? 0.0f : m, o);
                     if (whole) {
                         finish_row<C>(pc, tk, hd, m, l, o);
@@ -574,7 +573,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             }
             if (p.a == 0u && p.b < p.n) {
                 cut = true;
-                if (threadIdx.x == 0u) note_cut(pc, st, p, min(kTcRows, p.R - p.r0), at);
+                if (threadIdx.x == 0u) note_cut(pc, st, p, min(kTcRows, p.R - p.r0));
             }
             tc_fence_before();   // (the next P V overwrites the accumulator behind an arrival of this thread)
         }

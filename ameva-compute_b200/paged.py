@@ -130,8 +130,8 @@ def record_prefix_attention(batch: rt.Batch, cache: Cache, seqs: Sequences, q: r
 
 
 def scratch_bytes(ctx: rt.Context, seqs: Sequences, *, heads: int, head_dim: int, prefix: bool = False, sms: int = 148) -> int:
-    """Bytes of scratch with which the attention of this batch takes the whole GPU: two row tiles of 16 and of 256 rows per SM, and for a
-    shared prefix the rows' results over their own keys."""
+    """Bytes of scratch with which the attention of this batch takes the whole GPU: per SM two row tiles of 16 rows of eight KV heads and
+    two of 256 rows, and for a shared prefix the rows' results over their own keys."""
     row = (head_dim + 4) * 4
     own = seqs.rows * heads * row + 256 if prefix else 0
-    return own + sms * (2 * (16 + 256) * row + 64) * 8 // 7 + 4096
+    return own + sms * (2 * (8 * 16 + 256) * row + 128) + 8192

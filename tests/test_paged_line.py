@@ -1,4 +1,4 @@
-"""How the work of a ragged batch is dealt to CTAs (csrc/paged.cuh), restated: every (sequence, KV head, row tile, key tile) belongs to one
+"""How the work of a ragged batch is dealt to CTAs (csrc/paged.cuh), restated: every (sequence, head group, row tile, key tile) belongs to one
 CTA's stretch of the line, a cut row tile's parts lie in the slots where the merge looks for them, and no slot is written twice."""
 import random
 
@@ -18,7 +18,7 @@ def tile_range(n_q, kv, G, window, keys, r0, r1):
 
 
 def line(seqs, Hkv, G, window, rows, keys):
-    """[(seq, head, first row, first key tile, key tiles)] in the line's order."""
+    """[(seq, head group, first row, first key tile, key tiles)] in the line's order."""
     out = []
     for s, (n_q, kv) in enumerate(seqs):
         R = n_q * G
@@ -39,8 +39,9 @@ def test_stretches_cover_the_line_and_parts_meet(seed):
     G, Hkv, window = rng.randint(1, 9), rng.randint(1, 4), rng.choice([0, 0, rng.randint(1, 400)])
     top = rng.choice([1, 6, 400])
     seqs = [(rng.randint(0, top), rng.choice([0, rng.randint(1, 3000)])) for _ in range(rng.randint(1, 12))]
+    over = rng.randint(0, 3)      # places behind a row tile's key tiles that stand for its other work
     items = line(seqs, Hkv, G, window, rows, keys)
-    total = sum(x[4] for x in items)
+    total = sum(x[4] + over for x in items)
     grid = rng.choice([1, 5, 148])
     ctas = min(grid, total)
     starts = [c * total // ctas for c in range(ctas + 1)] if ctas else [0]
@@ -48,25 +49,24 @@ def test_stretches_cover_the_line_and_parts_meet(seed):
     begin_of, at = [], 0
     for x in items:
         begin_of.append(at)
-        at += x[4]
+        at += x[4] + over
     for c in range(ctas):
-        assert starts[c] < starts[c + 1]      # no CTA in front of the last one is idle
         t, cut = starts[c], 0
         i = max(j for j, b in enumerate(begin_of) if b <= t)
         while t < starts[c + 1]:
-            n = items[i][4]
-            a = t - begin_of[i]
-            b = min(n, a + starts[c + 1] - t)
-            t += b - a
-            if a == 0 and b == n:
+            n, rem = items[i][4], t - begin_of[i]
+            step = min(n + over - rem, starts[c + 1] - t)
+            a, b = min(rem, n), min(n, rem + step)
+            t += step
+            if b > a and a == 0 and b == n:
                 finished.append(i)
-            else:
+            elif b > a:
                 slot = 2 * c + (1 if a == 0 else 0)
                 assert slot not in slots and slot < 2 * grid
                 slots[slot] = (i, a, b)
                 if a == 0:
                     cut += 1
-                    noted[c] = (i, last_cta(t + n - b, ctas, total) - c + 1)
+                    noted[c] = (i, last_cta(begin_of[i] + n, ctas, total) - c + 1)
             i += 1
         assert cut <= 1
     for c, (i, parts) in noted.items():
