@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "sync_ptx.cuh"
 
 namespace amv {
 namespace paged {
@@ -33,7 +34,7 @@ struct Args {
     const int32_t* prefix;      // prefix launch: [0] keys, [1 ..] pages; otherwise null
     void* dst;
     float* slots;               // results of cut row tiles: slot 2 c (a tile begun elsewhere), 2 c + 1 (one that goes on elsewhere)
-    uint4* cut;                 // per CTA two words of four: what the merge kernel needs of a cut row tile
+    uint4* cut;                 // per CTA what the merge kernel needs of a cut row tile: parts | group << 16 (0: none), first token, first row, rows
     uint32_t HB, groups, keys_log2, over;   // KV heads of a group, groups, the line's tiles and its allowance per row tile
     const float* extra;         // results over other keys of the same rows that the final ones take in (the layout of OUT_PARTS)
     uint32_t* refused;          // the caller's status words: count of refused entries, lowest node
@@ -268,10 +269,24 @@ struct Walk {
 // Notes for the merge kernel what the CTA's last piece leaves (the first word 0: nothing).
 __device__ __forceinline__ void note_cut(const Args& pc, const Stretch& x, const Piece& p, uint32_t rows) {
     const uint32_t last = last_cta(x, p.begin + p.n);
-    pc.cut[2u * blockIdx.x] = make_uint4(last - blockIdx.x + 1u, p.q.tok0, p.r0, rows);
-    pc.cut[2u * blockIdx.x + 1u] = make_uint4(p.group, 0u, 0u, 0u);
+    pc.cut[blockIdx.x] = make_uint4((last - blockIdx.x + 1u) | p.group << 16, p.q.tok0, p.r0, rows);
 }
 
+// mbar_wait (sync_ptx.cuh) without a call: the registers of a warp whose share setmaxnreg has changed leave no room for a callee's.
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, ptx::Ctl* ctl, uint32_t* status, uint32_t tag) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!ptx::mbar_try_wait(bar, parity)) {
+        if (ctl->abort) return false;
+        if (clock64() - t0 > ptx::kWaitCycles) {
+            ctl->abort = 1u;
+            if (atomicCAS(status, DEV_STATUS_OK, DEV_STATUS_WAIT_TIMEOUT) == DEV_STATUS_OK) status[1] = tag;
+            return false;
+        }
+    }
+    return true;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -2,9 +2,9 @@
 // long prefix. Here: the kernel for few rows per sequence (tokens, drafts), the merge kernel and the launchers; many rows per
 // sequence (prompts, the prefix of a batch) run in paged_tc.cu.
 //
-// paged_rows_kernel: W + 1 warps. The last one streams key tiles (KB blocks of 16 keys of HB KV heads, K and V) through a ring in shared
+// paged_rows_kernel: W + 1 warps. The last one streams key tiles (KB x 32 keys of HB KV heads; K and V in turn) through a ring in shared
 // memory with TMA, a box of 64 columns x 16 keys x HB heads each, and runs ahead across the pieces of the CTA's stretch, so that the
-// reads never pause. Each of the others takes one head and one block of 16 keys of every tile for the tile's 16 rows: both products on
+// reads never pause. Each of the others takes one head and 32 keys of every tile for the row tile's 16 rows: both products on
 // mma.sync (f16 in, f32 out), an online softmax per row to base 2, the scores' accumulators reused as the A operand of the second
 // product. With W = HB (eight KV heads, say) a warp owns its head's rows from the first key to the last and the warps never meet; with
 // fewer heads the KB warps of a head are joined pairwise through shared memory at the end of a piece. All heads of a block of keys are
@@ -13,6 +13,7 @@
 // bytes, and 8 us per (sequence, head). P: for an f32 result as an f16 value and its remainder (rounded once, 2^-12 of every probability
 // would show there), for an f16 result rounded once (2^-12 against the 2^-12 of the result itself, averaged over the keys).
 #include <cstring>
+#include <type_traits>
 
 #include "paged.h"
 #include "sync_ptx.cuh"
@@ -26,14 +27,16 @@ using namespace ptx;
 
 template <int D>
 struct Rows {
-    static constexpr uint32_t W = D == 256 ? 4 : 8, ATOMS = D / 64, MAX_STAGES = 8;
-    static constexpr uint32_t BLOCK = 16u * D * 2u;                    // K or V of one head and 16 keys
-    static constexpr uint32_t RING = 3u * 2u * 8u * 16u * 128u * 2u;   // 192 KB
+    static constexpr uint32_t W = D == 256 ? 4 : 8, THREADS = D == 256 ? 160 : 384, ATOMS = D / 64, MAX_STAGES = 8;
+    static constexpr uint32_t RING = 196608u;                          // K and V tiles in turn: three of 64 KB where all warps have work
     static constexpr uint32_t MERGE = (W / 2) * 8u * (D + 4u) * 4u;    // half the warps' results for eight rows
     static constexpr uint32_t FIXED = 1024u + RING + MERGE + 128u + 16u * MAX_STAGES;
+    // Registers a thread after the split between the warps that multiply and the warpgroup of the one that loads (D 64, 128): 256 x 208 +
+    // 128 x 88 = 384 x 168, what the block is launched with.
+    static constexpr bool SPLIT = D != 256;
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
-// How W warps share HB heads: blocks of 16 keys per tile, a power of two
+// How W warps share HB heads: warps (32 keys each) per head and tile, a power of two
 __host__ __device__ constexpr uint32_t blocks_of(uint32_t W, uint32_t HB) { return W >= 8u * HB ? 8u : W >= 4u * HB ? 4u : W >= 2u * HB ? 2u : 1u; }
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
@@ -104,23 +107,23 @@ __device__ __forceinline__ void store_part(float* row, uint32_t t4, float m, flo
 
 // TOP: every row tile has at most eight rows (the upper half of the MMA tile), so the lower half's work is left out.
 template <int D, bool TOP, bool EXACT>
-__global__ void __launch_bounds__((Rows<D>::W + 1) * 32, 1)
+__global__ void __launch_bounds__(Rows<D>::THREADS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args pc) {
     using L = Rows<D>;
-    constexpr uint32_t W = L::W, A = L::ATOMS, C = D / 32, H = TOP ? 1 : 2;
+    constexpr uint32_t W = L::W, A = L::ATOMS, C = D / 32, H = TOP ? 1 : 2;   // H: halves of the MMA tile's rows
     constexpr int KS = D / 16, NT = D / 8;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     float* s_merge = reinterpret_cast<float*>(base + L::RING);                     // [W / 2][8][D + 4]
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_merge + L::MERGE / 4u);         // full, empty
     Ctl* ctl = reinterpret_cast<Ctl*>(bars + 2u * L::MAX_STAGES);
-    uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                       // [W + 1]
-    uint32_t* s_bad = s_warp + W + 1u;                                             // per stage: 16-key blocks whose page is none
+    uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                       // [THREADS / 32]
+    uint32_t* s_bad = s_warp + L::THREADS / 32u;                                             // per K tile: 16-key blocks whose page is none
     uint32_t* s_pref = s_bad + L::MAX_STAGES;
     const uint32_t full = smem_u32(bars), empty = full + 8u * L::MAX_STAGES;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t HB = pc.HB, KB = 1u << (pc.keys_log2 - 4u);
-    const uint32_t half = KB * HB * L::BLOCK, stages = min(L::MAX_STAGES, L::RING / (2u * half));   // bytes of K (and of V) of a tile
+    const uint32_t HB = pc.HB, KB = 1u << (pc.keys_log2 - 5u), atom = HB * 2048u;   // atom: 16 keys x 64 columns of the heads
+    const uint32_t tile = 2u * KB * A * atom, stages = min(L::MAX_STAGES, L::RING / tile);
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < L::MAX_STAGES; ++s) {
             mbar_init(full + 8u * s, 1u);
@@ -131,54 +134,56 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     }
     pdl_trigger();
     pdl_wait();
-    const uint32_t total = build_line<kDecRows, W + 1u>(pc, s_pref, s_warp);   // (its barriers publish the ones above)
+    const uint32_t total = build_line<kDecRows, L::THREADS / 32u>(pc, s_pref, s_warp);   // (its barriers publish the ones above)
     const Stretch st = my_stretch(total);
     Walk<kDecRows> walk(st);
     Ring ring(stages);
     bool ok = true;
 
-    if (warp == W) {   // ---- loads ----
+    if (warp >= W) {   // ---- loads ----
+        if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp != W) return;   // (they fill the warpgroup)
         const uint32_t mask = (1u << pc.page_log2) - 1u;
         uint32_t issued = 0;
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
             const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + kDecRows, p.R) - 1u).hi;
-            for (uint32_t i = p.a; i < p.b; ++i) {
+            for (uint32_t i = p.a; ok && i < p.b; ++i) {
                 const uint32_t key0 = (p.first + i) << pc.keys_log2;
-                // lane b < KB looks block b's page up; blocks that hold a key somebody sees are loaded, box j of 2 A KB by lane j
-                const uint32_t b = lane & (KB - 1u), b0 = key0 + 16u * b, j = lane / KB;
+                // lanes b < 2 KB look block b's page up; blocks that hold a key somebody sees are loaded, 64 columns by lane b + 2 KB j
+                const uint32_t blocks = 2u * KB, b = lane & (blocks - 1u), b0 = key0 + 16u * b;
                 const bool want = b0 < hi && b0 + 16u > lo;
                 const int32_t page = want ? page_of(pc, p.q, b0) : -1;
-                ok = mbar_wait(empty + 8u * ring.idx, ring.phase ^ 1u, ctl, pc.status, 0xC00u);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const uint32_t ours = KB == 32u ? 0xffffffffu : (1u << KB) - 1u;
+                const uint32_t ours = (1u << blocks) - 1u;
                 const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0) & ours, load = __ballot_sync(0xffffffffu, page >= 0) & ours;
-                const uint32_t stage = smem_u32(base) + ring.idx * 2u * half, bar = full + 8u * ring.idx;
-                if (lane == 0u) {
-                    if (none) refuse(pc, __popc(none));
-                    s_bad[ring.idx] = none;
-                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(load) * HB * L::BLOCK * 2u);
+                if (none && lane == 0u) refuse(pc, __popc(none));
+                for (uint32_t kv = 0; kv < 2u; ++kv) {
+                    ok = wait_on(empty + 8u * ring.idx, ring.phase ^ 1u, ctl, pc.status, 0xC00u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint32_t stage = smem_u32(base) + ring.idx * tile, bar = full + 8u * ring.idx;
+                    if (lane == 0u) {
+                        s_bad[ring.idx] = none;
+                        mbar_arrive_expect_tx(bar, (uint32_t)__popc(load) * A * atom);
+                    }
+                    __syncwarp();
+                    for (uint32_t a = lane / blocks; a < A; a += 32u / blocks)
+                        if (page >= 0)
+                            tma_page(stage + (b * A + a) * atom, kv ? &v_map : &k_map, bar, (int)(64u * a), (int)(b0 & mask), (int)(p.group * HB), page);
+                    ++issued;
+                    ring.advance();
                 }
-                __syncwarp();
-                for (uint32_t n = j; n < 2u * A; n += 32u / KB) {   // K and V, 64 columns each
-                    const uint32_t kv = n / A, a = n % A;
-                    if (page >= 0)
-                        tma_page(stage + kv * half + (b * A + a) * (HB * 2048u), kv ? &v_map : &k_map, bar, (int)(64u * a), (int)(b0 & mask),
-                                 (int)(p.group * HB), page);
-                }
-                ++issued;
-                ring.advance();
             }
         }
         if (ctl->abort) {   // copies already requested finish before the CTA leaves
             for (uint32_t i = issued > stages ? issued - stages : 0u; i < issued; ++i)
-                mbar_wait(full + 8u * (i % stages), (i / stages) & 1u, ctl, pc.status, 0xC10u);
+                wait_on(full + 8u * (i % stages), (i / stages) & 1u, ctl, pc.status, 0xC10u);
         }
         return;
     }
 
-    // ---- products: head `hb` of the group, block `kb` of the tile ----
+    if constexpr (L::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ---- products: head `hb` of the group, keys 32 kb .. of the tile ----
     const uint32_t kb = warp / HB, hb = warp - kb * HB;
     const uint32_t g = lane >> 2, t4 = lane & 3u;
     const uint32_t lm_row = (lane & 7u) + ((lane >> 4) << 3), lm_hi = (lane >> 3) & 1u;   // K: key in the block, upper eight columns
@@ -198,7 +203,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 #pragma unroll
         for (uint32_t h = 0; h < 2u; ++h) {
             const uint32_t r = p.r0 + g + 8u * h;
-            valid[h] = mine && h < H && g + 8u * h < rows;
+            valid[h] = mine && g + 8u * h < rows;
             span[h] = valid[h] ? row_span(pc, p.q, r) : Span{0u, 0u};
             token[h] = p.q.tok0 + (valid[h] ? r / pc.G : 0u);
             head[h] = valid[h] ? hkv * pc.G + r % pc.G : 0u;
@@ -217,49 +222,55 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             for (int j = 0; j < 4; ++j) oc[nt][j] = 0.0f;
 
         for (uint32_t i = p.a; i < p.b; ++i) {
-            const uint32_t key0 = ((p.first + i) << pc.keys_log2) + 16u * kb;
-            ok = ok && mbar_wait(full + 8u * ring.idx, ring.phase, ctl, pc.status, 0xC20u);
+            const uint32_t key0 = ((p.first + i) << pc.keys_log2) + 32u * kb;
+            ok = ok && wait_on(full + 8u * ring.idx, ring.phase, ctl, pc.status, 0xC20u);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;   // (the pieces are walked to the end all the same: the warps meet at their barriers)
-            // [block][64 columns][head][16 keys][128 bytes, swizzled]
-            const uint32_t tk = smem_u32(base) + ring.idx * 2u * half + kb * A * HB * 2048u + hb * 2048u, tv = tk + half, atom = HB * 2048u;
-            const bool seen = mine && key0 < hi_all && key0 + 16u > lo_all && !(s_bad[ring.idx] >> kb & 1u);
-            if (seen) {
-                float sc[2][4];
+            // a tile: [block of 16 keys][64 columns][head][16 keys][128 bytes, swizzled]
+            const uint32_t mine_at = 2u * kb * A * atom + hb * 2048u, tk = smem_u32(base) + ring.idx * tile + mine_at, gone = s_bad[ring.idx] >> (2u * kb);
+            bool seen[2];
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+            for (uint32_t kk = 0; kk < 2u; ++kk)
+                seen[kk] = mine && key0 + 16u * kk < hi_all && key0 + 16u * kk + 16u > lo_all && !(gone >> kk & 1u);
+            float sc[4][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sc[nt][j] = 0.0f;
+            for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[nt][j] = 0.0f;
+            if (seen[0] || seen[1]) {
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t piece = 2u * (ks & 3) + lm_hi;
-                    uint32_t b[4];
-                    ldsm_x4(b, tk + (ks >> 2) * atom + lm_row * 128u + ((piece ^ (lm_row & 7u)) << 4));
-                    mma16816(sc[0], qa[ks], b[0], b[1]);
-                    mma16816(sc[1], qa[ks], b[2], b[3]);
-                }
-                // V rows behind the last key are whatever the page holds there: probabilities of zero do not hide a NaN
-                if (key0 + 16u > hi_all) {
-                    const uint32_t from = hi_all - key0;   // 1 .. 15
-                    for (uint32_t j = lane; j < (16u - from) * (D / 8u); j += 32u) {
-                        const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tv + (c >> 3) * atom + r * 128u + ((c & 7u) << 4)), "r"(0u) : "memory");
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) {   // (of a block that is not there: whatever the memory holds, hidden below)
+                        uint32_t b[4];
+                        ldsm_x4(b, tk + (kk * A + (ks >> 2)) * atom + lm_row * 128u + ((piece ^ (lm_row & 7u)) << 4));
+                        mma16816(sc[2 * kk], qa[ks], b[0], b[1]);
+                        mma16816(sc[2 * kk + 1], qa[ks], b[2], b[3]);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (before TMA writes there again)
-                    __syncwarp();
                 }
-                const bool plain = key0 >= lo_both && key0 + 16u <= hi_both;
-                uint32_t ph[4], pl[4];
+            }
+            __syncwarp();
+            if (lane == 0u) mbar_arrive(empty + 8u * ring.idx);
+            ring.advance();
+            uint32_t ph[2][4], pl[2][4];
+            if (seen[0] || seen[1]) {
+                const bool plain = key0 >= lo_both && key0 + 32u <= hi_both && !(gone & 3u);
 #pragma unroll
-                for (uint32_t h = 0; h < H; ++h) {
-                    float x[2][2], mx = neg_inf();
+                for (uint32_t h = 0; h < 2u; ++h) {
+                    if (h >= H) {
 #pragma unroll
-                    for (uint32_t nt = 0; nt < 2u; ++nt)
+                        for (uint32_t kk = 0; kk < 2u; ++kk) ph[kk][1] = ph[kk][3] = pl[kk][1] = pl[kk][3] = 0u;
+                        break;
+                    }
+                    float x[4][2], mx = neg_inf();
+#pragma unroll
+                    for (uint32_t nt = 0; nt < 4u; ++nt)
 #pragma unroll
                         for (uint32_t j = 0; j < 2u; ++j) {
                             const uint32_t key = key0 + 8u * nt + 2u * t4 + j;
                             const float v = score2(pc, sc[nt][2u * h + j]);
-                            x[nt][j] = plain || (key >= span[h].lo && key < span[h].hi) ? v : neg_inf();
+                            x[nt][j] = plain || (key >= span[h].lo && key < span[h].hi && seen[nt >> 1]) ? v : neg_inf();
                             mx = fmaxf(mx, x[nt][j]);
                         }
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -278,29 +289,47 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                     const float ref = m_new == neg_inf() ? 0.0f : m_new;
                     float sum = 0.0f;
 #pragma unroll
-                    for (uint32_t nt = 0; nt < 2u; ++nt) {
+                    for (uint32_t nt = 0; nt < 4u; ++nt) {
                         const float p0 = ex2(x[nt][0] - ref), p1 = ex2(x[nt][1] - ref);
                         sum += p0 + p1;
                         const __half2 hi2 = __floats2half2_rn(p0, p1);
-                        ph[2u * nt + h] = *reinterpret_cast<const uint32_t*>(&hi2);
+                        ph[nt >> 1][2u * (nt & 1u) + h] = *reinterpret_cast<const uint32_t*>(&hi2);
                         if (EXACT) {
                             const float2 f2 = __half22float2(hi2);
-                            pl[2u * nt + h] = halves(p0 - f2.x, p1 - f2.y);
+                            pl[nt >> 1][2u * (nt & 1u) + h] = halves(p0 - f2.x, p1 - f2.y);
                         }
                     }
                     l_run[h] += sum;   // (this lane's keys; the four lanes of a row are added at the end)
                 }
-                if (TOP) ph[1] = ph[3] = pl[1] = pl[3] = 0u;
+            }
+            ok = ok && wait_on(full + 8u * ring.idx, ring.phase, ctl, pc.status, 0xC30u);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t tv = smem_u32(base) + ring.idx * tile + mine_at;
+#pragma unroll
+            for (uint32_t kk = 0; kk < 2u; ++kk) {
+                if (!seen[kk]) continue;
+                const uint32_t v0 = tv + kk * A * atom, k0 = key0 + 16u * kk;
+                // V rows behind the last key are whatever the page holds there: probabilities of zero do not hide a NaN
+                if (k0 + 16u > hi_all) {
+                    const uint32_t from = hi_all - k0;   // 1 .. 15
+                    for (uint32_t j = lane; j < (16u - from) * (D / 8u); j += 32u) {
+                        const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v0 + (c >> 3) * atom + r * 128u + ((c & 7u) << 4)), "r"(0u) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (before TMA writes there again)
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int np = 0; np < NT / 2; ++np) {   // columns 16 np .. 16 np + 15
                     const uint32_t piece = 2u * (np & 3) + lv_nt;
                     uint32_t b[4];
-                    ldsm_x4_trans(b, tv + (np >> 2) * atom + lv_row * 128u + ((piece ^ (lv_row & 7u)) << 4));
-                    mma16816(oc[2 * np], ph, b[0], b[1]);
-                    mma16816(oc[2 * np + 1], ph, b[2], b[3]);
+                    ldsm_x4_trans(b, v0 + (np >> 2) * atom + lv_row * 128u + ((piece ^ (lv_row & 7u)) << 4));
+                    mma16816(oc[2 * np], ph[kk], b[0], b[1]);
+                    mma16816(oc[2 * np + 1], ph[kk], b[2], b[3]);
                     if (EXACT) {
-                        mma16816(oc[2 * np], pl, b[0], b[1]);
-                        mma16816(oc[2 * np + 1], pl, b[2], b[3]);
+                        mma16816(oc[2 * np], pl[kk], b[0], b[1]);
+                        mma16816(oc[2 * np + 1], pl[kk], b[2], b[3]);
                     }
                 }
             }
@@ -309,15 +338,15 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             ring.advance();
         }
 #pragma unroll
-        for (uint32_t h = 0; h < H; ++h) {
+        for (uint32_t h = 0; h < 2u; ++h) {
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
         }
         // ---- the warps of a head as one: the upper half of the blocks hands its rows to the lower, until one is left ----
         for (uint32_t n = KB >> 1; n; n >>= 1) {
 #pragma unroll
-            for (uint32_t h = 0; h < H; ++h) {
-                if (h * 8u >= rows) break;
+            for (uint32_t h = 0; h < 2u; ++h) {
+                if (h >= H) break;
                 float* row = s_merge + (((kb & (n - 1u)) * HB + hb) * 8u + g) * (D + 4u);
                 worker_sync<W * 32u>();   // (the rows written before have been read)
                 if (mine && kb >= n && kb < 2u * n) store_part<NT>(row, t4, m_run[h], l_run[h], oc, h);
@@ -341,7 +370,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             const bool whole = p.a == 0u && p.b == p.n;
             float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * HB + hb) * kDecRows * (D + 4u);
 #pragma unroll
-            for (uint32_t h = 0; h < H; ++h) {
+            for (uint32_t h = 0; h < 2u; ++h) {
+                if (h >= H) break;
                 float check = 0.0f;   // NaN once a column is not finite
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) check = fmaf(oc[nt][2u * h], 0.0f, fmaf(oc[nt][2u * h + 1u], 0.0f, check));
@@ -379,64 +409,132 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             if (threadIdx.x == 0u) note_cut(pc, st, p, rows);
         }
     }
-    if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[2u * blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// Joins the cut row tiles: CTA x of the kernel in front whose last row tile goes on elsewhere has noted it; its parts lie in slot
-// 2 x + 1 and in slots 2 y of the CTAs behind. SHARE warps take the parts of a row in turn, the more the more parts there are; the
-// CTAs of one x share the rows.
-constexpr uint32_t kMergeWarps = 8;
+// Joins the cut row tiles. CTA x of the kernel in front notes a row tile that it begins and others end; its parts lie in slot 2 x + 1 and
+// in slots 2 y of the CTAs behind. The rows of a kernel's notes form one list that the warps of the grid share;
+// SHARE warps take the parts of a row in turn, the more the more parts there are.
+constexpr uint32_t kMergeWarps = 16, kMergeNotes = 512;
+struct MergeSet {
+    Args pc;
+    uint32_t ctas, tile_rows;
+};
 template <uint32_t C>
-__device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_t tile_rows, uint32_t chunk, uint32_t chunks) {
-    constexpr uint32_t D = 32u * C, ROW = D + 4u;
-    const uint4 note = pc.cut[2u * cta];
-    const uint32_t parts = note.x, tok0 = note.y, r0 = note.z, rows = note.w;
-    if (parts == 0u) return;
-    const uint32_t hkv0 = pc.cut[2u * cta + 1u].x * pc.HB, all = min(pc.HB, pc.n_head_kv - hkv0) * rows;   // rows of every head
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+__device__ __forceinline__ void load_columns(const float* p, float (&x)[C]) {   // (16 bytes at a time where there are)
+    if constexpr (C == 2u) {
+        const float2 y = *reinterpret_cast<const float2*>(p);
+        x[0] = y.x;
+        x[1] = y.y;
+    } else {
+#pragma unroll
+        for (uint32_t c = 0; c < C; c += 4u) {
+            const float4 y = *reinterpret_cast<const float4*>(p + c);
+            x[c] = y.x;
+            x[c + 1u] = y.y;
+            x[c + 2u] = y.z;
+            x[c + 3u] = y.w;
+        }
+    }
+}
+template <uint32_t C>
+__device__ __forceinline__ void merge_set(const MergeSet& set) {
+    constexpr uint32_t D = 32u * C, ROW = D + 4u, kTogether = C == 8u ? 4u : 8u;
+    __shared__ uint4 s_note[kMergeNotes];
+    __shared__ uint32_t s_at[kMergeNotes], s_sum[kMergeWarps], s_top[kMergeWarps];   // s_at: rows in front of note i
     __shared__ float s_ml[kMergeWarps][2], s_o[kMergeWarps][D];
-    const uint32_t share = parts <= 8u ? 1u : parts <= 16u ? 2u : parts <= 32u ? 4u : kMergeWarps, at_once = kMergeWarps / share;
+    const Args& pc = set.pc;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, notes = set.ctas;
+    uint32_t total = 0, most = 0;
+    for (uint32_t base = 0; base < notes; base += kMergeWarps * 32u) {   // exclusive sums, a note per thread
+        const uint32_t i = base + threadIdx.x;
+        uint32_t rows = 0, parts = 0;
+        if (i < notes) {
+            const uint4 note = pc.cut[i];
+            s_note[i] = note;
+            parts = note.x & 0xFFFFu;
+            if (parts) rows = min(pc.HB, pc.n_head_kv - (note.x >> 16) * pc.HB) * note.w;
+        }
+        uint32_t incl = rows, top = parts;
+#pragma unroll
+        for (uint32_t o = 1; o < 32u; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+        if (lane == 31u) {
+            s_sum[warp] = incl;
+            s_top[warp] = top;
+        }
+        __syncthreads();
+        uint32_t before = total + incl - rows;
+#pragma unroll
+        for (uint32_t w = 0; w < kMergeWarps; ++w) {
+            before += w < warp ? s_sum[w] : 0u;
+            total += s_sum[w];
+            most = max(most, s_top[w]);
+        }
+        if (i < notes) s_at[i] = before;
+        __syncthreads();
+    }
+    const uint32_t share = most <= 8u ? 1u : most <= 16u ? 2u : most <= 32u ? 4u : most <= 64u ? 8u : kMergeWarps, at_once = kMergeWarps / share;
     const uint32_t begin = warp % share;
-    for (uint32_t base = chunk * at_once; base < all; base += chunks * at_once) {
-        const uint32_t i_row = base + warp / share, hb = i_row / rows, r = i_row - hb * rows;
+    // rows beside one another to a warp (they mostly share their note), `per` of them
+    const uint32_t per = (total + gridDim.x * at_once - 1u) / (gridDim.x * at_once), first = (blockIdx.x * at_once + warp / share) * per;
+    uint32_t note_i = 0, note_end = 0, group = 0;
+    uint4 note = make_uint4(0u, 0u, 0u, 1u);
+    for (uint32_t k = 0; k < per; ++k) {
+        const uint32_t at = first + k;
+        const bool have_row = at < total;
+        if (have_row && at >= note_end) {
+            uint32_t lo = 0, hi = notes;   // the last note with s_at <= at (of equal ones the last, which has the rows)
+            while (hi - lo > 1u) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (s_at[mid] <= at) lo = mid;
+                else hi = mid;
+            }
+            note_i = lo;
+            note_end = lo + 1u < notes ? s_at[lo + 1u] : total;
+            note = s_note[lo];
+            group = note.x >> 16;
+        }
+        const uint32_t parts = note.x & 0xFFFFu, i_row = have_row ? at - s_at[note_i] : 0u, hb = i_row / note.w, r = i_row - hb * note.w;
         float m = neg_inf(), l = 0.0f, o[C];
 #pragma unroll
         for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
-        if (i_row < all) {
-            auto part = [&](uint32_t i) { return pc.slots + (((uint64_t)(i == 0u ? 2u * cta + 1u : 2u * (cta + i)) * pc.HB + hb) * tile_rows + r) * ROW; };
-            float x[8][C], ml[8][2];   // eight parts on their way together
-            for (uint32_t i0 = begin; i0 < parts; i0 += 8u * share) {
-                float top = m;
+        auto part = [&](uint32_t i) { return pc.slots + (((uint64_t)(i == 0u ? 2u * note_i + 1u : 2u * (note_i + i)) * pc.HB + hb) * set.tile_rows + r) * ROW; };
+        auto take = [&](auto n_const, uint32_t i0) {   // some parts on their way together
+            constexpr uint32_t N = decltype(n_const)::value;
+            float x[N][C], ml[N][2], top = m;
 #pragma unroll
-                for (uint32_t j = 0; j < 8u; ++j) {
-                    const uint32_t i = i0 + j * share;
-                    const bool have = i < parts;
-                    const float* p = part(have ? i : begin);
-                    const float2 v = *reinterpret_cast<const float2*>(p);
-                    ml[j][0] = have ? v.x : neg_inf();
-                    ml[j][1] = have ? v.y : 0.0f;
-#pragma unroll
-                    for (uint32_t c = 0; c < C; c += 2u) {
-                        const float2 y = *reinterpret_cast<const float2*>(p + 4u + C * lane + c);
-                        x[j][c] = y.x;
-                        x[j][c + 1u] = y.y;
-                    }
-                }
-#pragma unroll
-                for (uint32_t j = 0; j < 8u; ++j) top = fmaxf(top, ml[j][0]);
-                const float f0 = weight(m, top);
-                m = top;
-                l *= f0;
-#pragma unroll
-                for (uint32_t c = 0; c < C; ++c) o[c] *= f0;
-#pragma unroll
-                for (uint32_t j = 0; j < 8u; ++j) {
-                    const float f = weight(ml[j][0], top);
-                    l = fmaf(ml[j][1], f, l);
-#pragma unroll
-                    for (uint32_t c = 0; c < C; ++c) o[c] += f != 0.0f ? x[j][c] * f : 0.0f;
-                }
+            for (uint32_t j = 0; j < N; ++j) {
+                const uint32_t i = i0 + j * share;
+                const bool have = i < parts;
+                const float* p = part(have ? i : begin);
+                const float2 v = *reinterpret_cast<const float2*>(p);
+                ml[j][0] = have ? v.x : neg_inf();
+                ml[j][1] = have ? v.y : 0.0f;
+                load_columns<C>(p + 4u + C * lane, x[j]);
             }
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) top = fmaxf(top, ml[j][0]);
+            const float f0 = weight(m, top);
+            m = top;
+            l *= f0;
+#pragma unroll
+            for (uint32_t c = 0; c < C; ++c) o[c] *= f0;
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) {
+                const float f = weight(ml[j][0], top);
+                l = fmaf(ml[j][1], f, l);
+#pragma unroll
+                for (uint32_t c = 0; c < C; ++c) o[c] += f != 0.0f ? x[j][c] * f : 0.0f;
+            }
+        };
+        if (have_row && begin < parts) {
+            if (parts <= 2u * share) take(std::integral_constant<uint32_t, 2>(), begin);
+            else
+                for (uint32_t i0 = begin; i0 < parts; i0 += kTogether * share) take(std::integral_constant<uint32_t, kTogether>(), i0);
         }
         if (share > 1u) {
             if (lane == 0u) {
@@ -446,7 +544,7 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
 #pragma unroll
             for (uint32_t c = 0; c < C; ++c) s_o[warp][C * lane + c] = o[c];
             __syncthreads();
-            if (begin == 0u && i_row < all) {
+            if (begin == 0u && have_row) {
                 m = neg_inf();
                 for (uint32_t w = warp; w < warp + share; ++w) m = fmaxf(m, s_ml[w][0]);
                 l = 0.0f;
@@ -462,27 +560,25 @@ __device__ __forceinline__ void merge_tile(const Args& pc, uint32_t cta, uint32_
             __syncthreads();
             if (begin != 0u) continue;
         }
-        if (i_row < all) {
-            const uint32_t row = r0 + r;
-            finish_row<C>(pc, tok0 + row / pc.G, (hkv0 + hb) * pc.G + row % pc.G, m, l, o);
+        if (have_row) {
+            const uint32_t row = note.z + r;
+            finish_row<C>(pc, note.y + row / pc.G, (group * pc.HB + hb) * pc.G + row % pc.G, m, l, o);
         }
     }
+    __syncthreads();   // (the memory is used again)
 }
-// CTAs 0 .. n_first - 1 join the tiles of `a`, the others those of `b`.
 template <uint32_t C>
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ Args a, const __grid_constant__ Args b, uint32_t n_first,
-                                                                       uint32_t rows_a, uint32_t rows_b) {
+__global__ void __launch_bounds__(kMergeWarps * 32, 2) paged_merge_kernel(const __grid_constant__ MergeSet s0, const __grid_constant__ MergeSet s1) {
     pdl_trigger();
     pdl_wait();
-    if (blockIdx.x < n_first) merge_tile<C>(a, blockIdx.x, rows_a, blockIdx.y, gridDim.y);
-    else merge_tile<C>(b, blockIdx.x - n_first, rows_b, blockIdx.y, gridDim.y);
+    if (s0.ctas) merge_set<C>(s0);
+    if (s1.ctas) merge_set<C>(s1);
 }
 
 template <int D, bool TOP, bool EXACT>
 static bool launch_rows_t(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
     if (!ensure_dynamic_smem<paged_rows_kernel<D, TOP, EXACT>>((int)Rows<D>::smem(kMaxSeqs))) return false;
-    launch_pdl(paged_rows_kernel<D, TOP, EXACT>, dim3(ctas), dim3((Rows<D>::W + 1) * 32), Rows<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k,
-               maps.v, pc);
+    launch_pdl(paged_rows_kernel<D, TOP, EXACT>, dim3(ctas), dim3(Rows<D>::THREADS), Rows<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, pc);
     return true;
 }
 template <int D>
@@ -496,10 +592,13 @@ static bool launch_rows(const LaunchArgs& a, const Args& pc, const Maps& maps, u
 }
 
 static bool launch_merge(const LaunchArgs& a, const Args& x, const Args& y, uint32_t D, uint32_t n_x, uint32_t n_y, uint32_t rows_x, uint32_t rows_y) {
-    const dim3 grid(n_x + n_y, 16), block(kMergeWarps * 32);
-    if (D == 64u) launch_pdl(paged_merge_kernel<2>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
-    else if (D == 128u) launch_pdl(paged_merge_kernel<4>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
-    else launch_pdl(paged_merge_kernel<8>, grid, block, 0, a.stream, x, y, n_x, rows_x, rows_y);
+    const MergeSet s0 = {x, n_x, rows_x}, s1 = {y, n_y, rows_y};
+    if (n_x > kMergeNotes || n_y > kMergeNotes) return false;
+    const uint64_t rows = (uint64_t)x.rows * x.n_head, most = 2u * (uint32_t)a.sm_count;   // (no row is cut twice)
+    const dim3 grid((uint32_t)(rows < most ? rows : most)), block(kMergeWarps * 32);
+    if (D == 64u) launch_pdl(paged_merge_kernel<2>, grid, block, 0, a.stream, s0, s1);
+    else if (D == 128u) launch_pdl(paged_merge_kernel<4>, grid, block, 0, a.stream, s0, s1);
+    else launch_pdl(paged_merge_kernel<8>, grid, block, 0, a.stream, s0, s1);
     return true;
 }
 
@@ -591,7 +690,7 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
 // Which kernel a sequence of R rows per KV head runs in: up to kFewRows in paged_rows_kernel, more in paged_tc.cu's (D 64, 128).
 constexpr uint32_t kFewRows = 64;
 // What a row tile costs beside its key tiles, in key tiles (the line's allowance).
-constexpr uint32_t kFewOver = 2, kManyOver = 1;
+constexpr uint32_t kFewOver = 1, kManyOver = 2;
 // KV heads that paged_rows_kernel takes at once: all of them where its warps suffice, otherwise equal groups
 static uint32_t few_heads(uint32_t D, uint32_t n_head_kv) {
     const uint32_t W = D == 256u ? 4u : 8u, groups = (n_head_kv + W - 1u) / W;
@@ -630,11 +729,11 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
     few.HB = few_heads(D, pc.n_head_kv);
     few.groups = (pc.n_head_kv + few.HB - 1u) / few.HB;
     const uint32_t kb = blocks_of(D == 256u ? 4u : 8u, few.HB);
-    for (few.keys_log2 = 4u; (16u << (few.keys_log2 - 4u)) < 16u * kb; ++few.keys_log2) {}
+    for (few.keys_log2 = 5u; (1u << (few.keys_log2 - 5u)) < kb; ++few.keys_log2) {}
     few.over = kFewOver;
     many.HB = 1u;
     many.groups = pc.n_head_kv;
-    many.keys_log2 = 7u;
+    many.keys_log2 = 6u;
     many.over = kManyOver;
     // the line's length in 32 bits
     const uint64_t few_rows = both ? kFewRows : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs;
@@ -646,13 +745,13 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
     uint32_t n_few = 0, n_many = 0;
     if (use_few) {
         n_few = ctas_for(use_many ? scratch.left * few.HB / (few.HB + 16u) : scratch.left, few.HB * kDecRows * row, sms);
-        few.cut = (uint4*)scratch.take(n_few * 32ull);
+        few.cut = (uint4*)scratch.take(n_few * 16ull);
         few.slots = (float*)scratch.take(n_few > 1u ? 2ull * n_few * few.HB * kDecRows * row : 0u);
         if (!few.cut || !few.slots) n_few = 1u, few.cut = nullptr, few.slots = nullptr;
     }
     if (use_many) {
         n_many = ctas_for(scratch.left, kTcRows * row, sms);
-        many.cut = (uint4*)scratch.take(n_many * 32ull);
+        many.cut = (uint4*)scratch.take(n_many * 16ull);
         many.slots = (float*)scratch.take(n_many > 1u ? 2ull * n_many * kTcRows * row : 0u);
         if (!many.cut || !many.slots) n_many = 1u, many.cut = nullptr, many.slots = nullptr;
     }

@@ -1,17 +1,20 @@
 // Attention over a paged KV cache for many rows per sequence (prompts, the shared prefix of a batch; D 64, 128) on the 5th-generation
 // tensor cores. Arguments, rows and the line of work: paged.cuh; launchers: paged_attn.cu.
 //
-// A CTA (one per SM) takes row tiles of 256 rows, two groups of 128, and walks key tiles of 128 for both:
-//   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 128 scores from tensor memory, online softmax to base 2, write P
+// A CTA (one per SM) takes row tiles of 256 rows, two groups of 128, and walks key tiles of 64 for both:
+//   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 64 scores from tensor memory, online softmax to base 2, write P
 //                    over the scores as f16 (and, for a 32-bit result, what that rounding left beside it). The accumulator is rescaled
 //                    only when a row's maximum has grown by more than 2^kGrowth since its last rescale. They write the piece's results.
-//   warp 8           issues the MMAs: S = Q K^T (both in shared memory), O += P V (P in tensor memory, V MN-major): P V of a group and
-//                    its next S leave together, so that the tensor core works on one group while the other's softmax runs
-//   warp 9           streams K and V tiles with TMA, a box of 64 columns x one page each
-//   warps 10, 11     bring the Q rows of group 0 and 1 in, those of the next piece as soon as the last S of this one has read them
-// Tensor memory: two S / P of 128 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
+//   warps 8, 9       issue the MMAs of group 0 and 1: S = Q K^T (both in shared memory), O += P V (P in tensor memory, V MN-major). Each
+//                    group has two S / P tiles; P V of key tile j and S of tile j + 2, which takes its place, leave together, so that a
+//                    group's softmax finds the next scores there while the tensor core works on the other's. A warp per group, and the
+//                    MMAs of a whole tile behind one elected lane: what a warp does around its MMAs takes longer than the MMAs (one
+//                    warp for both groups, an elected lane per MMA: 1240 clocks per group and tile, 640 of them the tensor core's)
+//   warp 10          streams K and V tiles with TMA, a box of 64 columns x one page each, K two tiles ahead of V
+//   warp 11          brings the Q rows in, those of the next piece as soon as the last S of this one has read them
+// Tensor memory: four S / P tiles of 64 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
 // steps of 16 keys that none sees; V rows behind the last key are zeroed before they are multiplied (a page holds anything there).
-// Every wait on a barrier is bounded (sync_ptx.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
+// Every wait on a barrier is bounded (paged.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
 #include <cstring>
 
 #include "paged.h"
@@ -24,34 +27,20 @@ namespace paged {
 using namespace ptx;
 using namespace tc;
 
-constexpr uint32_t kGroupRows = 128, kWarpMma = 8, kWarpLoad = 9, kWarpQ = 10, kTcThreads = 384, kTmemCols = 512, kBadRing = 8;
+constexpr uint32_t kGroupRows = 128, kWarpMma = 8, kWarpLoad = 10, kWarpQ = 11, kTcThreads = 384, kTmemCols = 512, kBadRing = 8;
 // Registers a thread after the split: 256 x 200 + 128 x 104 = 384 x 168, what the block is launched with.
 constexpr uint32_t kSoftmaxRegs = 200, kOtherRegs = 104;
 constexpr float kGrowth = 7.0f;   // probabilities stay below 2^7
 
 template <int D>
 struct Tc {
-    static constexpr uint32_t A = D / 64, STAGES = D == 64 ? 4 : 2;
+    static constexpr uint32_t A = D / 64, STAGES = D == 64 ? 5 : 3;
     static constexpr uint32_t Q = A * kGroupRows * 128u, TILE = A * kTcKeys * 128u;
-    static constexpr uint32_t FIXED = 1024u + 2u * Q + 2u * STAGES * TILE + 512u;
+    static constexpr uint32_t STAGE_OUT = 8u * 32u * 64u;   // a warp's 32 rows x 16 columns on their way out
+    static constexpr uint32_t FIXED = 1024u + 2u * Q + 2u * STAGES * TILE + STAGE_OUT + 512u;
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
 
-// mbar_wait (sync_ptx.cuh) without a call: the registers of a warp whose share setmaxnreg has changed leave no room for a callee's.
-__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, Ctl* ctl, uint32_t* status, uint32_t tag) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-#pragma unroll 1
-    while (!mbar_try_wait(bar, parity)) {
-        if (ctl->abort) return false;
-        if (clock64() - t0 > kWaitCycles) {
-            ctl->abort = 1u;
-            if (atomicCAS(status, DEV_STATUS_OK, DEV_STATUS_WAIT_TIMEOUT) == DEV_STATUS_OK) status[1] = tag;
-            return false;
-        }
-    }
-    return true;
-}
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int page) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map),
@@ -108,18 +97,64 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile(
         "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
+}
+// The MMAs of a whole tile and the commits behind them, one lane elected once. P V of 64 keys:
+template <bool EXACT>
+__device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t bar0, uint32_t bar1) {
+#define AMV_TS(A, B, P) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [" A "], " B ", %3, " P ";\n\t"
+#define AMV_PV_HEAD                                                                                                                            \
+    "{\n\t.reg .pred p, q, t;\n\t.reg .b32 a1, a2, a3, c0, c1, c2, c3;\n\t.reg .b64 b1, b2, b3;\n\telect.sync _|q, 0xffffffff;\n\t"              \
+    "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 t, 0, 0;\n\tadd.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"                         \
+    "add.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\t"
+#define AMV_PV_TAIL                                                                                                                            \
+    "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t"                                                       \
+    "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t}"
+    if constexpr (EXACT)
+        asm volatile(AMV_PV_HEAD "add.u32 c0, %1, 32;\n\tadd.u32 c1, %1, 40;\n\tadd.u32 c2, %1, 48;\n\tadd.u32 c3, %1, 56;\n\t" AMV_TS("%1", "%2", "p")
+                         AMV_TS("a1", "b1", "t") AMV_TS("a2", "b2", "t") AMV_TS("a3", "b3", "t") AMV_TS("c0", "%2", "t") AMV_TS("c1", "b1", "t")
+                             AMV_TS("c2", "b2", "t") AMV_TS("c3", "b3", "t") AMV_PV_TAIL ::"r"(d),
+                     "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(bar0), "r"(bar1)
+                     : "memory");
+    else
+        asm volatile(AMV_PV_HEAD AMV_TS("%1", "%2", "p") AMV_TS("a1", "b1", "t") AMV_TS("a2", "b2", "t") AMV_TS("a3", "b3", "t") AMV_PV_TAIL ::"r"(d), "r"(a),
+                     "l"(b), "r"(idesc), "r"(acc), "r"(bar0), "r"(bar1)
+                     : "memory");
+#undef AMV_TS
+#undef AMV_PV_HEAD
+#undef AMV_PV_TAIL
+}
+// S of 64 keys and 64 A columns of Q and K:
+template <uint32_t A>
+__device__ __forceinline__ void mma_s(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t bar0, uint32_t bar1) {
+    constexpr uint64_t QA = kGroupRows * 128u / 16u, KA = kTcKeys * 128u / 16u;   // to the next 64 columns
+#define AMV_SS(A, B, P) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], " A ", " B ", %3, " P ";\n\t"
+#define AMV_S_HEAD                                                                                                                             \
+    "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a1, a2, a3, a4, a5, a6, a7, b1, b2, b3, b4, b5, b6, b7;\n\telect.sync _|q, 0xffffffff;\n\t"             \
+    "setp.ne.u32 p, 0, 0;\n\tsetp.eq.u32 t, 0, 0;\n\tadd.u64 a1, %1, 2;\n\tadd.u64 a2, %1, 4;\n\tadd.u64 a3, %1, 6;\n\t"                           \
+    "add.u64 b1, %2, 2;\n\tadd.u64 b2, %2, 4;\n\tadd.u64 b3, %2, 6;\n\t"
+#define AMV_S_TAIL                                                                                                                             \
+    "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t"                                                       \
+    "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+    if constexpr (A == 2u)
+        asm volatile(AMV_S_HEAD
+                     "add.u64 a4, %1, %6;\n\tadd.u64 a5, a1, %6;\n\tadd.u64 a6, a2, %6;\n\tadd.u64 a7, a3, %6;\n\t"
+                     "add.u64 b4, %2, %7;\n\tadd.u64 b5, b1, %7;\n\tadd.u64 b6, b2, %7;\n\tadd.u64 b7, b3, %7;\n\t" AMV_SS("%1", "%2", "p")
+                         AMV_SS("a1", "b1", "t") AMV_SS("a2", "b2", "t") AMV_SS("a3", "b3", "t") AMV_SS("a4", "b4", "t") AMV_SS("a5", "b5", "t")
+                             AMV_SS("a6", "b6", "t") AMV_SS("a7", "b7", "t") AMV_S_TAIL ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(bar0), "r"(bar1), "n"(QA), "n"(KA)
+                     : "memory");
+    else
+        asm volatile(AMV_S_HEAD AMV_SS("%1", "%2", "p") AMV_SS("a1", "b1", "t") AMV_SS("a2", "b2", "t") AMV_SS("a3", "b3", "t") AMV_S_TAIL ::"r"(d), "l"(a),
+                     "l"(b), "r"(idesc), "r"(bar0), "r"(bar1)
+                     : "memory");
+#undef AMV_SS
+#undef AMV_S_HEAD
+#undef AMV_S_TAIL
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Descriptor of a V tile as the B operand with its columns (N) contiguous: 64-column groups of the 128-byte swizzle
@@ -158,10 +193,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t *sQ = base, *sK = sQ + 2u * L::Q, *sV = sK + ST * L::TILE;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * L::TILE);
+    uint8_t* s_out = sV + ST * L::TILE;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + L::STAGE_OUT);
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST,
-                   q_full = v_empty + 8u * ST, s_full = q_full + 16u, p_full = s_full + 16u, pv_done = p_full + 16u, q_empty = pv_done + 16u, drain = q_empty + 16u;
-    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 4u * ST + 11u);
+                   q_full = v_empty + 8u * ST, q_empty = q_full + 16u, s_full = q_empty + 16u, p_full = s_full + 32u, pv_done = p_full + 32u,
+                   drain = pv_done + 32u;   // the last three: [group][tile & 1]
+    Ctl* ctl = reinterpret_cast<Ctl*>(bars + 4u * ST + 18u);
     uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                   // [12]
     volatile uint32_t* s_bad = s_warp + kTcThreads / 32u;                      // 16-key steps whose page is none, of the last key tiles
     uint32_t* s_pref = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + 512u);
@@ -169,18 +206,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < ST; ++s) {
             mbar_init(k_full + 8u * s, 1u);
-            mbar_init(k_empty + 8u * s, 1u);
+            mbar_init(k_empty + 8u * s, 2u);
             mbar_init(v_full + 8u * s, 1u);
-            mbar_init(v_empty + 8u * s, 1u);
+            mbar_init(v_empty + 8u * s, 2u);
         }
         for (uint32_t g = 0; g < 2u; ++g) {
             mbar_init(q_full + 8u * g, 1u);
             mbar_init(q_empty + 8u * g, 1u);
-            mbar_init(s_full + 8u * g, 1u);
-            mbar_init(p_full + 8u * g, 4u);
-            mbar_init(pv_done + 8u * g, 1u);
+            for (uint32_t b = 0; b < 2u; ++b) {
+                mbar_init(s_full + 16u * g + 8u * b, 1u);
+                mbar_init(p_full + 16u * g + 8u * b, 4u);
+                mbar_init(pv_done + 16u * g + 8u * b, 1u);   // two of them: a wait for tile j - 1's meets it at most one phase behind
+            }
         }
         mbar_init(drain, 1u);
+        mbar_init(drain + 8u, 1u);
         ctl->abort = 0u;
         fence_barrier_init();
     }
@@ -208,68 +248,88 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
             const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + kTcRows, p.R) - 1u).hi;
-            for (uint32_t i = p.a; i < p.b; ++i, ++tiles) {
+            int32_t page = -1, page_v = -1;   // this lane's box: K's, and V's of the tile before
+            uint32_t load = 0, load_v = 0;
+            for (uint32_t i = p.a; ok && i <= p.b; ++i) {
                 const uint32_t key0 = (p.first + i) * kTcKeys, b0 = key0 + lane * box;
-                int32_t page = -1;
-                const bool want = lane < boxes && b0 < hi && b0 + box > lo;
-                if (want) page = page_of(pc, p.q, b0);
-                const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0), load = __ballot_sync(0xffffffffu, want && page >= 0);
-                uint32_t bad = 0;
-                if (none) {
-                    for (uint32_t j = 0; j < kTcKeys / 16u; ++j) bad |= (none >> (16u * j / box) & 1u) << j;
-                    if (lane == 0u) refuse(pc, __popc(none));
-                }
-                const uint32_t bytes = (uint32_t)__popc(load) * box * 128u * A;
-                for (uint32_t kv = 0; kv < 2u; ++kv) {
-                    Ring& r = kv ? vr : kr;
-                    const uint32_t full = (kv ? v_full : k_full) + 8u * r.idx, empty = (kv ? v_empty : k_empty) + 8u * r.idx;
-                    ok = wait_on(empty, r.phase ^ 1u, ctl, pc.status, kv ? 0xD10u : 0xD00u);
+                if (i < p.b) {
+                    const bool want = lane < boxes && b0 < hi && b0 + box > lo;
+                    page = want ? page_of(pc, p.q, b0) : -1;
+                    const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0);
+                    load = __ballot_sync(0xffffffffu, page >= 0);
+                    uint32_t bad = 0;
+                    if (none) {
+                        for (uint32_t j = 0; j < kTcKeys / 16u; ++j) bad |= (none >> (16u * j / box) & 1u) << j;
+                        if (lane == 0u) refuse(pc, __popc(none));
+                    }
+                    ok = wait_on(k_empty + 8u * kr.idx, kr.phase ^ 1u, ctl, pc.status, 0xD00u);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (lane == 0u) {
-                        if (!kv) s_bad[tiles & (kBadRing - 1u)] = bad;
-                        mbar_arrive_expect_tx(full, bytes);
+                        s_bad[tiles & (kBadRing - 1u)] = bad;
+                        mbar_arrive_expect_tx(k_full + 8u * kr.idx, (uint32_t)__popc(load) * box * 128u * A);
                     }
                     __syncwarp();
-                    const uint32_t stage = smem_u32((kv ? sV : sK) + r.idx * L::TILE);
-                    if (lane < boxes && (load >> lane & 1u))
+                    if (page >= 0)
                         for (uint32_t a = 0; a < A; ++a)
-                            tma_box(stage + a * (kTcKeys * 128u) + lane * box * 128u, kv ? &v_map : &k_map, full, (int)(64u * a), (int)(b0 & (P - 1u)),
-                                    (int)p.group, page);
-                    if (kv) ++v_issued;
-                    else ++k_issued;
-                    r.advance();
+                            tma_box(smem_u32(sK + kr.idx * L::TILE) + a * (kTcKeys * 128u) + lane * box * 128u, &k_map, k_full + 8u * kr.idx,
+                                    (int)(64u * a), (int)(b0 & (P - 1u)), (int)p.group, page);
+                    ++k_issued;
+                    ++tiles;
+                    kr.advance();
                 }
-                if (!ok) break;
+                if (i > p.a) {   // V of the tile before
+                    ok = wait_on(v_empty + 8u * vr.idx, vr.phase ^ 1u, ctl, pc.status, 0xD10u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0u) mbar_arrive_expect_tx(v_full + 8u * vr.idx, (uint32_t)__popc(load_v) * box * 128u * A);
+                    __syncwarp();
+                    if (page_v >= 0)
+                        for (uint32_t a = 0; a < A; ++a)
+                            tma_box(smem_u32(sV + vr.idx * L::TILE) + a * (kTcKeys * 128u) + lane * box * 128u, &v_map, v_full + 8u * vr.idx,
+                                    (int)(64u * a), (int)((b0 - kTcKeys) & (P - 1u)), (int)p.group, page_v);
+                    ++v_issued;
+                    vr.advance();
+                }
+                page_v = page;
+                load_v = load;
             }
         }
         if (ctl->abort) {   // copies already requested finish before the CTA leaves
             for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) wait_on(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
             for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) wait_on(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
         }
-    } else if (warp == kWarpMma) {
+    } else if (warp < kWarpLoad) {
+        const uint32_t g = warp - kWarpMma;
         const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
+        const uint32_t t_s = tmem + 2u * g * kTcKeys, t_o = tmem + 4u * kTcKeys + g * D;
+        const uint64_t dq = make_smem_desc(smem_u32(sQ + g * L::Q)), dk = make_smem_desc(smem_u32(sK)), dv = v_desc(smem_u32(sV));
+        const uint32_t my_s = s_full + 16u * g, my_p = p_full + 16u * g, my_pv = pv_done + 16u * g;
         Ring kr(ST), vr(ST);
-        uint32_t tiles = 0, q_uses[2] = {0u, 0u}, p_uses[2] = {0u, 0u};
+        uint32_t tiles = 0, q_uses = 0, s_tiles = 0, p_tiles = 0;   // of the CTA; of this group: pieces with Q, tiles with S, with P V issued
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
-            const Group grp[2] = {group_of(pc, p, 0u), group_of(pc, p, 1u)};
-            const uint32_t hi_all = max(grp[0].hi, grp[1].hi), T0 = p.first + p.a, T1 = p.first + p.b;
-            uint32_t started[2] = {0u, 0u};
-            // step u: P V of key tile u - 1 and S of key tile u, group by group
-            for (uint32_t u = T0; u <= T1 && ok; ++u) {
-                bool have_k = false, have_v = false;
-                uint32_t steps = 0xFFu;   // 16-key steps of tile u - 1 whose pages are there
-                if (u > T0) steps = ~s_bad[(tiles + (u - 1u - T0)) & (kBadRing - 1u)] & 0xFFu;
-#pragma unroll
-                for (uint32_t g = 0; g < 2u; ++g) {
-                    const Group& x = grp[g];
-                    if (u > T0 && u - 1u >= x.t0 && u - 1u < x.t1) {
-                        const uint32_t key0 = (u - 1u) * kTcKeys;
-                        if (!have_v) {
-                            ok = ok && wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
-                            have_v = true;
-                            if (ok && hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
+            const Group x = group_of(pc, p, g);
+            const uint32_t hi_all = row_span(pc, p.q, min(p.r0 + kTcRows, p.R) - 1u).hi, T0 = p.first + p.a, T1 = p.first + p.b;
+            uint32_t started = 0u;
+            for (uint32_t t = T0; t < T1 + 2u; ++t) {   // P V of tile t - 2, then S of tile t in its place
+                if (t >= T0 + 2u) {
+                    const uint32_t u = t - 2u, key0 = u * kTcKeys, b = p_tiles & 1u;
+                    const bool mine = u >= x.t0 && u < x.t1;
+                    ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
+                    if (mine) ok = ok && wait_on(my_p + 8u * b, (p_tiles >> 1) & 1u, ctl, pc.status, 0xD50u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (mine) {
+                        ++p_tiles;
+                        tc_fence_after();
+                        const uint32_t steps = ~s_bad[(tiles + (u - T0)) & (kBadRing - 1u)] & 0xFu;   // 16 keys whose page is there
+                        const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
+                        if (steps == 0xFu && key0 >= x.lo && key0 + kTcKeys <= x.hi) {
+                            mma_pv<EXACT>(t_o, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
+                            started = 1u;
+                        } else {
+                            if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
                                 const uint32_t from = hi_all - key0, n = (16u - (from & 15u)) & 15u;
                                 for (uint32_t j = lane; j < n * (D / 8u); j += 32u) {
                                     const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
@@ -279,110 +339,84 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                 fence_async_smem();
                                 __syncwarp();
                             }
-                        }
-                        ok = ok && wait_on(p_full + 8u * g, p_uses[g] & 1u, ctl, pc.status, 0xD50u);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        ++p_uses[g];
-                        tc_fence_after();
-                        const uint32_t s0 = x.lo > key0 ? (x.lo - key0) / 16u : 0u, s1 = (min(x.hi - key0, kTcKeys) + 15u) / 16u;
-                        const uint64_t dv = v_desc(smem_u32(sV + vr.idx * L::TILE));
-                        const uint32_t ta = tmem + g * kTcKeys, to = tmem + 2u * kTcKeys + g * D;
-                        // 16 keys a step: 8 columns of P, two groups of eight V rows
-                        if (s0 == 0u && s1 == kTcKeys / 16u && steps == 0xFFu) {
-#pragma unroll
-                            for (uint32_t k = 0; k < kTcKeys / 16u; ++k) mma_ts(to, ta + 8u * k, dv + 128u * k, idesc_o, k ? 1u : started[g]);
-                            if (EXACT) {
-#pragma unroll
-                                for (uint32_t k = 0; k < kTcKeys / 16u; ++k) mma_ts(to, ta + 64u + 8u * k, dv + 128u * k, idesc_o, 1u);
-                            }
-                            started[g] = 1u;
-                        } else {
+                            const uint32_t s0 = x.lo > key0 ? (x.lo - key0) / 16u : 0u, s1 = (min(x.hi - key0, kTcKeys) + 15u) / 16u;
 #pragma unroll 1
-                            for (uint32_t k = s0; k < s1; ++k) {
+                            for (uint32_t k = s0; k < s1; ++k) {   // 16 keys a step: 8 columns of P, two groups of eight V rows
                                 if (!(steps >> k & 1u)) continue;
-                                mma_ts(to, ta + 8u * k, dv + 128u * k, idesc_o, started[g]);
-                                if (EXACT) mma_ts(to, ta + 64u + 8u * k, dv + 128u * k, idesc_o, 1u);
-                                started[g] = 1u;
+                                mma_ts(t_o, t_s + b * kTcKeys + 8u * k, dvt + 128u * k, idesc_o, started);
+                                if (EXACT) mma_ts(t_o, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
+                                started = 1u;
                             }
+                            commit(my_pv + 8u * b);
+                            commit(v_empty + 8u * vr.idx);
                         }
-                        if (u == x.t1) commit(pv_done + 8u * g);
+                    } else if (lane == 0u) {
+                        mbar_arrive(v_empty + 8u * vr.idx);
                     }
-                    if (u < T1 && u >= x.t0 && u < x.t1) {
-                        if (!have_k) ok = ok && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
-                        have_k = true;
-                        if (u == x.t0) {
-                            ok = ok && wait_on(q_full + 8u * g, q_uses[g] & 1u, ctl, pc.status, 0xD70u);
-                            ++q_uses[g];
-                        }
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (uint32_t a = 0; a < A; ++a) {
-                            const uint64_t da = make_smem_desc(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)));
-                            const uint64_t db = make_smem_desc(smem_u32(sK + kr.idx * L::TILE + a * (kTcKeys * 128u)));
-#pragma unroll
-                            for (uint32_t k = 0; k < 4u; ++k)
-                                mma_ss(tmem + g * kTcKeys, da + 2u * k, db + 2u * k, idesc_s, (uint32_t)((a | k) != 0u));
-                        }
-                        commit(s_full + 8u * g);
-                        if (u + 1u == x.t1) commit(q_empty + 8u * g);
-                    }
-                }
-                if (!ok) break;
-                if (u > T0) {   // (a tile that neither group sees is given back, too)
-                    if (!have_v) ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD80u);
-                    commit(v_empty + 8u * vr.idx);
                     vr.advance();
                 }
-                if (u < T1) {
-                    if (!have_k) ok = ok && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD90u);
-                    commit(k_empty + 8u * kr.idx);
+                if (t < T1) {
+                    const bool mine = t >= x.t0 && t < x.t1;
+                    ok = wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
+                    if (mine && t == x.t0) {
+                        ok = ok && wait_on(q_full + 8u * g, q_uses & 1u, ctl, pc.status, 0xD70u);
+                        ++q_uses;
+                    }
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (mine) {
+                        const uint32_t b = s_tiles & 1u;
+                        ++s_tiles;
+                        mma_s<A>(t_s + b * kTcKeys, dq, dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
+                        if (t + 1u == x.t1) commit(q_empty + 8u * g);
+                    } else if (lane == 0u) {
+                        mbar_arrive(k_empty + 8u * kr.idx);
+                    }
                     kr.advance();
                 }
             }
-            ok = __all_sync(0xffffffffu, ok);
             tiles += p.b - p.a;
         }
         if (__any_sync(0xffffffffu, ctl->abort != 0u)) {   // MMAs already issued finish before the CTA leaves
-            commit(drain);
-            for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain, 0u); ++spins) __nanosleep(64);
+            commit(drain + 8u * g);
+            for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain + 8u * g, 0u); ++spins) __nanosleep(64);
         }
-    } else if (warp >= kWarpQ) {
-        // Q rows of a group into the K-major 128-byte swizzle, idle rows zero
-        const uint32_t g = warp - kWarpQ;
-        uint32_t uses = 0;
+    } else {
+        // Q rows into the K-major 128-byte swizzle, idle rows zero
+        uint32_t uses[2] = {0u, 0u};
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
-            const Group x = group_of(pc, p, g);
-            if (x.t1 <= x.t0) continue;
-            if (uses) ok = wait_on(q_empty + 8u * g, (uses - 1u) & 1u, ctl, pc.status, 0xDC0u);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            ++uses;
-            constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
-            const uint32_t c = lane % PIECES, at = smem_u32(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u));
+#pragma unroll 1
+            for (uint32_t g = 0; g < 2u; ++g) {
+                const Group x = group_of(pc, p, g);
+                if (x.t1 <= x.t0) continue;
+                const uint32_t n = g ? uses[1]++ : uses[0]++;
+                if (n) ok = wait_on(q_empty + 8u * g, (n - 1u) & 1u, ctl, pc.status, 0xDC0u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
+                const uint32_t c = lane % PIECES, at = smem_u32(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u));
 #pragma unroll 4
-            for (uint32_t i = 0; i < kGroupRows / PER; ++i) {
-                const uint32_t r = i * PER + lane / PIECES, row = x.r0 + r, to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
-                if (r < x.rows)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to),
-                                 "l"(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.group * pc.G + row % pc.G) * D + 8u * c)
-                                 : "memory");
-                else
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0u) : "memory");
+                for (uint32_t i = 0; i < kGroupRows / PER; ++i) {
+                    const uint32_t r = i * PER + lane / PIECES, row = x.r0 + r, to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
+                    if (r < x.rows)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to),
+                                     "l"(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.group * pc.G + row % pc.G) * D + 8u * c)
+                                     : "memory");
+                    else
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0u) : "memory");
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem();   // the MMAs read Q through the async proxy
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(q_full + 8u * g);
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_async_smem();   // the MMAs read Q through the async proxy
-            __syncwarp();
-            if (lane == 0u) mbar_arrive(q_full + 8u * g);
         }
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, ts = tmem + lanes + g * kTcKeys, to = tmem + lanes + 2u * kTcKeys + g * D;
-        uint32_t s_uses = 0, pv_uses = 0, tiles = 0;
+        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, to = tmem + lanes + 4u * kTcKeys + g * D;
+        uint32_t j = 0, tiles = 0;   // key tiles of this group, of the CTA, so far
         bool cut = false;
         while (walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
@@ -391,63 +425,71 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const bool valid = my < x.rows;
             const Span span = valid ? row_span(pc, p.q, row) : Span{0u, 0u};
             float m_run = neg_inf(), l_run = 0.0f;
-            for (uint32_t t = x.t0; t < x.t1; ++t) {
-                const uint32_t key0 = t * kTcKeys;
-                ok = ok && wait_on(s_full + 8u * g, s_uses & 1u, ctl, pc.status, 0xDA0u);
+            for (uint32_t t = x.t0; t < x.t1; ++t, ++j) {
+                const uint32_t key0 = t * kTcKeys, b = j & 1u, ts = tmem + lanes + (2u * g + b) * kTcKeys;
+                ok = ok && wait_on(s_full + 16u * g + 8u * b, (j >> 1) & 1u, ctl, pc.status, 0xDA0u);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                ++s_uses;
                 tc_fence_after();
                 const uint32_t gone = s_bad[(tiles + (t - p.first - p.a)) & (kBadRing - 1u)];
-                // the same for every thread of the group
-                const bool plain = gone == 0u && key0 >= x.lo_all && key0 + kTcKeys <= x.hi_all && pc.softcap == 0.0f && pc.scale2 > 0.0f;
-                if (!plain) {   // hidden keys and the cap, on the scores where they are: few tiles, so few registers rather than few steps
-#pragma unroll 1
-                    for (uint32_t c = 0; c < kTcKeys; c += 16u) {
-                        uint32_t v[16];
-                        tmem_ld16(ts + c, v);
-#pragma unroll
-                        for (uint32_t k = 0; k < 16u; ++k) {
-                            const uint32_t key = key0 + c + k;
-                            const bool seen = key >= span.lo && key < span.hi && !(gone >> (c >> 4) & 1u);
-                            v[k] = __float_as_uint(seen ? capped(pc, __uint_as_float(v[k])) : neg_inf());
-                        }
-                        tmem_st16_async(ts + c, v);
-                    }
-                    tmem_wait_st();
-                }
-                float s[kTcKeys], m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+                float s[kTcKeys];
 #pragma unroll
                 for (uint32_t c = 0; c < kTcKeys; c += 32u) tmem_ld32_async(ts + c, reinterpret_cast<uint32_t*>(s) + c);
                 tmem_wait_ld();
+                // the same for every thread of the group
+                const bool open = gone == 0u && key0 >= x.lo_all && key0 + kTcKeys <= x.hi_all, scaled = pc.softcap == 0.0f && pc.scale2 > 0.0f;
+                if (!scaled) {   // the cap, or a scale that is not positive
 #pragma unroll
-                for (uint32_t k = 0; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
-                const float mul = plain ? pc.scale2 : 1.0f, mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+                    for (uint32_t k = 0; k < kTcKeys; ++k) s[k] = capped(pc, s[k]);
+                }
+                if (!open) {     // hidden keys: a bit per key of 32
+#pragma unroll
+                    for (uint32_t c = 0; c < kTcKeys; c += 32u) {
+                        const uint32_t a = span.lo > key0 + c ? min(span.lo - key0 - c, 32u) : 0u, e = span.hi > key0 + c ? min(span.hi - key0 - c, 32u) : 0u;
+                        const uint32_t below = e >= 32u ? 0xffffffffu : (1u << e) - 1u, from = a >= 32u ? 0u : 0xffffffffu << a;
+                        const uint32_t there = ((gone >> (c >> 4) & 1u) ? 0u : 0xffffu) | ((gone >> ((c >> 4) + 1u) & 1u) ? 0u : 0xffff0000u);
+                        const uint32_t seen = below & from & there;
+#pragma unroll
+                        for (uint32_t k = 0; k < 32u; ++k) s[c + k] = seen >> k & 1u ? s[c + k] : neg_inf();
+                    }
+                }
+                float m4[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) m4[k] = fmaxf(s[2u * k], s[2u * k + 1u]);
+#pragma unroll
+                for (uint32_t k = 8u; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
+                const float mul = scaled ? pc.scale2 : 1.0f, mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * mul;
                 const bool grow = mx > m_run + kGrowth || (m_run == neg_inf() && mx != neg_inf());
-                if (__any_sync(0xffffffffu, grow)) {   // (no P V of this group is on its way: S of this tile was issued behind the last)
+                if (__any_sync(0xffffffffu, grow)) {   // a row's sum and accumulator move to the new reference
                     const float f = !grow ? 1.0f : weight(m_run, mx);
                     if (grow) m_run = mx;
                     l_run *= f;
                     if (t != x.t0) {
+                        ok = wait_on(pv_done + 16u * g + 8u * (b ^ 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDC8u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
-                        for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {   // (the scores stay in registers meanwhile)
-                            uint32_t v[16];
-                            tmem_ld16(to + c, v);
+                        for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
+                            uint32_t v[32];
+                            tmem_ld32_async(to + c, v);
+                            tmem_wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
                             tmem_st16_async(to + c, v);
+                            tmem_st16_async(to + c + 16u, v + 16);
                         }
                     }
                 }
                 const float ref = m_run == neg_inf() ? 0.0f : m_run;
-                const uint64_t mul2 = pack2(mul, mul), ref2 = pack2(-ref, -ref);
+                const uint64_t mul_2 = pack2(mul, mul), ref2 = pack2(-ref, -ref);
                 uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-                for (uint32_t part = 0; part < 4u; ++part) {
+                for (uint32_t part = 0; part < 2u; ++part) {
                     uint32_t ph[16], pl[16];
 #pragma unroll
                     for (uint32_t k = 0; k < 16u; ++k) {
-                        const float2 e = unpack2(fma2(pack2(s[32u * part + 2u * k], s[32u * part + 2u * k + 1u]), mul2, ref2));
+                        const float2 e = unpack2(fma2(pack2(s[32u * part + 2u * k], s[32u * part + 2u * k + 1u]), mul_2, ref2));
                         const float p0 = ex2(e.x), p1 = ex2(e.y);
                         sum2[k & 1u] = add2(sum2[k & 1u], pack2(p0, p1));
                         const __half2 h = __floats2half2_rn(p0, p1);
@@ -459,21 +501,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         }
                     }
                     tmem_st16_async(ts + 16u * part, ph);   // over this tile's scores
-                    if (EXACT) tmem_st16_async(ts + 64u + 16u * part, pl);
+                    if (EXACT) tmem_st16_async(ts + 32u + 16u * part, pl);
                 }
                 const float2 sums = unpack2(add2(sum2[0], sum2[1]));
                 l_run += sums.x + sums.y;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0u) mbar_arrive(p_full + 8u * g);
+                if (lane == 0u) mbar_arrive(p_full + 16u * g + 8u * b);
             }
             // ---- results of this piece ----
             const bool some = x.t1 > x.t0, whole = p.a == 0u && p.b == p.n;
-            if (some) {
-                ok = ok && wait_on(pv_done + 8u * g, pv_uses & 1u, ctl, pc.status, 0xDB0u) && !ctl->abort;
-                ++pv_uses;
-            }
+            if (some) ok = ok && wait_on(pv_done + 16u * g + 8u * ((j - 1u) & 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDB0u) && !ctl->abort;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -510,49 +549,61 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 }
                 const bool nothing = l_run == 0.0f;   // nothing was accumulated, or only what zeros made
                 float check = 0.0f;
-#pragma unroll 1
-                for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
-                    uint32_t v[32];
-                    if (some) {
-                        tmem_ld32_async(to + c, v);
-                        tmem_wait_ld();
-                    }
-                    float y[32];
+                // Through shared memory, so that a row leaves 64 bytes at a time (a lane per row and 16 bytes: 32 lines per store, 10 us a
+                // piece): lane 4 i + j of a round has columns 4 j .. 4 j + 3 of row i.
+                const uint32_t mine = smem_u32(s_out) + warp * 2048u, my_at = mine + lane * 64u, sub = lane >> 2, piece = lane & 3u;
+                const uint32_t swz = (lane >> 1) & 3u;
+                unsigned long long row_dst[4], row_extra[4];
+                float row_other[4];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
+                for (uint32_t i = 0; i < 4u; ++i) {
+                    row_dst[i] = __shfl_sync(0xffffffffu, (unsigned long long)dst, 8u * i + sub);
+                    row_extra[i] = __shfl_sync(0xffffffffu, (unsigned long long)extra, 8u * i + sub);
+                    row_other[i] = __shfl_sync(0xffffffffu, other, 8u * i + sub);
+                }
+                const bool f16 = !parts && pc.out == OUT_F16;
+#pragma unroll 1
+                for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
+                    uint32_t v[16];
+                    if (some) tmem_ld16(to + c, v);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
                         const float o = nothing || !some ? 0.0f : __uint_as_float(v[j]);
                         check = fmaf(o, 0.0f, check);
-                        y[j] = own == 0.0f ? 0.0f : o * own;
+                        v[j] = __float_as_uint(own == 0.0f ? 0.0f : o * own);
                     }
-                    if (valid) {
-                        if (extra) {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) {
-                                const float4 e = *reinterpret_cast<const float4*>(extra + 4u + c + j);
-                                y[j] = fmaf(e.x, other, y[j]);
-                                y[j + 1] = fmaf(e.y, other, y[j + 1]);
-                                y[j + 2] = fmaf(e.z, other, y[j + 2]);
-                                y[j + 3] = fmaf(e.w, other, y[j + 3]);
-                            }
+                    for (uint32_t j = 0; j < 4u; ++j)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(my_at + ((j ^ swz) << 4)), "r"(v[4 * j]), "r"(v[4 * j + 1]),
+                                     "r"(v[4 * j + 2]), "r"(v[4 * j + 3])
+                                     : "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; ++i) {
+                        if (!row_dst[i]) continue;
+                        const uint32_t r = 8u * i + sub;
+                        float4 y;
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
+                                     : "r"(mine + r * 64u + ((piece ^ ((r >> 1) & 3u)) << 4))
+                                     : "memory");
+                        if (row_extra[i]) {
+                            const float4 e = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row_extra[i]) + 4u + c + 4u * piece);
+                            y.x = fmaf(e.x, row_other[i], y.x);
+                            y.y = fmaf(e.y, row_other[i], y.y);
+                            y.z = fmaf(e.z, row_other[i], y.z);
+                            y.w = fmaf(e.w, row_other[i], y.w);
                         }
-                        if (!parts && pc.out == OUT_F16) {
-#pragma unroll
-                            for (int j = 0; j < 32; j += 8) {
-                                uint4 h;
-                                __half2 h2[4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) h2[k] = __floats2half2_rn(y[j + 2 * k], y[j + 2 * k + 1]);
-                                memcpy(&h, h2, 16);
-                                *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(dst) + c + j) = h;
-                            }
+                        if (f16) {
+                            const __half2 h0 = __floats2half2_rn(y.x, y.y), h1 = __floats2half2_rn(y.z, y.w);
+                            *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(row_dst[i]) + c + 4u * piece) =
+                                make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
                         } else {
-#pragma unroll
-                            for (int j = 0; j < 32; j += 4)
-                                *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + c + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                            *reinterpret_cast<float4*>(reinterpret_cast<float*>(row_dst[i]) + c + 4u * piece) = y;
                         }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
                 // rows that are not finite although their sum is: over the keys they see, by the whole warp
                 for (uint32_t again = __ballot_sync(0xffffffffu, valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
                     const int i = __ffs(again) - 1;
@@ -577,7 +628,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             }
             tc_fence_before();   // (the next P V overwrites the accumulator behind an arrival of this thread)
         }
-        if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[2u * blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+        if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
     }
     tc_fence_before();
     __syncthreads();
