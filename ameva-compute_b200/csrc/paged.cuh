@@ -35,6 +35,7 @@ struct Args {
     void* dst;
     float* slots;               // results of cut row tiles: slot 2 c (a tile begun elsewhere), 2 c + 1 (one that goes on elsewhere)
     uint4* cut;                 // per CTA what the merge kernel needs of a cut row tile: parts | group << 16 (0: none), first token, first row, rows
+    uint32_t q_boxes;           // the map of q serves the rows of a group
     uint32_t HB, groups, keys_log2, over;   // KV heads of a group, groups, the line's tiles and its allowance per row tile
     const float* extra;         // results over other keys of the same rows that the final ones take in (the layout of OUT_PARTS)
     uint32_t* refused;          // the caller's status words: count of refused entries, lowest node

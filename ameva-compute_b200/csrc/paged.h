@@ -5,9 +5,9 @@
 namespace amv {
 namespace paged {
 
-// Maps of the cache for boxes of 64 columns x tokens x heads of one page.
+// Maps of the cache for boxes of 64 columns x tokens x heads of one page, and of q for 64 columns x the heads of a group x tokens.
 struct Maps {
-    CUtensorMap k, v;
+    CUtensorMap k, v, q;
 };
 
 constexpr uint32_t kDecRows = 16;                        // paged_attn.cu: rows per tile

@@ -762,13 +762,22 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
     return check_launch();
 }
 
-static AcResult cache_maps(const LaunchArgs& a, const Args& pc, uint32_t D, Maps& rows_maps, Maps& tc_maps) {
+static AcResult cache_maps(const LaunchArgs& a, Args& pc, uint32_t D, Maps& rows_maps, Maps& tc_maps) {
     tc::EncodeTiledFn enc = tc::encode_fn();
     const uint32_t P = 1u << pc.page_log2, heads = few_heads(D, pc.n_head_kv), tc_box = P < kTcKeys ? P : kTcKeys;
     if (!enc) return AC_ERR_DRIVER_SYMBOL_MISSING;
     const bool ok = encode_cache(enc, &rows_maps.k, a.ptr[1], pc, D, 16u, heads) && encode_cache(enc, &rows_maps.v, a.ptr[2], pc, D, 16u, heads) &&
                     encode_cache(enc, &tc_maps.k, a.ptr[1], pc, D, tc_box, 1u) && encode_cache(enc, &tc_maps.v, a.ptr[2], pc, D, tc_box, 1u);
-    return ok ? AC_SUCCESS : AC_ERR_INVALID_SHAPE;
+    if (!ok) return AC_ERR_INVALID_SHAPE;
+    memset(&tc_maps.q, 0, sizeof(tc_maps.q));
+    pc.q_boxes = D <= 128u && (pc.G & (pc.G - 1u)) == 0u && pc.G <= 128u;
+    if (pc.q_boxes) {
+        const cuuint64_t dims[3] = {D, pc.n_head, pc.rows}, strides[2] = {2ull * D, 2ull * (pc.rows > 1u ? pc.q_s : (uint64_t)pc.n_head * D)};
+        const cuuint32_t box[3] = {64, pc.G, 128u / pc.G}, estr[3] = {1, 1, 1};
+        pc.q_boxes = strides[1] && enc(&tc_maps.q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.ptr[0], dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    return AC_SUCCESS;
 }
 
 }  // namespace paged

@@ -156,6 +156,44 @@ __device__ __forceinline__ void mma_s(uint32_t d, uint64_t a, uint64_t b, uint32
 #undef AMV_S_HEAD
 #undef AMV_S_TAIL
 }
+// P V of a tile and S of the one that takes its place, as mma_pv and mma_s.
+template <uint32_t A, bool EXACT>
+__device__ __forceinline__ void mma_step(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t bar0, uint32_t bar1, uint64_t q, uint64_t k,
+                                         uint32_t idesc_s, uint32_t bar2, uint32_t bar3) {
+    constexpr uint64_t QA = kGroupRows * 128u / 16u, KA = kTcKeys * 128u / 16u;
+#define AMV_TS(X, B, P) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [" X "], " B ", %3, " P ";\n\t"
+#define AMV_SS(X, B, P) "@q tcgen05.mma.cta_group::1.kind::f16 [%1], " X ", " B ", %9, " P ";\n\t"
+#define AMV_COMMIT(X) "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [" X "];\n\t"
+#define AMV_HEAD                                                                                                                               \
+    "{\n\t.reg .pred p, q, t, z;\n\t.reg .b32 a1, a2, a3, c0, c1, c2, c3;\n\t.reg .b64 b1, b2, b3, x1, x2, x3, x4, x5, x6, x7, y1, y2, y3, y4, y5, y6, y7;\n\t" \
+    "elect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 t, 0, 0;\n\tsetp.ne.u32 z, 0, 0;\n\t"                                      \
+    "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\tadd.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\t" \
+    "add.u64 x1, %7, 2;\n\tadd.u64 x2, %7, 4;\n\tadd.u64 x3, %7, 6;\n\tadd.u64 y1, %8, 2;\n\tadd.u64 y2, %8, 4;\n\tadd.u64 y3, %8, 6;\n\t"        \
+    AMV_TS("%1", "%2", "p") AMV_TS("a1", "b1", "t") AMV_TS("a2", "b2", "t") AMV_TS("a3", "b3", "t")
+#define AMV_LOW                                                                                                                                \
+    "add.u32 c0, %1, 32;\n\tadd.u32 c1, %1, 40;\n\tadd.u32 c2, %1, 48;\n\tadd.u32 c3, %1, 56;\n\t" AMV_TS("c0", "%2", "t") AMV_TS("c1", "b1", "t")      \
+        AMV_TS("c2", "b2", "t") AMV_TS("c3", "b3", "t")
+#define AMV_MID AMV_COMMIT("%5") AMV_COMMIT("%6") AMV_SS("%7", "%8", "z") AMV_SS("x1", "y1", "t") AMV_SS("x2", "y2", "t") AMV_SS("x3", "y3", "t")
+#define AMV_MORE                                                                                                                               \
+    "add.u64 x4, %7, %12;\n\tadd.u64 x5, x1, %12;\n\tadd.u64 x6, x2, %12;\n\tadd.u64 x7, x3, %12;\n\t"                                             \
+    "add.u64 y4, %8, %13;\n\tadd.u64 y5, y1, %13;\n\tadd.u64 y6, y2, %13;\n\tadd.u64 y7, y3, %13;\n\t"                                             \
+    AMV_SS("x4", "y4", "t") AMV_SS("x5", "y5", "t") AMV_SS("x6", "y6", "t") AMV_SS("x7", "y7", "t")
+#define AMV_TAIL AMV_COMMIT("%10") AMV_COMMIT("%11") "}"
+#define AMV_ARGS "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(bar0), "r"(bar1), "l"(q), "l"(k), "r"(idesc_s), "r"(bar2), "r"(bar3), "n"(QA), "n"(KA)
+    if constexpr (A == 2u && EXACT) asm volatile(AMV_HEAD AMV_LOW AMV_MID AMV_MORE AMV_TAIL ::AMV_ARGS : "memory");
+    else if constexpr (A == 2u) asm volatile(AMV_HEAD AMV_MID AMV_MORE AMV_TAIL ::AMV_ARGS : "memory");
+    else if constexpr (EXACT) asm volatile(AMV_HEAD AMV_LOW AMV_MID AMV_TAIL ::AMV_ARGS : "memory");
+    else asm volatile(AMV_HEAD AMV_MID AMV_TAIL ::AMV_ARGS : "memory");
+#undef AMV_TS
+#undef AMV_SS
+#undef AMV_COMMIT
+#undef AMV_HEAD
+#undef AMV_LOW
+#undef AMV_MID
+#undef AMV_MORE
+#undef AMV_TAIL
+#undef AMV_ARGS
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Descriptor of a V tile as the B operand with its columns (N) contiguous: 64-column groups of the 128-byte swizzle
 // kTcKeys * 128 bytes apart (leading offset), groups of eight keys 1024 bytes apart (stride offset).
@@ -187,7 +225,8 @@ __device__ __forceinline__ Group group_of(const Args& pc, const Piece& p, uint32
 
 template <int D, bool EXACT>
 __global__ void __launch_bounds__(kTcThreads, 1)
-paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args pc) {
+paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map,
+                const __grid_constant__ Args pc) {
     using L = Tc<D>;
     constexpr uint32_t A = L::A, ST = L::STAGES, C = D / 32;
     extern __shared__ uint8_t smem_raw[];
@@ -312,7 +351,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const Group x = group_of(pc, p, g);
             const uint32_t hi_all = row_span(pc, p.q, min(p.r0 + kTcRows, p.R) - 1u).hi, T0 = p.first + p.a, T1 = p.first + p.b;
             uint32_t started = 0u;
+            uint32_t bad_1 = 0u, bad_2 = 0u;   // 16-key steps without a page, of tile t - 1 and t - 2
             for (uint32_t t = T0; t < T1 + 2u; ++t) {   // P V of tile t - 2, then S of tile t in its place
+                // (the group's rows see some of tile t, all of tile t - 2, and neither is its first)
+                if (t >= T0 + 2u && t < T1 && t - 2u >= x.t0 && t < x.t1 && bad_2 == 0u && (t - 2u) * kTcKeys >= x.lo) {
+                    const uint32_t b = p_tiles & 1u;
+                    ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u) && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u) &&
+                         wait_on(my_p + 8u * b, (p_tiles >> 1) & 1u, ctl, pc.status, 0xD50u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    mma_step<A, EXACT>(t_o, t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
+                                       dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
+                    started = 1u;
+                    if (t + 1u == x.t1) commit(q_empty + 8u * g);
+                    bad_2 = bad_1;
+                    bad_1 = s_bad[(tiles + (t - T0)) & (kBadRing - 1u)];
+                    ++p_tiles;
+                    ++s_tiles;
+                    vr.advance();
+                    kr.advance();
+                    continue;
+                }
                 if (t >= T0 + 2u) {
                     const uint32_t u = t - 2u, key0 = u * kTcKeys, b = p_tiles & 1u;
                     const bool mine = u >= x.t0 && u < x.t1;
@@ -323,7 +383,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (mine) {
                         ++p_tiles;
                         tc_fence_after();
-                        const uint32_t steps = ~s_bad[(tiles + (u - T0)) & (kBadRing - 1u)] & 0xFu;   // 16 keys whose page is there
+                        const uint32_t steps = ~bad_2 & 0xFu;   // 16 keys whose page is there
                         const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
                         if (steps == 0xFu && key0 >= x.lo && key0 + kTcKeys <= x.hi) {
                             mma_pv<EXACT>(t_o, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
@@ -374,6 +434,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     }
                     kr.advance();
                 }
+                bad_2 = bad_1;
+                bad_1 = t < T1 ? s_bad[(tiles + (t - T0)) & (kBadRing - 1u)] : 0u;
             }
             tiles += p.b - p.a;
         }
@@ -394,17 +456,33 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 if (n) ok = wait_on(q_empty + 8u * g, (n - 1u) & 1u, ctl, pc.status, 0xDC0u);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                if (pc.q_boxes) {   // heads of a group in a power of two: 128 / G tokens by one copy per 64 columns (rows of others behind the last)
+                    if (lane == 0u) {
+                        mbar_arrive_expect_tx(q_full + 8u * g, L::Q);
+                        for (uint32_t a = 0; a < A; ++a)
+                            tma_load_3d(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)), &q_map, q_full + 8u * g, (int)(64u * a), (int)(p.group * pc.G),
+                                        (int)(p.q.tok0 + x.r0 / pc.G));
+                    }
+                    __syncwarp();
+                    continue;
+                }
                 constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
                 const uint32_t c = lane % PIECES, at = smem_u32(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u));
+                uint32_t r = lane / PIECES, token = (x.r0 + r) / pc.G, head = (x.r0 + r) % pc.G;
+                const __half* q0 = pc.q + (uint64_t)p.q.tok0 * pc.q_s + (uint64_t)p.group * pc.G * D + 8u * c;
 #pragma unroll 4
                 for (uint32_t i = 0; i < kGroupRows / PER; ++i) {
-                    const uint32_t r = i * PER + lane / PIECES, row = x.r0 + r, to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
+                    const uint32_t to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
                     if (r < x.rows)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to),
-                                     "l"(pc.q + (uint64_t)(p.q.tok0 + row / pc.G) * pc.q_s + (uint64_t)(p.group * pc.G + row % pc.G) * D + 8u * c)
-                                     : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(q0 + (uint64_t)token * pc.q_s + head * D) : "memory");
                     else
                         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0u) : "memory");
+                    r += PER;
+                    head += PER;
+                    while (head >= pc.G) {
+                        head -= pc.G;
+                        ++token;
+                    }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_async_smem();   // the MMAs read Q through the async proxy
@@ -638,7 +716,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 template <int D, bool EXACT>
 static bool launch_tc_t(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
     if (!ensure_dynamic_smem<paged_tc_kernel<D, EXACT>>((int)Tc<D>::smem(kMaxSeqs))) return false;
-    launch_pdl(paged_tc_kernel<D, EXACT>, dim3(ctas), dim3(kTcThreads), Tc<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, pc);
+    launch_pdl(paged_tc_kernel<D, EXACT>, dim3(ctas), dim3(kTcThreads), Tc<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, maps.q, pc);
     return true;
 }
 
