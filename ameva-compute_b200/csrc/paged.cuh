@@ -348,6 +348,14 @@ __device__ __forceinline__ float score2(const Args& pc, float s) {
     return pc.softcap != 0.0f ? pc.softcap * tanhf(s * pc.scale / pc.softcap) * kLog2e : s * pc.scale2;
 }
 
+// score2 from 1 - 2 / (1 + e^2y) = tanh(y), two special functions instead of tanhf's some 25 instructions. Its absolute error of 2^-22 is,
+// times a cap of 30, 7e-6 of a score (a 32-bit score of 30 has a spacing of 2e-6).
+__device__ __forceinline__ float capped(const Args& pc, float s) {
+    if (pc.softcap == 0.0f) return s * pc.scale2;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s * pc.cap_in)));
+    return fmaf(-2.0f * pc.cap_out, r, pc.cap_out);
+}
 // One row by a whole warp over keys [lo, hi), hidden keys left out instead of multiplied by zero: a lane's C columns of
 // sum 2^(score - ref) v. For rows whose accumulator is not finite: the matrix instructions multiply every key of a step with every
 // row, so a NaN or an infinity in V would reach rows that do not see its key, and an infinity would meet the remainder of its

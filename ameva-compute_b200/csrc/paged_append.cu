@@ -21,7 +21,7 @@ struct AppendArgs {
         theta_scale, freq_scale, ext_factor, attn_factor, corr0, corr1, node;
 };
 constexpr uint32_t kHasPositions = 1u, kHasFactors = 2u;
-constexpr uint32_t kMaxTokens = 4, kMaxHeadDim = 256;
+constexpr uint32_t kMaxTokens = 2, kMaxHeadDim = 256;
 
 __device__ __forceinline__ float as_f(uint32_t u) { return __uint_as_float(u); }
 
@@ -44,7 +44,7 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(256) append_kernel(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+__global__ void __launch_bounds__(256, 8) append_kernel(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                                                      const int32_t* __restrict__ table, const int32_t* __restrict__ q_start,
                                                      const int32_t* __restrict__ kv_len, const int32_t* __restrict__ positions,
                                                      const float* __restrict__ factors, __half* __restrict__ q_out, __half* __restrict__ k_cache,
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) append_kernel(const float* __restrict__ q
     };
     if (VEC) {   // units of eight elements: four pairs of a rotated head, or eight elements beside one another that are copied
         const uint32_t units = pc.D >> 3, all = tokens * heads * units, rotated_units = pc.n_dims >> 3;
-#pragma unroll 2
+#pragma unroll 1
         for (uint32_t i = threadIdx.x; i < all; i += 256u) {
             const uint32_t row = i / units, u = i - row * units, t = row / heads, h = row - t * heads;
             if (s_slot[t] < 0) continue;
@@ -224,7 +224,7 @@ AcResult launch_paged_append(const LaunchArgs& a) {
         }
     const bool vec = !(pc.n_dims & 7u);
     // tokens per CTA: one while the CTAs do not fill the GPU
-    const uint32_t T = pc.rows >= 4u * 8u * (uint32_t)a.sm_count ? kMaxTokens : 1u;
+    const uint32_t T = pc.rows >= kMaxTokens * 8u * (uint32_t)a.sm_count ? kMaxTokens : 1u;
     const dim3 grid((pc.rows + T - 1u) / T);
     auto run = [&](auto* kernel) {
         launch_pdl(kernel, grid, dim3(256), 0, a.stream, (const float*)a.ptr[0], (const float*)a.ptr[1], (const float*)a.ptr[2],

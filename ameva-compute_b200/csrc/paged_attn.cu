@@ -269,7 +269,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 #pragma unroll
                         for (uint32_t j = 0; j < 2u; ++j) {
                             const uint32_t key = key0 + 8u * nt + 2u * t4 + j;
-                            const float v = score2(pc, sc[nt][2u * h + j]);
+                            const float v = capped(pc, sc[nt][2u * h + j]);
                             x[nt][j] = plain || (key >= span[h].lo && key < span[h].hi && seen[nt >> 1]) ? v : neg_inf();
                             mx = fmaxf(mx, x[nt][j]);
                         }
@@ -533,6 +533,7 @@ __device__ __forceinline__ void merge_set(const MergeSet& set) {
         };
         if (have_row && begin < parts) {
             if (parts <= 2u * share) take(std::integral_constant<uint32_t, 2>(), begin);
+            else if (parts <= 4u * share) take(std::integral_constant<uint32_t, 4>(), begin);
             else
                 for (uint32_t i0 = begin; i0 < parts; i0 += kTogether * share) take(std::integral_constant<uint32_t, kTogether>(), i0);
         }

@@ -80,14 +80,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// score2 (paged.cuh) from 1 - 2 / (1 + e^2y) = tanh(y): tanhf, 128 times over, leaves no registers for the scores. Its absolute error of
-// 2^-22 is, times a cap of 30, 7e-6 of a score (a 32-bit score of 30 has a spacing of 2e-6).
-__device__ __forceinline__ float capped(const Args& pc, float s) {
-    if (pc.softcap == 0.0f) return s * pc.scale2;
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s * pc.cap_in)));
-    return fmaf(-2.0f * pc.cap_out, r, pc.cap_out);
-}
 // The MMAs and commits of a converged warp, issued by one lane, the same every time, without a branch around them: what a branch that
 // only one lane takes computes is not uniform to the compiler, and every descriptor then takes a detour of some 100 clocks.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
