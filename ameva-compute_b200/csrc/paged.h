@@ -11,7 +11,7 @@ struct Maps {
 };
 
 constexpr uint32_t kDecRows = 16;                        // paged_attn.cu: rows per tile
-constexpr uint32_t kTcRows = 256, kTcKeys = 64;          // paged_tc.cu: rows and keys per tile
+constexpr uint32_t kTcRows = 256, kTcKeys = 64;          // paged_tc.cu: rows (half as many for a 32-bit result) and keys per tile
 
 bool launch_tc(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t head_dim, uint32_t ctas);
 

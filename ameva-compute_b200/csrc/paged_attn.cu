@@ -10,8 +10,10 @@
 // fewer heads the KB warps of a head are joined pairwise through shared memory at the end of a piece. All heads of a block of keys are
 // read together because in a cache with a token's heads beside one another they are one run of memory: a head at a time (a warp per
 // 16 keys of a tile of 128) took 195 us for 96 sequences of 20 to 8192 keys, 8 KV heads of 128, 160 k keys, as against 100 us for the
-// bytes, and 8 us per (sequence, head). P: for an f32 result as an f16 value and its remainder (rounded once, 2^-12 of every probability
-// would show there), for an f16 result rounded once (2^-12 against the 2^-12 of the result itself, averaged over the keys).
+// bytes, and 8 us per (sequence, head). P enters the second product as an f16 value and its remainder (rounded once, 2^-12 of every
+// probability would show in an f32 result, and makes an f16 one's error 1.25 times what its own rounding is; the second product costs 2 %
+// of the time above), and the matrix instruction's sums, which are cut rather than rounded, are added up per 32 keys by ordinary
+// additions: left in its accumulator from the first key to the last, 131072 keys are off by 2.3e-6 instead of 4e-7.
 #include <cstring>
 #include <type_traits>
 
@@ -106,7 +108,7 @@ __device__ __forceinline__ void store_part(float* row, uint32_t t4, float m, flo
 }
 
 // TOP: every row tile has at most eight rows (the upper half of the MMA tile), so the lower half's work is left out.
-template <int D, bool TOP, bool EXACT>
+template <int D, bool TOP>
 __global__ void __launch_bounds__(Rows<D>::THREADS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args pc) {
     using L = Rows<D>;
@@ -294,10 +296,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                         sum += p0 + p1;
                         const __half2 hi2 = __floats2half2_rn(p0, p1);
                         ph[nt >> 1][2u * (nt & 1u) + h] = *reinterpret_cast<const uint32_t*>(&hi2);
-                        if (EXACT) {
-                            const float2 f2 = __half22float2(hi2);
-                            pl[nt >> 1][2u * (nt & 1u) + h] = halves(p0 - f2.x, p1 - f2.y);
-                        }
+                        const float2 f2 = __half22float2(hi2);
+                        pl[nt >> 1][2u * (nt & 1u) + h] = halves(p0 - f2.x, p1 - f2.y);
                     }
                     l_run[h] += sum;   // (this lane's keys; the four lanes of a row are added at the end)
                 }
@@ -308,30 +308,38 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             const uint32_t tv = smem_u32(base) + ring.idx * tile + mine_at;
 #pragma unroll
             for (uint32_t kk = 0; kk < 2u; ++kk) {
-                if (!seen[kk]) continue;
-                const uint32_t v0 = tv + kk * A * atom, k0 = key0 + 16u * kk;
+                const uint32_t k0 = key0 + 16u * kk;
                 // V rows behind the last key are whatever the page holds there: probabilities of zero do not hide a NaN
-                if (k0 + 16u > hi_all) {
+                if (seen[kk] && k0 + 16u > hi_all) {
                     const uint32_t from = hi_all - k0;   // 1 .. 15
                     for (uint32_t j = lane; j < (16u - from) * (D / 8u); j += 32u) {
                         const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v0 + (c >> 3) * atom + r * 128u + ((c & 7u) << 4)), "r"(0u) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tv + kk * A * atom + (c >> 3) * atom + r * 128u + ((c & 7u) << 4)), "r"(0u)
+                                     : "memory");
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (before TMA writes there again)
                     __syncwarp();
                 }
+            }
 #pragma unroll
-                for (int np = 0; np < NT / 2; ++np) {   // columns 16 np .. 16 np + 15
-                    const uint32_t piece = 2u * (np & 3) + lv_nt;
+            for (int np = 0; np < NT / 2; ++np) {   // columns 16 np .. 16 np + 15
+                if (!seen[0] && !seen[1]) break;
+                const uint32_t piece = 2u * (np & 3) + lv_nt;
+                float acc[2][4] = {};   // this tile's sum
+#pragma unroll
+                for (uint32_t kk = 0; kk < 2u; ++kk) {
+                    if (!seen[kk]) continue;
                     uint32_t b[4];
-                    ldsm_x4_trans(b, v0 + (np >> 2) * atom + lv_row * 128u + ((piece ^ (lv_row & 7u)) << 4));
-                    mma16816(oc[2 * np], ph[kk], b[0], b[1]);
-                    mma16816(oc[2 * np + 1], ph[kk], b[2], b[3]);
-                    if (EXACT) {
-                        mma16816(oc[2 * np], pl[kk], b[0], b[1]);
-                        mma16816(oc[2 * np + 1], pl[kk], b[2], b[3]);
-                    }
+                    ldsm_x4_trans(b, tv + kk * A * atom + (np >> 2) * atom + lv_row * 128u + ((piece ^ (lv_row & 7u)) << 4));
+                    mma16816(acc[0], ph[kk], b[0], b[1]);
+                    mma16816(acc[1], ph[kk], b[2], b[3]);
+                    mma16816(acc[0], pl[kk], b[0], b[1]);
+                    mma16816(acc[1], pl[kk], b[2], b[3]);
                 }
+#pragma unroll
+                for (uint32_t n = 0; n < 2u; ++n)
+#pragma unroll
+                    for (uint32_t c = 0; c < 2u * H; ++c) oc[2 * np + n][c] += acc[n][c];
             }
             __syncwarp();
             if (lane == 0u) mbar_arrive(empty + 8u * ring.idx);
@@ -576,17 +584,15 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 2) paged_merge_kernel(const 
     if (s1.ctas) merge_set<C>(s1);
 }
 
-template <int D, bool TOP, bool EXACT>
+template <int D, bool TOP>
 static bool launch_rows_t(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
-    if (!ensure_dynamic_smem<paged_rows_kernel<D, TOP, EXACT>>((int)Rows<D>::smem(kMaxSeqs))) return false;
-    launch_pdl(paged_rows_kernel<D, TOP, EXACT>, dim3(ctas), dim3(Rows<D>::THREADS), Rows<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, pc);
+    if (!ensure_dynamic_smem<paged_rows_kernel<D, TOP>>((int)Rows<D>::smem(kMaxSeqs))) return false;
+    launch_pdl(paged_rows_kernel<D, TOP>, dim3(ctas), dim3(Rows<D>::THREADS), Rows<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, pc);
     return true;
 }
 template <int D>
 static bool launch_rows_d(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
-    const bool top = (uint64_t)pc.max_q * pc.G <= 8u, exact = pc.out != OUT_F16;
-    return top ? (exact ? launch_rows_t<D, true, true>(a, pc, maps, ctas) : launch_rows_t<D, true, false>(a, pc, maps, ctas))
-               : (exact ? launch_rows_t<D, false, true>(a, pc, maps, ctas) : launch_rows_t<D, false, false>(a, pc, maps, ctas));
+    return (uint64_t)pc.max_q * pc.G <= 8u ? launch_rows_t<D, true>(a, pc, maps, ctas) : launch_rows_t<D, false>(a, pc, maps, ctas);
 }
 static bool launch_rows(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t D, uint32_t ctas) {
     return D == 64u ? launch_rows_d<64>(a, pc, maps, ctas) : D == 128u ? launch_rows_d<128>(a, pc, maps, ctas) : launch_rows_d<256>(a, pc, maps, ctas);
@@ -736,13 +742,14 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
     many.groups = pc.n_head_kv;
     many.keys_log2 = 6u;
     many.over = kManyOver;
+    const uint32_t tc_rows = pc.out == OUT_F16 ? kTcRows : kTcRows / 2u;   // (paged_tc.cu)
     // the line's length in 32 bits
     const uint64_t few_rows = both ? kFewRows : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs;
     auto too_long = [&](const Args& x, uint64_t row_tiles) {
         return seqs * x.groups * row_tiles * (((uint64_t)pc.max_kv >> x.keys_log2) + 2u + x.over) > 0xFFFFFFFFull;
     };
     if (use_few && too_long(few, (few_rows + kDecRows - 1u) / kDecRows)) return AC_ERR_INVALID_SHAPE;
-    if (use_many && too_long(many, (max_rows + kTcRows - 1u) / kTcRows)) return AC_ERR_INVALID_SHAPE;
+    if (use_many && too_long(many, (max_rows + tc_rows - 1u) / tc_rows)) return AC_ERR_INVALID_SHAPE;
     uint32_t n_few = 0, n_many = 0;
     if (use_few) {
         n_few = ctas_for(use_many ? scratch.left * few.HB / (few.HB + 16u) : scratch.left, few.HB * kDecRows * row, sms);
@@ -751,15 +758,15 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
         if (!few.cut || !few.slots) n_few = 1u, few.cut = nullptr, few.slots = nullptr;
     }
     if (use_many) {
-        n_many = ctas_for(scratch.left, kTcRows * row, sms);
+        n_many = ctas_for(scratch.left, tc_rows * row, sms);
         many.cut = (uint4*)scratch.take(n_many * 16ull);
-        many.slots = (float*)scratch.take(n_many > 1u ? 2ull * n_many * kTcRows * row : 0u);
+        many.slots = (float*)scratch.take(n_many > 1u ? 2ull * n_many * tc_rows * row : 0u);
         if (!many.cut || !many.slots) n_many = 1u, many.cut = nullptr, many.slots = nullptr;
     }
     if (use_many && !launch_tc(a, many, tc_maps, D, n_many)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
     if (use_few && !launch_rows(a, few, rows_maps, D, n_few)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
     const uint32_t merge_few = n_few > 1u ? n_few : 0u, merge_many = n_many > 1u ? n_many : 0u;
-    if (merge_few + merge_many && !launch_merge(a, few, many, D, merge_few, merge_many, kDecRows, kTcRows)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
+    if (merge_few + merge_many && !launch_merge(a, few, many, D, merge_few, merge_many, kDecRows, tc_rows)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
     return check_launch();
 }
 

@@ -1,7 +1,8 @@
 // Attention over a paged KV cache for many rows per sequence (prompts, the shared prefix of a batch; D 64, 128) on the 5th-generation
 // tensor cores. Arguments, rows and the line of work: paged.cuh; launchers: paged_attn.cu.
 //
-// A CTA (one per SM) takes row tiles of 256 rows, two groups of 128, and walks key tiles of 64 for both:
+// A CTA (one per SM) takes row tiles of 256 rows, two groups of 128 (f16 results; one group for 32-bit ones, EXACT, with the warps behind
+// the first four moved up), and walks key tiles of 64 for both:
 //   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 64 scores from tensor memory, online softmax to base 2, write P
 //                    over the scores as f16 (and, for a 32-bit result, what that rounding left beside it). The accumulator is rescaled
 //                    only when a row's maximum has grown by more than 2^kGrowth since its last rescale. They write the piece's results.
@@ -14,6 +15,9 @@
 //   warp 11          brings the Q rows in, those of the next piece as soon as the last S of this one has read them
 // Tensor memory: four S / P tiles of 64 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
 // steps of 16 keys that none sees; V rows behind the last key are zeroed before they are multiplied (a page holds anything there).
+// The tensor core's sums are cut rather than rounded, which an f16 result does not show and a 32-bit one would (2.2e-6 after 300 of them, in
+// proportion to their number): for those the accumulator is added to a sum in registers every kFlush tiles and begins anew, which takes
+// the registers of a second group's softmax.
 // Every wait on a barrier is bounded (paged.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
 #include <cstring>
 
@@ -27,19 +31,23 @@ namespace paged {
 using namespace ptx;
 using namespace tc;
 
-constexpr uint32_t kGroupRows = 128, kWarpMma = 8, kWarpLoad = 10, kWarpQ = 11, kTcThreads = 384, kTmemCols = 512, kBadRing = 8;
+constexpr uint32_t kGroupRows = 128, kBadRing = 8;
 // Registers a thread after the split: 256 x 200 + 128 x 104 = 384 x 168, what the block is launched with.
 constexpr uint32_t kSoftmaxRegs = 200, kOtherRegs = 104;
 constexpr float kGrowth = 7.0f;   // probabilities stay below 2^7
 
-template <int D>
+template <int D, bool EXACT>
 struct Tc {
-    static constexpr uint32_t A = D / 64, STAGES = D == 64 ? 5 : 3;
+    static constexpr uint32_t GROUPS = EXACT ? 1 : 2, ROWS = GROUPS * kGroupRows;
+    static constexpr uint32_t MMA = 4 * GROUPS, LOAD = MMA + GROUPS, QWARP = LOAD + 1, THREADS = EXACT ? 256 : 384;   // warps by role
+    static constexpr uint32_t TMEM = EXACT ? 256 : 512;
+    static constexpr uint32_t A = D / 64, STAGES = EXACT || D == 64 ? 5 : 3;
     static constexpr uint32_t Q = A * kGroupRows * 128u, TILE = A * kTcKeys * 128u;
-    static constexpr uint32_t STAGE_OUT = 8u * 32u * 64u;   // a warp's 32 rows x 16 columns on their way out
-    static constexpr uint32_t FIXED = 1024u + 2u * Q + 2u * STAGES * TILE + STAGE_OUT + 512u;
+    static constexpr uint32_t STAGE_OUT = GROUPS * 4u * 32u * 64u;   // a warp's 32 rows x 16 columns on their way out
+    static constexpr uint32_t FIXED = 1024u + GROUPS * Q + 2u * STAGES * TILE + STAGE_OUT + 512u;
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
+constexpr uint32_t kFlush = 8;   // EXACT: key tiles between two additions of the accumulator to the row's sum
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int page) {
     asm volatile(
@@ -216,14 +224,15 @@ __device__ __forceinline__ Group group_of(const Args& pc, const Piece& p, uint32
 }
 
 template <int D, bool EXACT>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(Tc<D, EXACT>::THREADS, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map,
                 const __grid_constant__ Args pc) {
-    using L = Tc<D>;
+    using L = Tc<D, EXACT>;
+    constexpr uint32_t GROUPS = L::GROUPS;
     constexpr uint32_t A = L::A, ST = L::STAGES, C = D / 32;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t *sQ = base, *sK = sQ + 2u * L::Q, *sV = sK + ST * L::TILE;
+    uint8_t *sQ = base, *sK = sQ + GROUPS * L::Q, *sV = sK + ST * L::TILE;
     uint8_t* s_out = sV + ST * L::TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + L::STAGE_OUT);
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST,
@@ -231,15 +240,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                    drain = pv_done + 32u;   // the last three: [group][tile & 1]
     Ctl* ctl = reinterpret_cast<Ctl*>(bars + 4u * ST + 18u);
     uint32_t* s_warp = reinterpret_cast<uint32_t*>(ctl + 1);                   // [12]
-    volatile uint32_t* s_bad = s_warp + kTcThreads / 32u;                      // 16-key steps whose page is none, of the last key tiles
+    volatile uint32_t* s_bad = s_warp + L::THREADS / 32u;                      // 16-key steps whose page is none, of the last key tiles
     uint32_t* s_pref = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + 512u);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < ST; ++s) {
             mbar_init(k_full + 8u * s, 1u);
-            mbar_init(k_empty + 8u * s, 2u);
+            mbar_init(k_empty + 8u * s, GROUPS);
             mbar_init(v_full + 8u * s, 1u);
-            mbar_init(v_empty + 8u * s, 2u);
+            mbar_init(v_empty + 8u * s, GROUPS);
         }
         for (uint32_t g = 0; g < 2u; ++g) {
             mbar_init(q_full + 8u * g, 1u);
@@ -256,29 +265,29 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         fence_barrier_init();
     }
     // boxes that no row needs are not loaded: their steps are not multiplied, but a zero is a better guest than a NaN
-    for (uint32_t i = threadIdx.x; i < 2u * ST * L::TILE / 16u; i += kTcThreads) reinterpret_cast<uint4*>(sK)[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (warp == kWarpMma) tmem_alloc<false>(smem_u32(&ctl->tmem_base), kTmemCols);
+    for (uint32_t i = threadIdx.x; i < 2u * ST * L::TILE / 16u; i += L::THREADS) reinterpret_cast<uint4*>(sK)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (warp == L::MMA) tmem_alloc<false>(smem_u32(&ctl->tmem_base), L::TMEM);
     fence_async_smem();
     pdl_wait();
     tc_fence_before();
-    const uint32_t total = build_line<kTcRows, kTcThreads / 32u>(pc, s_pref, s_warp);   // (its barriers publish the above)
+    const uint32_t total = build_line<L::ROWS, L::THREADS / 32u>(pc, s_pref, s_warp);   // (its barriers publish the above)
     tc_fence_after();
     pdl_trigger();   // not before the tensor memory is this CTA's
     const uint32_t tmem = ctl->tmem_base;
     const Stretch st = my_stretch(total);
-    Walk<kTcRows> walk(st);
+    Walk<L::ROWS> walk(st);
     const uint32_t P = 1u << pc.page_log2, box = P < kTcKeys ? P : kTcKeys, boxes = kTcKeys / box;
     bool ok = true;
 
-    if (warp >= kWarpMma) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == kWarpLoad) {
+    if (warp >= L::MMA) {
+    if constexpr (!EXACT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == L::LOAD) {
         Ring kr(ST), vr(ST);
         uint32_t tiles = 0;     // of this CTA so far
         uint32_t k_issued = 0, v_issued = 0;
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
-            const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + kTcRows, p.R) - 1u).hi;
+            const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + L::ROWS, p.R) - 1u).hi;
             int32_t page = -1, page_v = -1;   // this lane's box: K's, and V's of the tile before
             uint32_t load = 0, load_v = 0;
             for (uint32_t i = p.a; ok && i <= p.b; ++i) {
@@ -330,10 +339,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) wait_on(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
             for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) wait_on(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
         }
-    } else if (warp < kWarpLoad) {
-        const uint32_t g = warp - kWarpMma;
+    } else if (warp < L::LOAD) {
+        const uint32_t g = warp - L::MMA;
         const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
-        const uint32_t t_s = tmem + 2u * g * kTcKeys, t_o = tmem + 4u * kTcKeys + g * D;
+        const uint32_t t_s = tmem + 2u * g * kTcKeys, t_o = tmem + 2u * GROUPS * kTcKeys + g * D;
         const uint64_t dq = make_smem_desc(smem_u32(sQ + g * L::Q)), dk = make_smem_desc(smem_u32(sK)), dv = v_desc(smem_u32(sV));
         const uint32_t my_s = s_full + 16u * g, my_p = p_full + 16u * g, my_pv = pv_done + 16u * g;
         Ring kr(ST), vr(ST);
@@ -341,7 +350,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
             const Group x = group_of(pc, p, g);
-            const uint32_t hi_all = row_span(pc, p.q, min(p.r0 + kTcRows, p.R) - 1u).hi, T0 = p.first + p.a, T1 = p.first + p.b;
+            const uint32_t hi_all = row_span(pc, p.q, min(p.r0 + L::ROWS, p.R) - 1u).hi, T0 = p.first + p.a, T1 = p.first + p.b;
             uint32_t started = 0u;
             uint32_t bad_1 = 0u, bad_2 = 0u;   // 16-key steps without a page, of tile t - 1 and t - 2
             for (uint32_t t = T0; t < T1 + 2u; ++t) {   // P V of tile t - 2, then S of tile t in its place
@@ -353,6 +362,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
+                    if (EXACT && (t - 2u - x.t0) % kFlush == 0u) started = 0u;
                     mma_step<A, EXACT>(t_o, t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
                                        dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
                     started = 1u;
@@ -375,6 +385,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (mine) {
                         ++p_tiles;
                         tc_fence_after();
+                        if (EXACT && (u - x.t0) % kFlush == 0u) started = 0u;
                         const uint32_t steps = ~bad_2 & 0xFu;   // 16 keys whose page is there
                         const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
                         if (steps == 0xFu && key0 >= x.lo && key0 + kTcKeys <= x.hi) {
@@ -397,6 +408,17 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                 if (!(steps >> k & 1u)) continue;
                                 mma_ts(t_o, t_s + b * kTcKeys + 8u * k, dvt + 128u * k, idesc_o, started);
                                 if (EXACT) mma_ts(t_o, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
+                                started = 1u;
+                            }
+                            if (EXACT && !started) {   // no page of the tile is there, and the accumulator is to begin anew: with zeros
+                                for (uint32_t j = lane; j < 16u * (D / 8u); j += 32u) {
+                                    const uint32_t r = 16u * s0 + j / (D / 8u), c = j % (D / 8u);
+                                    *reinterpret_cast<uint4*>(sV + vr.idx * L::TILE + (c >> 3) * (kTcKeys * 128u) + r * 128u + ((c & 7u) << 4)) =
+                                        make_uint4(0u, 0u, 0u, 0u);
+                                }
+                                fence_async_smem();
+                                __syncwarp();
+                                mma_ts(t_o, t_s + b * kTcKeys + 8u * s0, dvt + 128u * s0, idesc_o, 0u);
                                 started = 1u;
                             }
                             commit(my_pv + 8u * b);
@@ -435,13 +457,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             commit(drain + 8u * g);
             for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain + 8u * g, 0u); ++spins) __nanosleep(64);
         }
-    } else {
+    } else if (warp == L::QWARP) {
         // Q rows into the K-major 128-byte swizzle, idle rows zero
         uint32_t uses[2] = {0u, 0u};
         while (ok && walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
 #pragma unroll 1
-            for (uint32_t g = 0; g < 2u; ++g) {
+            for (uint32_t g = 0; g < GROUPS; ++g) {
                 const Group x = group_of(pc, p, g);
                 if (x.t1 <= x.t0) continue;
                 const uint32_t n = g ? uses[1]++ : uses[0]++;
@@ -484,8 +506,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         }
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, to = tmem + lanes + 4u * kTcKeys + g * D;
+        if constexpr (!EXACT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, to = tmem + lanes + 2u * GROUPS * kTcKeys + g * D;
         uint32_t j = 0, tiles = 0;   // key tiles of this group, of the CTA, so far
         bool cut = false;
         while (walk.next(pc, s_pref)) {
@@ -495,6 +517,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const bool valid = my < x.rows;
             const Span span = valid ? row_span(pc, p.q, row) : Span{0u, 0u};
             float m_run = neg_inf(), l_run = 0.0f;
+            float sum_o[EXACT ? D : 1];   // EXACT: the row's sum; the accumulator holds the tiles since the last addition
+            if (EXACT) {
+#pragma unroll
+                for (uint32_t c = 0; c < (uint32_t)D; ++c) sum_o[c] = 0.0f;
+            }
             for (uint32_t t = x.t0; t < x.t1; ++t, ++j) {
                 const uint32_t key0 = t * kTcKeys, b = j & 1u, ts = tmem + lanes + (2u * g + b) * kTcKeys;
                 ok = ok && wait_on(s_full + 16u * g + 8u * b, (j >> 1) & 1u, ctl, pc.status, 0xDA0u);
@@ -529,25 +556,41 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 #pragma unroll
                 for (uint32_t k = 8u; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
                 const float mul = scaled ? pc.scale2 : 1.0f, mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * mul;
+                const bool added = EXACT && (t - x.t0) % kFlush == 0u;   // the accumulator begins anew with this tile
+                if (EXACT && added && t != x.t0) {
+                    ok = wait_on(pv_done + 16u * g + 8u * (b ^ 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDC4u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
+                        uint32_t v[16];
+                        tmem_ld16(to + c, v);
+#pragma unroll
+                        for (uint32_t k = 0; k < 16u; ++k) sum_o[EXACT ? c + k : 0u] += __uint_as_float(v[k]);
+                    }
+                }
                 const bool grow = mx > m_run + kGrowth || (m_run == neg_inf() && mx != neg_inf());
                 if (__any_sync(0xffffffffu, grow)) {   // a row's sum and accumulator move to the new reference
                     const float f = !grow ? 1.0f : weight(m_run, mx);
                     if (grow) m_run = mx;
                     l_run *= f;
-                    if (t != x.t0) {
+                    if (EXACT) {
+#pragma unroll
+                        for (uint32_t c = 0; c < (uint32_t)D; ++c) sum_o[EXACT ? c : 0u] *= f;
+                    }
+                    if (t != x.t0 && !added) {
                         ok = wait_on(pv_done + 16u * g + 8u * (b ^ 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDC8u);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
-                        for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
-                            uint32_t v[32];
-                            tmem_ld32_async(to + c, v);
-                            tmem_wait_ld();
+                        for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
+                            uint32_t v[16];
+                            tmem_ld16(to + c, v);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                            for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
                             tmem_st16_async(to + c, v);
-                            tmem_st16_async(to + c + 16u, v + 16);
                         }
                     }
                 }
@@ -589,7 +632,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             tiles += p.b - p.a;
             if (x.rows) {
                 const uint32_t token = p.q.tok0 + row / pc.G, head = p.group * pc.G + row % pc.G;
-                float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * kTcRows + (x.r0 - p.r0)) * (D + 4u);
+                float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * L::ROWS + (x.r0 - p.r0)) * (D + 4u);
                 const bool parts = !whole || pc.out == OUT_PARTS;
                 float own = 1.0f, other = 0.0f;      // factors of the values here and of those over other keys
                 const float* extra = nullptr;
@@ -632,13 +675,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     row_other[i] = __shfl_sync(0xffffffffu, other, 8u * i + sub);
                 }
                 const bool f16 = !parts && pc.out == OUT_F16;
-#pragma unroll 1
+#pragma unroll(EXACT ? D / 16 : 1)
                 for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
                     uint32_t v[16];
                     if (some) tmem_ld16(to + c, v);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const float o = nothing || !some ? 0.0f : __uint_as_float(v[j]);
+                        const float o = nothing || !some ? 0.0f : EXACT ? sum_o[EXACT ? c + j : 0u] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
                         check = fmaf(o, 0.0f, check);
                         v[j] = __float_as_uint(own == 0.0f ? 0.0f : o * own);
                     }
@@ -694,7 +737,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             }
             if (p.a == 0u && p.b < p.n) {
                 cut = true;
-                if (threadIdx.x == 0u) note_cut(pc, st, p, min(kTcRows, p.R - p.r0));
+                if (threadIdx.x == 0u) note_cut(pc, st, p, min(L::ROWS, p.R - p.r0));
             }
             tc_fence_before();   // (the next P V overwrites the accumulator behind an arrival of this thread)
         }
@@ -702,13 +745,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kWarpMma) tmem_dealloc<false>(tmem, kTmemCols);
+    if (warp == L::MMA) tmem_dealloc<false>(tmem, L::TMEM);
 }
 
 template <int D, bool EXACT>
 static bool launch_tc_t(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t ctas) {
-    if (!ensure_dynamic_smem<paged_tc_kernel<D, EXACT>>((int)Tc<D>::smem(kMaxSeqs))) return false;
-    launch_pdl(paged_tc_kernel<D, EXACT>, dim3(ctas), dim3(kTcThreads), Tc<D>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, maps.q, pc);
+    if (!ensure_dynamic_smem<paged_tc_kernel<D, EXACT>>((int)Tc<D, EXACT>::smem(kMaxSeqs))) return false;
+    launch_pdl(paged_tc_kernel<D, EXACT>, dim3(ctas), dim3(Tc<D, EXACT>::THREADS), Tc<D, EXACT>::smem(pc.prefix ? 1u : pc.n_seqs), a.stream, maps.k, maps.v, maps.q, pc);
     return true;
 }
 

@@ -253,6 +253,24 @@ def test_numbers_that_do_not_fit_are_left_out_and_counted(ctx):
     s.close()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_runs_of_pages_that_are_not_there(ctx, D):
+    """Whole key tiles, and more of them than lie between two additions of an accumulator, without a page: in front, inside, at the end."""
+    kv, q = 2500, 90
+    for gone in (range(0, 60), range(40, 100), range(70, 156)):
+        s = Setup(ctx, [q], [kv], 4, 2, D, garbage=True)
+        bad = s.table.copy()
+        bad[0, list(gone)] = -1
+        s.seqs.table.write(bad)
+        got = s.attend(), s.attend(f16=True)
+        keep = [p for i, p in enumerate(s.table[0]) if i not in gone]
+        for j in range(q):
+            seen = sum(1 for key in range(kv - q + j + 1) if key // 16 not in gone)
+            w = ref.attention(s.q[j:j + 1], s.k, s.v, [keep], [0, 1], [seen], s.D ** -0.5)[0]
+            assert np.max(np.abs(w - got[0][j])) <= TOL32 and np.max(np.abs(w - got[1][j])) <= TOL16, (gone, j)
+        s.close()
+
+
 def test_prefix_batches_that_do_not_fit_are_left_out(ctx):
     s = Setup(ctx, [1, 2, 1], [20, 30, 5], 4, 2, 128, prefix=200)
     for buf, value in ((s.seqs.kv_len, np.array([20, 999, 5], np.int32)), (s.seqs.q_start, np.array([1, 1, 3, 4], np.int32))):
