@@ -16,7 +16,7 @@
 // Tensor memory: four S / P tiles of 64 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
 // steps of 16 keys that none sees; V rows behind the last key are zeroed before they are multiplied (a page holds anything there).
 // The tensor core's sums are cut rather than rounded, which an f16 result does not show and a 32-bit one would (2.2e-6 after 300 of them, in
-// proportion to their number): for those the accumulator is added to a sum in registers every kFlush tiles and begins anew, which takes
+// proportion to their number): for those two accumulators take kFlush tiles each in turn and are added to a sum in registers, which takes
 // the registers of a second group's softmax.
 // Every wait on a barrier is bounded (paged.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
 #include <cstring>
@@ -40,14 +40,14 @@ template <int D, bool EXACT>
 struct Tc {
     static constexpr uint32_t GROUPS = EXACT ? 1 : 2, ROWS = GROUPS * kGroupRows;
     static constexpr uint32_t MMA = 4 * GROUPS, LOAD = MMA + GROUPS, QWARP = LOAD + 1, THREADS = EXACT ? 256 : 384;   // warps by role
-    static constexpr uint32_t TMEM = EXACT ? 256 : 512;
+    static constexpr uint32_t TMEM = EXACT && D == 64 ? 256 : 512;
     static constexpr uint32_t A = D / 64, STAGES = EXACT || D == 64 ? 5 : 3;
     static constexpr uint32_t Q = A * kGroupRows * 128u, TILE = A * kTcKeys * 128u;
     static constexpr uint32_t STAGE_OUT = GROUPS * 4u * 32u * 64u;   // a warp's 32 rows x 16 columns on their way out
     static constexpr uint32_t FIXED = 1024u + GROUPS * Q + 2u * STAGES * TILE + STAGE_OUT + 512u;
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
-constexpr uint32_t kFlush = 8;   // EXACT: key tiles between two additions of the accumulator to the row's sum
+constexpr uint32_t kFlush = 4;   // EXACT: key tiles that an accumulator takes before it is added to the row's sum
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int page) {
     asm volatile(
@@ -343,6 +343,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         const uint32_t g = warp - L::MMA;
         const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
         const uint32_t t_s = tmem + 2u * g * kTcKeys, t_o = tmem + 2u * GROUPS * kTcKeys + g * D;
+        // EXACT: the accumulator of the group's tile i of a piece, two in turn
+        auto acc_of = [](uint32_t i) { return EXACT ? (i / kFlush & 1u) * (uint32_t)D : 0u; };
         const uint64_t dq = make_smem_desc(smem_u32(sQ + g * L::Q)), dk = make_smem_desc(smem_u32(sK)), dv = v_desc(smem_u32(sV));
         const uint32_t my_s = s_full + 16u * g, my_p = p_full + 16u * g, my_pv = pv_done + 16u * g;
         Ring kr(ST), vr(ST);
@@ -363,7 +365,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (!ok) break;
                     tc_fence_after();
                     if (EXACT && (t - 2u - x.t0) % kFlush == 0u) started = 0u;
-                    mma_step<A, EXACT>(t_o, t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
+                    mma_step<A, EXACT>(t_o + acc_of(t - 2u - x.t0), t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
                                        dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
                     started = 1u;
                     if (t + 1u == x.t1) commit(q_empty + 8u * g);
@@ -386,10 +388,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         ++p_tiles;
                         tc_fence_after();
                         if (EXACT && (u - x.t0) % kFlush == 0u) started = 0u;
+                        const uint32_t t_acc = t_o + acc_of(u - x.t0);
                         const uint32_t steps = ~bad_2 & 0xFu;   // 16 keys whose page is there
                         const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
                         if (steps == 0xFu && key0 >= x.lo && key0 + kTcKeys <= x.hi) {
-                            mma_pv<EXACT>(t_o, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
+                            mma_pv<EXACT>(t_acc, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
                             started = 1u;
                         } else {
                             if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
@@ -406,8 +409,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 #pragma unroll 1
                             for (uint32_t k = s0; k < s1; ++k) {   // 16 keys a step: 8 columns of P, two groups of eight V rows
                                 if (!(steps >> k & 1u)) continue;
-                                mma_ts(t_o, t_s + b * kTcKeys + 8u * k, dvt + 128u * k, idesc_o, started);
-                                if (EXACT) mma_ts(t_o, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
+                                mma_ts(t_acc, t_s + b * kTcKeys + 8u * k, dvt + 128u * k, idesc_o, started);
+                                if (EXACT) mma_ts(t_acc, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
                                 started = 1u;
                             }
                             if (EXACT && !started) {   // no page of the tile is there, and the accumulator is to begin anew: with zeros
@@ -418,7 +421,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                 }
                                 fence_async_smem();
                                 __syncwarp();
-                                mma_ts(t_o, t_s + b * kTcKeys + 8u * s0, dvt + 128u * s0, idesc_o, 0u);
+                                mma_ts(t_acc, t_s + b * kTcKeys + 8u * s0, dvt + 128u * s0, idesc_o, 0u);
                                 started = 1u;
                             }
                             commit(my_pv + 8u * b);
@@ -517,11 +520,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const bool valid = my < x.rows;
             const Span span = valid ? row_span(pc, p.q, row) : Span{0u, 0u};
             float m_run = neg_inf(), l_run = 0.0f;
-            float sum_o[EXACT ? D : 1];   // EXACT: the row's sum; the accumulator holds the tiles since the last addition
+            float sum_o[EXACT ? D : 1];   // EXACT: the row's sum; the accumulators hold the last tiles
             if (EXACT) {
 #pragma unroll
                 for (uint32_t c = 0; c < (uint32_t)D; ++c) sum_o[c] = 0.0f;
             }
+            auto add_up = [&](uint32_t acc) {
+#pragma unroll
+                for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
+                    uint32_t v[32];
+                    tmem_ld32_async(to + acc * (uint32_t)D + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (uint32_t k = 0; k < 32u; ++k) sum_o[EXACT ? c + k : 0u] += __uint_as_float(v[k]);
+                }
+            };
             for (uint32_t t = x.t0; t < x.t1; ++t, ++j) {
                 const uint32_t key0 = t * kTcKeys, b = j & 1u, ts = tmem + lanes + (2u * g + b) * kTcKeys;
                 ok = ok && wait_on(s_full + 16u * g + 8u * b, (j >> 1) & 1u, ctl, pc.status, 0xDA0u);
@@ -556,20 +569,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 #pragma unroll
                 for (uint32_t k = 8u; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
                 const float mul = scaled ? pc.scale2 : 1.0f, mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * mul;
-                const bool added = EXACT && (t - x.t0) % kFlush == 0u;   // the accumulator begins anew with this tile
-                if (EXACT && added && t != x.t0) {
-                    ok = wait_on(pv_done + 16u * g + 8u * (b ^ 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDC4u);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
-                        uint32_t v[16];
-                        tmem_ld16(to + c, v);
-#pragma unroll
-                        for (uint32_t k = 0; k < 16u; ++k) sum_o[EXACT ? c + k : 0u] += __uint_as_float(v[k]);
-                    }
-                }
+                // The accumulator that tile t - 2 completed is added up now: its P V is done, since S of this tile was issued behind it.
+                if (EXACT && t - x.t0 > kFlush && (t - x.t0) % kFlush == 1u) add_up((t - 2u - x.t0) / kFlush & 1u);
                 const bool grow = mx > m_run + kGrowth || (m_run == neg_inf() && mx != neg_inf());
                 if (__any_sync(0xffffffffu, grow)) {   // a row's sum and accumulator move to the new reference
                     const float f = !grow ? 1.0f : weight(m_run, mx);
@@ -579,7 +580,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 #pragma unroll
                         for (uint32_t c = 0; c < (uint32_t)D; ++c) sum_o[EXACT ? c : 0u] *= f;
                     }
-                    if (t != x.t0 && !added) {
+                    if (t != x.t0) {
+                        const uint32_t last = to + (EXACT ? ((t - 1u - x.t0) / kFlush & 1u) * (uint32_t)D : 0u);   // what tile t - 1 went to
                         ok = wait_on(pv_done + 16u * g + 8u * (b ^ 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDC8u);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
@@ -587,10 +589,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 #pragma unroll 1
                         for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
                             uint32_t v[16];
-                            tmem_ld16(to + c, v);
+                            tmem_ld16(last + c, v);
 #pragma unroll
                             for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-                            tmem_st16_async(to + c, v);
+                            tmem_st16_async(last + c, v);
                         }
                     }
                 }
@@ -630,6 +632,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             if (!ok) break;
             tc_fence_after();
             tiles += p.b - p.a;
+            // (the last tile's accumulator is read below; the other one where that tile was its first)
+            const uint32_t n_tiles = x.t1 - x.t0, to_last = to + (EXACT && some ? ((n_tiles - 1u) / kFlush & 1u) * (uint32_t)D : 0u);
+            if (EXACT && some && n_tiles > 1u && (n_tiles - 1u) % kFlush == 0u) add_up((n_tiles - 2u) / kFlush & 1u);
             if (x.rows) {
                 const uint32_t token = p.q.tok0 + row / pc.G, head = p.group * pc.G + row % pc.G;
                 float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * L::ROWS + (x.r0 - p.r0)) * (D + 4u);
@@ -678,7 +683,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 #pragma unroll(EXACT ? D / 16 : 1)
                 for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
                     uint32_t v[16];
-                    if (some) tmem_ld16(to + c, v);
+                    if (some) tmem_ld16(to_last + c, v);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const float o = nothing || !some ? 0.0f : EXACT ? sum_o[EXACT ? c + j : 0u] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
