@@ -36,6 +36,7 @@ struct Args {
     float* slots;               // results of cut row tiles: slot 2 c (a tile begun elsewhere), 2 c + 1 (one that goes on elsewhere)
     uint4* cut;                 // per CTA what the merge kernel needs of a cut row tile: parts | group << 16 (0: none), first token, first row, rows
     uint32_t q_boxes;           // the map of q serves the rows of a group
+    uint32_t report;            // this launch counts the sequences that do not fit
     uint32_t HB, groups, keys_log2, over;   // KV heads of a group, groups, the line's tiles and its allowance per row tile
     const float* extra;         // results over other keys of the same rows that the final ones take in (the layout of OUT_PARTS)
     uint32_t* refused;          // the caller's status words: count of refused entries, lowest node
@@ -106,7 +107,7 @@ __device__ __forceinline__ uint32_t build_line(const Args& pc, uint32_t* s_pref,
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     // lanes take sequences while there is a row tile or two of each, row tiles of one sequence where there are many
     const bool tiles_by_lane = (uint64_t)pc.max_q * pc.G > 4u * ROWS && (!pc.prefix);
-    const bool report = blockIdx.x == 0u;
+    const bool report = blockIdx.x == 0u && pc.report;
     bool whole = true;   // a shared prefix serves a batch without refused sequences, whose rows begin at 0
     if (pc.prefix) {
         bool fits = pc.q_start[0] == 0;

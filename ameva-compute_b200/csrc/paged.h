@@ -8,6 +8,7 @@ namespace paged {
 // Maps of the cache for boxes of 64 columns x tokens x heads of one page, and of q for 64 columns x the heads of a group x tokens.
 struct Maps {
     CUtensorMap k, v, q;
+    bool q_boxes;   // q's map serves the rows of a group
 };
 
 constexpr uint32_t kDecRows = 16;                        // paged_attn.cu: rows per tile

@@ -9,6 +9,7 @@
 // rounded: a 32-bit angle of position 300000 is off by up to 0.02 of a radian, which the rotated element would show. A CTA takes T
 // tokens: their angles by one thread each (64-bit products: theta_scale^j by squaring), then every thread rotates 8 elements of a
 // head at a time from 16-byte loads. Bound by HBM: 6 (H + 2 Hkv) D bytes per token.
+#include <algorithm>
 #include <cstring>
 
 #include "paged.cuh"
@@ -180,6 +181,20 @@ __global__ void __launch_bounds__(256, 8) append_kernel(const float* __restrict_
 
 }  // namespace paged
 
+// Whether (pages, tokens, heads) of D elements with these strides lie beside one another, in whatever order.
+static bool strides_apart(uint64_t D, uint64_t ps, uint64_t pages, uint64_t ts, uint64_t tokens, uint64_t hs, uint64_t heads) {
+    struct Dim {
+        uint64_t stride, n;
+    } dims[3] = {{ps, pages}, {ts, tokens}, {hs, heads}};
+    std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+    uint64_t span = D;
+    for (const Dim& d : dims) {
+        if (d.n == 1u) continue;
+        if (d.stride < span) return false;
+        span += d.stride * (d.n - 1u);
+    }
+    return true;
+}
 static bool ranges_meet(const LaunchArgs& a, uint32_t i, uint32_t j) {
     const uintptr_t p = (uintptr_t)a.ptr[i], q = (uintptr_t)a.ptr[j];
     return p < q + a.range[j] && q < p + a.range[i];
@@ -217,6 +232,7 @@ AcResult launch_paged_append(const LaunchArgs& a) {
         ((pc.flags & kHasFactors) && a.range[7] < (uint64_t)(pc.n_dims / 2u) * 4u) || a.range[8] < (last * pc.o_s + qw) * 2u ||
         a.range[9] < cache || a.range[10] < cache || a.range[11] < 8u)
         return AC_ERR_INVALID_BUFFER_SIZE;
+    if ((last && pc.o_s < qw) || !strides_apart(pc.D, pc.c_ps, pc.n_pages, pc.c_ts, pc.page_size, pc.c_hs, pc.n_head_kv)) return AC_ERR_INVALID_SHAPE;
     for (uint32_t o : {8u, 9u, 10u, 11u})   // what is written meets nothing else
         for (uint32_t i = 0; i < 12u; ++i) {
             const bool unused = (i == 6u && !(pc.flags & kHasPositions)) || (i == 7u && !(pc.flags & kHasFactors));

@@ -679,6 +679,7 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
         a.range[3] < (uint64_t)pc.n_seqs * pc.table_stride * 4u || a.range[4] < ((uint64_t)pc.n_seqs + 1u) * 4u || a.range[5] < (uint64_t)pc.n_seqs * 4u ||
         a.range[6] < (last * pc.dst_s + width) * esize || a.range[8] < 8u)
         return AC_ERR_INVALID_BUFFER_SIZE;
+    if (last && pc.dst_s < width) return AC_ERR_INVALID_SHAPE;   // rows of the result that overlap
     for (uint32_t o : {6u, 7u, 8u})   // what is written meets nothing else
         for (uint32_t i = 0; i < a.binding_count; ++i)
             if (i != o && meet(a, o, i)) return AC_ERR_KERNEL_ARG_INVALID;
@@ -722,34 +723,49 @@ static uint32_t ctas_for(uint64_t room, uint64_t tile_bytes, uint32_t sms) {
     return n < 1u ? 1u : n > sms ? sms : (uint32_t)n;
 }
 
-// One attention over one set of keys: the sequences of few rows, those of many, and the join of what both cut.
-static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t max_rows, Scratch scratch, const Maps& rows_maps, const Maps& tc_maps) {
-    const uint32_t sms = a.sm_count > 0 ? (uint32_t)a.sm_count : 148u;
+// One attention over one set of keys: which kernels run, and the line of each.
+struct Plan {
+    Args few, many;
+    bool use_few, use_many;
+    uint32_t tc_rows;
+};
+static AcResult plan_set(const Args& pc, uint32_t D, uint64_t max_rows, Plan& x) {
     const bool both = D <= 128u && max_rows > kFewRows;
-    const uint64_t row = (D + 4u) * 4u;
-    Args few = pc, many = pc;
-    few.min_rows = 1u;
-    few.max_rows = both ? kFewRows : 0xFFFFFFFFu;
-    many.min_rows = pc.prefix ? 1u : kFewRows + 1u;   // (a prefix has one number of rows, and one kernel)
-    many.max_rows = 0xFFFFFFFFu;
-    const bool use_few = !both || !pc.prefix, use_many = both;
-    few.HB = few_heads(D, pc.n_head_kv);
-    few.groups = (pc.n_head_kv + few.HB - 1u) / few.HB;
-    const uint32_t kb = blocks_of(D == 256u ? 4u : 8u, few.HB);
-    for (few.keys_log2 = 5u; (1u << (few.keys_log2 - 5u)) < kb; ++few.keys_log2) {}
-    few.over = kFewOver;
-    many.HB = 1u;
-    many.groups = pc.n_head_kv;
-    many.keys_log2 = 6u;
-    many.over = kManyOver;
-    const uint32_t tc_rows = pc.out == OUT_F16 ? kTcRows : kTcRows / 2u;   // (paged_tc.cu)
+    x.few = x.many = pc;
+    x.few.min_rows = 1u;
+    x.few.max_rows = both ? kFewRows : 0xFFFFFFFFu;
+    x.many.min_rows = pc.prefix ? 1u : kFewRows + 1u;   // (a prefix has one number of rows, and one kernel)
+    x.many.max_rows = 0xFFFFFFFFu;
+    x.use_few = !both || !pc.prefix;
+    x.use_many = both;
+    x.few.report = 1u;                                  // (what both kernels meet is counted by one)
+    x.many.report = !x.use_few;
+    x.few.HB = few_heads(D, pc.n_head_kv);
+    x.few.groups = (pc.n_head_kv + x.few.HB - 1u) / x.few.HB;
+    const uint32_t kb = blocks_of(D == 256u ? 4u : 8u, x.few.HB);
+    for (x.few.keys_log2 = 5u; (1u << (x.few.keys_log2 - 5u)) < kb; ++x.few.keys_log2) {}
+    x.few.over = kFewOver;
+    x.many.HB = 1u;
+    x.many.groups = pc.n_head_kv;
+    x.many.keys_log2 = 6u;
+    x.many.over = kManyOver;
+    x.tc_rows = pc.out == OUT_F16 ? kTcRows : kTcRows / 2u;   // (paged_tc.cu)
     // the line's length in 32 bits
     const uint64_t few_rows = both ? kFewRows : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs;
-    auto too_long = [&](const Args& x, uint64_t row_tiles) {
-        return seqs * x.groups * row_tiles * (((uint64_t)pc.max_kv >> x.keys_log2) + 2u + x.over) > 0xFFFFFFFFull;
+    auto too_long = [&](const Args& y, uint64_t row_tiles) {
+        return seqs * y.groups * row_tiles * (((uint64_t)pc.max_kv >> y.keys_log2) + 2u + y.over) > 0xFFFFFFFFull;
     };
-    if (use_few && too_long(few, (few_rows + kDecRows - 1u) / kDecRows)) return AC_ERR_INVALID_SHAPE;
-    if (use_many && too_long(many, (max_rows + tc_rows - 1u) / tc_rows)) return AC_ERR_INVALID_SHAPE;
+    if (x.use_few && too_long(x.few, (few_rows + kDecRows - 1u) / kDecRows)) return AC_ERR_INVALID_SHAPE;
+    if (x.use_many && too_long(x.many, (max_rows + x.tc_rows - 1u) / x.tc_rows)) return AC_ERR_INVALID_SHAPE;
+    return AC_SUCCESS;
+}
+// The sequences of few rows, those of many, and the join of what both cut.
+static AcResult launch_set(const LaunchArgs& a, const Plan& x, uint32_t D, Scratch scratch, const Maps& rows_maps, const Maps& tc_maps) {
+    const uint32_t sms = a.sm_count > 0 ? (uint32_t)a.sm_count : 148u, tc_rows = x.tc_rows;
+    const uint64_t row = (D + 4u) * 4u;
+    const bool use_few = x.use_few, use_many = x.use_many;
+    Args few = x.few, many = x.many;
+    few.q_boxes = many.q_boxes = tc_maps.q_boxes;
     uint32_t n_few = 0, n_many = 0;
     if (use_few) {
         n_few = ctas_for(use_many ? scratch.left * few.HB / (few.HB + 16u) : scratch.left, few.HB * kDecRows * row, sms);
@@ -770,7 +786,7 @@ static AcResult launch_set(const LaunchArgs& a, Args pc, uint32_t D, uint64_t ma
     return check_launch();
 }
 
-static AcResult cache_maps(const LaunchArgs& a, Args& pc, uint32_t D, Maps& rows_maps, Maps& tc_maps) {
+static AcResult cache_maps(const LaunchArgs& a, const Args& pc, uint32_t D, Maps& rows_maps, Maps& tc_maps) {
     tc::EncodeTiledFn enc = tc::encode_fn();
     const uint32_t P = 1u << pc.page_log2, heads = few_heads(D, pc.n_head_kv), tc_box = P < kTcKeys ? P : kTcKeys;
     if (!enc) return AC_ERR_DRIVER_SYMBOL_MISSING;
@@ -778,11 +794,11 @@ static AcResult cache_maps(const LaunchArgs& a, Args& pc, uint32_t D, Maps& rows
                     encode_cache(enc, &tc_maps.k, a.ptr[1], pc, D, tc_box, 1u) && encode_cache(enc, &tc_maps.v, a.ptr[2], pc, D, tc_box, 1u);
     if (!ok) return AC_ERR_INVALID_SHAPE;
     memset(&tc_maps.q, 0, sizeof(tc_maps.q));
-    pc.q_boxes = D <= 128u && (pc.G & (pc.G - 1u)) == 0u && pc.G <= 128u;
-    if (pc.q_boxes) {
+    tc_maps.q_boxes = D <= 128u && (pc.G & (pc.G - 1u)) == 0u && pc.G <= 128u;
+    if (tc_maps.q_boxes) {
         const cuuint64_t dims[3] = {D, pc.n_head, pc.rows}, strides[2] = {2ull * D, 2ull * (pc.rows > 1u ? pc.q_s : (uint64_t)pc.n_head * D)};
         const cuuint32_t box[3] = {64, pc.G, 128u / pc.G}, estr[3] = {1, 1, 1};
-        pc.q_boxes = strides[1] && enc(&tc_maps.q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.ptr[0], dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        tc_maps.q_boxes = strides[1] && enc(&tc_maps.q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.ptr[0], dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     }
     return AC_SUCCESS;
@@ -807,10 +823,13 @@ AcResult launch_paged_attn(const LaunchArgs& a) {
     if (rc != AC_SUCCESS) return rc;
     pc.window = a.push[18];
     pc.node = a.push[19];
+    Plan plan;
+    rc = plan_set(pc, D, (uint64_t)pc.max_q * pc.G, plan);
+    if (rc != AC_SUCCESS) return rc;
     Maps rows_maps, tc_maps;
     rc = cache_maps(a, pc, D, rows_maps, tc_maps);
     if (rc != AC_SUCCESS) return rc;
-    return launch_set(a, pc, D, (uint64_t)pc.max_q * pc.G, {(uint8_t*)a.ptr[7], a.range[7]}, rows_maps, tc_maps);
+    return launch_set(a, plan, D, {(uint8_t*)a.ptr[7], a.range[7]}, rows_maps, tc_maps);
 }
 
 // ameva_paged_prefix_attn: the same for sequences that share a prefix, whose pages are read once for all of them. Binding 9: prefix i32
@@ -828,16 +847,14 @@ AcResult launch_paged_prefix_attn(const LaunchArgs& a) {
     if (max_prefix > 0x7FFFFFFFu - 1024u) return AC_ERR_INVALID_SHAPE;
     if ((uintptr_t)a.ptr[9] & 3u) return AC_ERR_BUFFER_ALIGNMENT_INVALID;
     if (a.range[9] < 4u + 4ull * (((uint64_t)max_prefix + (1u << pc.page_log2) - 1u) >> pc.page_log2)) return AC_ERR_INVALID_BUFFER_SIZE;
-    Maps rows_maps, tc_maps;
-    rc = cache_maps(a, pc, D, rows_maps, tc_maps);
-    if (rc != AC_SUCCESS) return rc;
     Scratch scratch = {(uint8_t*)a.ptr[7], a.range[7]};
     float* own = (float*)scratch.take((uint64_t)pc.rows * pc.n_head * (D + 4u) * 4u);
     if (!own) return AC_ERR_INVALID_BUFFER_SIZE;
     Args first = pc;   // the sequences' own keys
     first.dst = own;
     first.out = OUT_PARTS;
-    rc = launch_set(a, first, D, (uint64_t)pc.max_q * pc.G, scratch, rows_maps, tc_maps);
+    Plan own_plan, plan;
+    rc = plan_set(first, D, (uint64_t)pc.max_q * pc.G, own_plan);
     if (rc != AC_SUCCESS) return rc;
     pc.extra = own;    // the prefix, for all rows at once, with those taken in
     pc.prefix = (const int32_t*)a.ptr[9];
@@ -845,7 +862,13 @@ AcResult launch_paged_prefix_attn(const LaunchArgs& a) {
     pc.max_own_kv = pc.max_kv;
     pc.max_q = pc.rows;
     pc.max_kv = max_prefix;
-    return launch_set(a, pc, D, (uint64_t)pc.rows * pc.G, scratch, rows_maps, tc_maps);
+    rc = plan_set(pc, D, (uint64_t)pc.rows * pc.G, plan);
+    if (rc != AC_SUCCESS) return rc;
+    Maps rows_maps, tc_maps;
+    rc = cache_maps(a, pc, D, rows_maps, tc_maps);
+    if (rc != AC_SUCCESS) return rc;
+    rc = launch_set(a, own_plan, D, scratch, rows_maps, tc_maps);
+    return rc != AC_SUCCESS ? rc : launch_set(a, plan, D, scratch, rows_maps, tc_maps);
 }
 
 }  // namespace amv

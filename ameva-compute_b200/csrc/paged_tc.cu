@@ -280,234 +280,234 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     bool ok = true;
 
     if (warp >= L::MMA) {
-    if constexpr (!EXACT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == L::LOAD) {
-        Ring kr(ST), vr(ST);
-        uint32_t tiles = 0;     // of this CTA so far
-        uint32_t k_issued = 0, v_issued = 0;
-        while (ok && walk.next(pc, s_pref)) {
-            const Piece& p = walk.p;
-            const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + L::ROWS, p.R) - 1u).hi;
-            int32_t page = -1, page_v = -1;   // this lane's box: K's, and V's of the tile before
-            uint32_t load = 0, load_v = 0;
-            for (uint32_t i = p.a; ok && i <= p.b; ++i) {
-                const uint32_t key0 = (p.first + i) * kTcKeys, b0 = key0 + lane * box;
-                if (i < p.b) {
-                    const bool want = lane < boxes && b0 < hi && b0 + box > lo;
-                    page = want ? page_of(pc, p.q, b0) : -1;
-                    const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0);
-                    load = __ballot_sync(0xffffffffu, page >= 0);
-                    uint32_t bad = 0;
-                    if (none) {
-                        for (uint32_t j = 0; j < kTcKeys / 16u; ++j) bad |= (none >> (16u * j / box) & 1u) << j;
-                        if (lane == 0u) refuse(pc, __popc(none));
-                    }
-                    ok = wait_on(k_empty + 8u * kr.idx, kr.phase ^ 1u, ctl, pc.status, 0xD00u);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (lane == 0u) {
-                        s_bad[tiles & (kBadRing - 1u)] = bad;
-                        mbar_arrive_expect_tx(k_full + 8u * kr.idx, (uint32_t)__popc(load) * box * 128u * A);
-                    }
-                    __syncwarp();
-                    if (page >= 0)
-                        for (uint32_t a = 0; a < A; ++a)
-                            tma_box(smem_u32(sK + kr.idx * L::TILE) + a * (kTcKeys * 128u) + lane * box * 128u, &k_map, k_full + 8u * kr.idx,
-                                    (int)(64u * a), (int)(b0 & (P - 1u)), (int)p.group, page);
-                    ++k_issued;
-                    ++tiles;
-                    kr.advance();
-                }
-                if (i > p.a) {   // V of the tile before
-                    ok = wait_on(v_empty + 8u * vr.idx, vr.phase ^ 1u, ctl, pc.status, 0xD10u);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (lane == 0u) mbar_arrive_expect_tx(v_full + 8u * vr.idx, (uint32_t)__popc(load_v) * box * 128u * A);
-                    __syncwarp();
-                    if (page_v >= 0)
-                        for (uint32_t a = 0; a < A; ++a)
-                            tma_box(smem_u32(sV + vr.idx * L::TILE) + a * (kTcKeys * 128u) + lane * box * 128u, &v_map, v_full + 8u * vr.idx,
-                                    (int)(64u * a), (int)((b0 - kTcKeys) & (P - 1u)), (int)p.group, page_v);
-                    ++v_issued;
-                    vr.advance();
-                }
-                page_v = page;
-                load_v = load;
-            }
-        }
-        if (ctl->abort) {   // copies already requested finish before the CTA leaves
-            for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) wait_on(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
-            for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) wait_on(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
-        }
-    } else if (warp < L::LOAD) {
-        const uint32_t g = warp - L::MMA;
-        const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
-        const uint32_t t_s = tmem + 2u * g * kTcKeys, t_o = tmem + 2u * GROUPS * kTcKeys + g * D;
-        // EXACT: the accumulator of the group's tile i of a piece, two in turn
-        auto acc_of = [](uint32_t i) { return EXACT ? (i / kFlush & 1u) * (uint32_t)D : 0u; };
-        const uint64_t dq = make_smem_desc(smem_u32(sQ + g * L::Q)), dk = make_smem_desc(smem_u32(sK)), dv = v_desc(smem_u32(sV));
-        const uint32_t my_s = s_full + 16u * g, my_p = p_full + 16u * g, my_pv = pv_done + 16u * g;
-        Ring kr(ST), vr(ST);
-        uint32_t tiles = 0, q_uses = 0, s_tiles = 0, p_tiles = 0;   // of the CTA; of this group: pieces with Q, tiles with S, with P V issued
-        while (ok && walk.next(pc, s_pref)) {
-            const Piece& p = walk.p;
-            const Group x = group_of(pc, p, g);
-            const uint32_t hi_all = row_span(pc, p.q, min(p.r0 + L::ROWS, p.R) - 1u).hi, T0 = p.first + p.a, T1 = p.first + p.b;
-            uint32_t started = 0u;
-            uint32_t bad_1 = 0u, bad_2 = 0u;   // 16-key steps without a page, of tile t - 1 and t - 2
-            for (uint32_t t = T0; t < T1 + 2u; ++t) {   // P V of tile t - 2, then S of tile t in its place
-                // (the group's rows see some of tile t, all of tile t - 2, and neither is its first)
-                if (t >= T0 + 2u && t < T1 && t - 2u >= x.t0 && t < x.t1 && bad_2 == 0u && (t - 2u) * kTcKeys >= x.lo) {
-                    const uint32_t b = p_tiles & 1u;
-                    ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u) && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u) &&
-                         wait_on(my_p + 8u * b, (p_tiles >> 1) & 1u, ctl, pc.status, 0xD50u);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (EXACT && (t - 2u - x.t0) % kFlush == 0u) started = 0u;
-                    mma_step<A, EXACT>(t_o + acc_of(t - 2u - x.t0), t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
-                                       dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
-                    started = 1u;
-                    if (t + 1u == x.t1) commit(q_empty + 8u * g);
-                    bad_2 = bad_1;
-                    bad_1 = s_bad[(tiles + (t - T0)) & (kBadRing - 1u)];
-                    ++p_tiles;
-                    ++s_tiles;
-                    vr.advance();
-                    kr.advance();
-                    continue;
-                }
-                if (t >= T0 + 2u) {
-                    const uint32_t u = t - 2u, key0 = u * kTcKeys, b = p_tiles & 1u;
-                    const bool mine = u >= x.t0 && u < x.t1;
-                    ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
-                    if (mine) ok = ok && wait_on(my_p + 8u * b, (p_tiles >> 1) & 1u, ctl, pc.status, 0xD50u);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (mine) {
-                        ++p_tiles;
-                        tc_fence_after();
-                        if (EXACT && (u - x.t0) % kFlush == 0u) started = 0u;
-                        const uint32_t t_acc = t_o + acc_of(u - x.t0);
-                        const uint32_t steps = ~bad_2 & 0xFu;   // 16 keys whose page is there
-                        const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
-                        if (steps == 0xFu && key0 >= x.lo && key0 + kTcKeys <= x.hi) {
-                            mma_pv<EXACT>(t_acc, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
-                            started = 1u;
-                        } else {
-                            if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
-                                const uint32_t from = hi_all - key0, n = (16u - (from & 15u)) & 15u;
-                                for (uint32_t j = lane; j < n * (D / 8u); j += 32u) {
-                                    const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
-                                    *reinterpret_cast<uint4*>(sV + vr.idx * L::TILE + (c >> 3) * (kTcKeys * 128u) + r * 128u + ((c & 7u) << 4)) =
-                                        make_uint4(0u, 0u, 0u, 0u);
-                                }
-                                fence_async_smem();
-                                __syncwarp();
-                            }
-                            const uint32_t s0 = x.lo > key0 ? (x.lo - key0) / 16u : 0u, s1 = (min(x.hi - key0, kTcKeys) + 15u) / 16u;
-#pragma unroll 1
-                            for (uint32_t k = s0; k < s1; ++k) {   // 16 keys a step: 8 columns of P, two groups of eight V rows
-                                if (!(steps >> k & 1u)) continue;
-                                mma_ts(t_acc, t_s + b * kTcKeys + 8u * k, dvt + 128u * k, idesc_o, started);
-                                if (EXACT) mma_ts(t_acc, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
-                                started = 1u;
-                            }
-                            if (EXACT && !started) {   // no page of the tile is there, and the accumulator is to begin anew: with zeros
-                                for (uint32_t j = lane; j < 16u * (D / 8u); j += 32u) {
-                                    const uint32_t r = 16u * s0 + j / (D / 8u), c = j % (D / 8u);
-                                    *reinterpret_cast<uint4*>(sV + vr.idx * L::TILE + (c >> 3) * (kTcKeys * 128u) + r * 128u + ((c & 7u) << 4)) =
-                                        make_uint4(0u, 0u, 0u, 0u);
-                                }
-                                fence_async_smem();
-                                __syncwarp();
-                                mma_ts(t_acc, t_s + b * kTcKeys + 8u * s0, dvt + 128u * s0, idesc_o, 0u);
-                                started = 1u;
-                            }
-                            commit(my_pv + 8u * b);
-                            commit(v_empty + 8u * vr.idx);
+        if constexpr (!EXACT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == L::LOAD) {
+            Ring kr(ST), vr(ST);
+            uint32_t tiles = 0;     // of this CTA so far
+            uint32_t k_issued = 0, v_issued = 0;
+            while (ok && walk.next(pc, s_pref)) {
+                const Piece& p = walk.p;
+                const uint32_t lo = row_span(pc, p.q, p.r0).lo, hi = row_span(pc, p.q, min(p.r0 + L::ROWS, p.R) - 1u).hi;
+                int32_t page = -1, page_v = -1;   // this lane's box: K's, and V's of the tile before
+                uint32_t load = 0, load_v = 0;
+                for (uint32_t i = p.a; ok && i <= p.b; ++i) {
+                    const uint32_t key0 = (p.first + i) * kTcKeys, b0 = key0 + lane * box;
+                    if (i < p.b) {
+                        const bool want = lane < boxes && b0 < hi && b0 + box > lo;
+                        page = want ? page_of(pc, p.q, b0) : -1;
+                        const uint32_t none = __ballot_sync(0xffffffffu, want && page < 0);
+                        load = __ballot_sync(0xffffffffu, page >= 0);
+                        uint32_t bad = 0;
+                        if (none) {
+                            for (uint32_t j = 0; j < kTcKeys / 16u; ++j) bad |= (none >> (16u * j / box) & 1u) << j;
+                            if (lane == 0u) refuse(pc, __popc(none));
                         }
-                    } else if (lane == 0u) {
-                        mbar_arrive(v_empty + 8u * vr.idx);
+                        ok = wait_on(k_empty + 8u * kr.idx, kr.phase ^ 1u, ctl, pc.status, 0xD00u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0u) {
+                            s_bad[tiles & (kBadRing - 1u)] = bad;
+                            mbar_arrive_expect_tx(k_full + 8u * kr.idx, (uint32_t)__popc(load) * box * 128u * A);
+                        }
+                        __syncwarp();
+                        if (page >= 0)
+                            for (uint32_t a = 0; a < A; ++a)
+                                tma_box(smem_u32(sK + kr.idx * L::TILE) + a * (kTcKeys * 128u) + lane * box * 128u, &k_map, k_full + 8u * kr.idx,
+                                        (int)(64u * a), (int)(b0 & (P - 1u)), (int)p.group, page);
+                        ++k_issued;
+                        ++tiles;
+                        kr.advance();
                     }
-                    vr.advance();
+                    if (i > p.a) {   // V of the tile before
+                        ok = wait_on(v_empty + 8u * vr.idx, vr.phase ^ 1u, ctl, pc.status, 0xD10u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0u) mbar_arrive_expect_tx(v_full + 8u * vr.idx, (uint32_t)__popc(load_v) * box * 128u * A);
+                        __syncwarp();
+                        if (page_v >= 0)
+                            for (uint32_t a = 0; a < A; ++a)
+                                tma_box(smem_u32(sV + vr.idx * L::TILE) + a * (kTcKeys * 128u) + lane * box * 128u, &v_map, v_full + 8u * vr.idx,
+                                        (int)(64u * a), (int)((b0 - kTcKeys) & (P - 1u)), (int)p.group, page_v);
+                        ++v_issued;
+                        vr.advance();
+                    }
+                    page_v = page;
+                    load_v = load;
                 }
-                if (t < T1) {
-                    const bool mine = t >= x.t0 && t < x.t1;
-                    ok = wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
-                    if (mine && t == x.t0) {
-                        ok = ok && wait_on(q_full + 8u * g, q_uses & 1u, ctl, pc.status, 0xD70u);
-                        ++q_uses;
+            }
+            if (ctl->abort) {   // copies already requested finish before the CTA leaves
+                for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) wait_on(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
+                for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) wait_on(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
+            }
+        } else if (warp < L::LOAD) {
+            const uint32_t g = warp - L::MMA;
+            const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
+            const uint32_t t_s = tmem + 2u * g * kTcKeys, t_o = tmem + 2u * GROUPS * kTcKeys + g * D;
+            // EXACT: the accumulator of the group's tile i of a piece, two in turn
+            auto acc_of = [](uint32_t i) { return EXACT ? (i / kFlush & 1u) * (uint32_t)D : 0u; };
+            const uint64_t dq = make_smem_desc(smem_u32(sQ + g * L::Q)), dk = make_smem_desc(smem_u32(sK)), dv = v_desc(smem_u32(sV));
+            const uint32_t my_s = s_full + 16u * g, my_p = p_full + 16u * g, my_pv = pv_done + 16u * g;
+            Ring kr(ST), vr(ST);
+            uint32_t tiles = 0, q_uses = 0, s_tiles = 0, p_tiles = 0;   // of the CTA; of this group: pieces with Q, tiles with S, with P V issued
+            while (ok && walk.next(pc, s_pref)) {
+                const Piece& p = walk.p;
+                const Group x = group_of(pc, p, g);
+                const uint32_t hi_all = row_span(pc, p.q, min(p.r0 + L::ROWS, p.R) - 1u).hi, T0 = p.first + p.a, T1 = p.first + p.b;
+                uint32_t started = 0u;
+                uint32_t bad_1 = 0u, bad_2 = 0u;   // 16-key steps without a page, of tile t - 1 and t - 2
+                for (uint32_t t = T0; t < T1 + 2u; ++t) {   // P V of tile t - 2, then S of tile t in its place
+                    // (the group's rows see some of tile t, all of tile t - 2, and neither is its first)
+                    if (t >= T0 + 2u && t < T1 && t - 2u >= x.t0 && t < x.t1 && bad_2 == 0u && (t - 2u) * kTcKeys >= x.lo) {
+                        const uint32_t b = p_tiles & 1u;
+                        ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u) && wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u) &&
+                             wait_on(my_p + 8u * b, (p_tiles >> 1) & 1u, ctl, pc.status, 0xD50u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (EXACT && (t - 2u - x.t0) % kFlush == 0u) started = 0u;
+                        mma_step<A, EXACT>(t_o + acc_of(t - 2u - x.t0), t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
+                                           dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
+                        started = 1u;
+                        if (t + 1u == x.t1) commit(q_empty + 8u * g);
+                        bad_2 = bad_1;
+                        bad_1 = s_bad[(tiles + (t - T0)) & (kBadRing - 1u)];
+                        ++p_tiles;
+                        ++s_tiles;
+                        vr.advance();
+                        kr.advance();
+                        continue;
                     }
+                    if (t >= T0 + 2u) {
+                        const uint32_t u = t - 2u, key0 = u * kTcKeys, b = p_tiles & 1u;
+                        const bool mine = u >= x.t0 && u < x.t1;
+                        ok = wait_on(v_full + 8u * vr.idx, vr.phase, ctl, pc.status, 0xD40u);
+                        if (mine) ok = ok && wait_on(my_p + 8u * b, (p_tiles >> 1) & 1u, ctl, pc.status, 0xD50u);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (mine) {
+                            ++p_tiles;
+                            tc_fence_after();
+                            if (EXACT && (u - x.t0) % kFlush == 0u) started = 0u;
+                            const uint32_t t_acc = t_o + acc_of(u - x.t0);
+                            const uint32_t steps = ~bad_2 & 0xFu;   // 16 keys whose page is there
+                            const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
+                            if (steps == 0xFu && key0 >= x.lo && key0 + kTcKeys <= x.hi) {
+                                mma_pv<EXACT>(t_acc, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
+                                started = 1u;
+                            } else {
+                                if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
+                                    const uint32_t from = hi_all - key0, n = (16u - (from & 15u)) & 15u;
+                                    for (uint32_t j = lane; j < n * (D / 8u); j += 32u) {
+                                        const uint32_t r = from + j / (D / 8u), c = j % (D / 8u);
+                                        *reinterpret_cast<uint4*>(sV + vr.idx * L::TILE + (c >> 3) * (kTcKeys * 128u) + r * 128u + ((c & 7u) << 4)) =
+                                            make_uint4(0u, 0u, 0u, 0u);
+                                    }
+                                    fence_async_smem();
+                                    __syncwarp();
+                                }
+                                const uint32_t s0 = x.lo > key0 ? (x.lo - key0) / 16u : 0u, s1 = (min(x.hi - key0, kTcKeys) + 15u) / 16u;
+    #pragma unroll 1
+                                for (uint32_t k = s0; k < s1; ++k) {   // 16 keys a step: 8 columns of P, two groups of eight V rows
+                                    if (!(steps >> k & 1u)) continue;
+                                    mma_ts(t_acc, t_s + b * kTcKeys + 8u * k, dvt + 128u * k, idesc_o, started);
+                                    if (EXACT) mma_ts(t_acc, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
+                                    started = 1u;
+                                }
+                                if (EXACT && !started) {   // no page of the tile is there, and the accumulator is to begin anew: with zeros
+                                    for (uint32_t j = lane; j < 16u * (D / 8u); j += 32u) {
+                                        const uint32_t r = 16u * s0 + j / (D / 8u), c = j % (D / 8u);
+                                        *reinterpret_cast<uint4*>(sV + vr.idx * L::TILE + (c >> 3) * (kTcKeys * 128u) + r * 128u + ((c & 7u) << 4)) =
+                                            make_uint4(0u, 0u, 0u, 0u);
+                                    }
+                                    fence_async_smem();
+                                    __syncwarp();
+                                    mma_ts(t_acc, t_s + b * kTcKeys + 8u * s0, dvt + 128u * s0, idesc_o, 0u);
+                                    started = 1u;
+                                }
+                                commit(my_pv + 8u * b);
+                                commit(v_empty + 8u * vr.idx);
+                            }
+                        } else if (lane == 0u) {
+                            mbar_arrive(v_empty + 8u * vr.idx);
+                        }
+                        vr.advance();
+                    }
+                    if (t < T1) {
+                        const bool mine = t >= x.t0 && t < x.t1;
+                        ok = wait_on(k_full + 8u * kr.idx, kr.phase, ctl, pc.status, 0xD60u);
+                        if (mine && t == x.t0) {
+                            ok = ok && wait_on(q_full + 8u * g, q_uses & 1u, ctl, pc.status, 0xD70u);
+                            ++q_uses;
+                        }
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (mine) {
+                            const uint32_t b = s_tiles & 1u;
+                            ++s_tiles;
+                            mma_s<A>(t_s + b * kTcKeys, dq, dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
+                            if (t + 1u == x.t1) commit(q_empty + 8u * g);
+                        } else if (lane == 0u) {
+                            mbar_arrive(k_empty + 8u * kr.idx);
+                        }
+                        kr.advance();
+                    }
+                    bad_2 = bad_1;
+                    bad_1 = t < T1 ? s_bad[(tiles + (t - T0)) & (kBadRing - 1u)] : 0u;
+                }
+                tiles += p.b - p.a;
+            }
+            if (__any_sync(0xffffffffu, ctl->abort != 0u)) {   // MMAs already issued finish before the CTA leaves
+                commit(drain + 8u * g);
+                for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain + 8u * g, 0u); ++spins) __nanosleep(64);
+            }
+        } else if (warp == L::QWARP) {
+            // Q rows into the K-major 128-byte swizzle, idle rows zero
+            uint32_t uses[2] = {0u, 0u};
+            while (ok && walk.next(pc, s_pref)) {
+                const Piece& p = walk.p;
+    #pragma unroll 1
+                for (uint32_t g = 0; g < GROUPS; ++g) {
+                    const Group x = group_of(pc, p, g);
+                    if (x.t1 <= x.t0) continue;
+                    const uint32_t n = g ? uses[1]++ : uses[0]++;
+                    if (n) ok = wait_on(q_empty + 8u * g, (n - 1u) & 1u, ctl, pc.status, 0xDC0u);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (mine) {
-                        const uint32_t b = s_tiles & 1u;
-                        ++s_tiles;
-                        mma_s<A>(t_s + b * kTcKeys, dq, dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
-                        if (t + 1u == x.t1) commit(q_empty + 8u * g);
-                    } else if (lane == 0u) {
-                        mbar_arrive(k_empty + 8u * kr.idx);
+                    if (pc.q_boxes) {   // heads of a group in a power of two: 128 / G tokens by one copy per 64 columns (rows of others behind the last)
+                        if (lane == 0u) {
+                            mbar_arrive_expect_tx(q_full + 8u * g, L::Q);
+                            for (uint32_t a = 0; a < A; ++a)
+                                tma_load_3d(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)), &q_map, q_full + 8u * g, (int)(64u * a), (int)(p.group * pc.G),
+                                            (int)(p.q.tok0 + x.r0 / pc.G));
+                        }
+                        __syncwarp();
+                        continue;
                     }
-                    kr.advance();
-                }
-                bad_2 = bad_1;
-                bad_1 = t < T1 ? s_bad[(tiles + (t - T0)) & (kBadRing - 1u)] : 0u;
-            }
-            tiles += p.b - p.a;
-        }
-        if (__any_sync(0xffffffffu, ctl->abort != 0u)) {   // MMAs already issued finish before the CTA leaves
-            commit(drain + 8u * g);
-            for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain + 8u * g, 0u); ++spins) __nanosleep(64);
-        }
-    } else if (warp == L::QWARP) {
-        // Q rows into the K-major 128-byte swizzle, idle rows zero
-        uint32_t uses[2] = {0u, 0u};
-        while (ok && walk.next(pc, s_pref)) {
-            const Piece& p = walk.p;
-#pragma unroll 1
-            for (uint32_t g = 0; g < GROUPS; ++g) {
-                const Group x = group_of(pc, p, g);
-                if (x.t1 <= x.t0) continue;
-                const uint32_t n = g ? uses[1]++ : uses[0]++;
-                if (n) ok = wait_on(q_empty + 8u * g, (n - 1u) & 1u, ctl, pc.status, 0xDC0u);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (pc.q_boxes) {   // heads of a group in a power of two: 128 / G tokens by one copy per 64 columns (rows of others behind the last)
-                    if (lane == 0u) {
-                        mbar_arrive_expect_tx(q_full + 8u * g, L::Q);
-                        for (uint32_t a = 0; a < A; ++a)
-                            tma_load_3d(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)), &q_map, q_full + 8u * g, (int)(64u * a), (int)(p.group * pc.G),
-                                        (int)(p.q.tok0 + x.r0 / pc.G));
+                    constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
+                    const uint32_t c = lane % PIECES, at = smem_u32(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u));
+                    uint32_t r = lane / PIECES, token = (x.r0 + r) / pc.G, head = (x.r0 + r) % pc.G;
+                    const __half* q0 = pc.q + (uint64_t)p.q.tok0 * pc.q_s + (uint64_t)p.group * pc.G * D + 8u * c;
+    #pragma unroll 4
+                    for (uint32_t i = 0; i < kGroupRows / PER; ++i) {
+                        const uint32_t to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
+                        if (r < x.rows)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(q0 + (uint64_t)token * pc.q_s + head * D) : "memory");
+                        else
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0u) : "memory");
+                        r += PER;
+                        head += PER;
+                        while (head >= pc.G) {
+                            head -= pc.G;
+                            ++token;
+                        }
                     }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_smem();   // the MMAs read Q through the async proxy
                     __syncwarp();
-                    continue;
+                    if (lane == 0u) mbar_arrive(q_full + 8u * g);
                 }
-                constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
-                const uint32_t c = lane % PIECES, at = smem_u32(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u));
-                uint32_t r = lane / PIECES, token = (x.r0 + r) / pc.G, head = (x.r0 + r) % pc.G;
-                const __half* q0 = pc.q + (uint64_t)p.q.tok0 * pc.q_s + (uint64_t)p.group * pc.G * D + 8u * c;
-#pragma unroll 4
-                for (uint32_t i = 0; i < kGroupRows / PER; ++i) {
-                    const uint32_t to = at + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
-                    if (r < x.rows)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(q0 + (uint64_t)token * pc.q_s + head * D) : "memory");
-                    else
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0u) : "memory");
-                    r += PER;
-                    head += PER;
-                    while (head >= pc.G) {
-                        head -= pc.G;
-                        ++token;
-                    }
-                }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_async_smem();   // the MMAs read Q through the async proxy
-                __syncwarp();
-                if (lane == 0u) mbar_arrive(q_full + 8u * g);
             }
         }
-    }
     } else {
         if constexpr (!EXACT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, to = tmem + lanes + 2u * GROUPS * kTcKeys + g * D;

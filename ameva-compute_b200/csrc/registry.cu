@@ -142,8 +142,8 @@ static const KernelEntry kTable[] = {
     {"ameva_soft_max", 3, 80, {128, 1, 1}, launch_soft_max},
     {"ameva_flash_attn", 6, 124, {128, 1, 1}, launch_flash_attn},
     {"ameva_paged_append", 12, 100, {256, 1, 1}, launch_paged_append},
-    {"ameva_paged_attn", 9, 80, {288, 1, 1}, launch_paged_attn},
-    {"ameva_paged_prefix_attn", 10, 80, {288, 1, 1}, launch_paged_prefix_attn},
+    {"ameva_paged_attn", 9, 80, {384, 1, 1}, launch_paged_attn},
+    {"ameva_paged_prefix_attn", 10, 80, {384, 1, 1}, launch_paged_prefix_attn},
     {"ameva_cpy", 2, 76, {256, 1, 1}, launch_cpy},
     {"ameva_unary", 2, 60, {256, 1, 1}, launch_unary},
     {"bitnet_gemv_f16_w1", 3, 12, {32, 4, 1}, launch_gemv_f16},

@@ -81,27 +81,32 @@ class Setup:
         self.status = self.own(np.array([0, 0xFFFFFFFF], np.uint32))
         self.qb = self.own(self.q)
 
-    def attend(self, f16=False, scratch=None, softcap=0.0, window=0, scale=None, node=3):
+    def attend(self, f16=False, scratch=None, softcap=0.0, window=0, scale=None, node=3, wider=0):
+        """wider: elements between the rows of q and of the result beside their own."""
         dt = np.float16 if f16 else np.float32
-        sentinel = np.full((self.held, self.H, self.D), 77.0, dt)
-        dst = self.own(sentinel)
+        width = self.H * self.D + wider
+        dst, qb = self.own(np.full((self.held, width), 77.0, dt)), self.qb
+        if wider:
+            qb = self.own(np.concatenate([self.q.reshape(self.held, -1), np.full((self.held, wider), np.nan, np.float16)], axis=1))
         prefix = self.prefix is not None
         need = paged.scratch_bytes(self.ctx, self.seqs, heads=self.H, head_dim=self.D, prefix=prefix)
         sb = self.own(np.full((scratch or need) // 4, np.nan, np.float32))      # (its contents do not matter)
         batch = self.ctx.batch(4)
-        kw = dict(heads=self.H, scale=self.D ** -0.5 if scale is None else scale, softcap=softcap, f16_out=f16, node=node)
+        kw = dict(heads=self.H, scale=self.D ** -0.5 if scale is None else scale, softcap=softcap, f16_out=f16, node=node, q_stride=width, dst_stride=width)
         try:
             if prefix:
-                paged.record_prefix_attention(batch, self.cache, self.seqs, self.qb, dst, sb, self.status, prefix=self.own(self.prefix),
+                paged.record_prefix_attention(batch, self.cache, self.seqs, qb, dst, sb, self.status, prefix=self.own(self.prefix),
                                               max_prefix=int(self.prefix[0]), **kw)
             else:
-                paged.record_attention(batch, self.cache, self.seqs, self.qb, dst, sb, self.status, window=window, **kw)
+                paged.record_attention(batch, self.cache, self.seqs, qb, dst, sb, self.status, window=window, **kw)
             ev = batch.submit()
             ev.wait()
             ev.destroy()
         finally:
             batch.destroy()
-        return dst.read(dt).reshape(self.held, self.H, self.D)
+        got = dst.read(dt).reshape(self.held, width)
+        assert np.all(got[:, self.H * self.D:] == 77.0)
+        return got[:, :self.H * self.D].reshape(self.held, self.H, self.D)
 
     def want(self, **kw):
         kw.setdefault("scale", self.D ** -0.5)
@@ -129,7 +134,7 @@ class Setup:
 
 
 def both(s, **kw):
-    want = s.want(**kw)
+    want = s.want(**{name: x for name, x in kw.items() if name != "wider"})
     for f16 in (False, True):
         s.check(s.attend(f16=f16, **kw), want, f16)
     assert s.refused() == [0, 0xFFFFFFFF]
@@ -169,6 +174,113 @@ def test_shared_prefix(ctx, D, H, Hkv, page, layout, q, prefix):
     kv = [n + int(rng.integers(0, 70)) for n in q]
     kv[0] = q[0]
     both(Setup(ctx, q, kv, H, Hkv, D, page, layout, seed=prefix, pad=2, garbage=True, prefix=prefix))
+
+
+@pytest.mark.parametrize("D,H,Hkv", [(128, 40, 2), (64, 128, 1), (128, 65, 1), (64, 200, 1), (128, 18, 9), (64, 17, 17), (256, 12, 6), (256, 96, 1)])
+def test_groups_of_all_sizes(ctx, D, H, Hkv):
+    """Many query heads per KV head (more than 64: single tokens in the tensor-core kernel), KV heads that are no multiple of the warps."""
+    both(Setup(ctx, [1, 3, 1, 0, 40], [70, 300, 1, 9, 41], H, Hkv, D, 16, "token", seed=H, pad=1, garbage=True))
+
+
+@pytest.mark.parametrize("q,kv,page", [([1] * 500, [17] * 500, 16), ([1, 0, 2] * 1365, [5, 3, 2] * 1365, 16), ([70, 1, 90, 3] * 20, [75, 30, 90, 3] * 20, 32),
+                                       ([1, 2000, 5], [4000, 2500, 1025], 1024), ([1] * 3, [1023, 1024, 1025], 1024)])
+@pytest.mark.parametrize("prefix", [0, 77])
+def test_many_sequences_and_large_pages(ctx, q, kv, page, prefix):
+    """Up to the most sequences of a batch; prompts of many; pages of 1024 tokens."""
+    H = 2 if max(q) < 1000 else 1
+    both(Setup(ctx, q, kv, H, 1, 64, page, "head", seed=len(q), pad=1, prefix=prefix))
+
+
+@pytest.mark.parametrize("q,kv", [([1, 3, 5], [100, 40, 300]), ([90, 1, 200], [100, 40, 300])])
+@pytest.mark.parametrize("kw", [dict(scale=0.0), dict(scale=-0.1), dict(scale=-0.1, softcap=3.0), dict(wider=8), dict(wider=520, window=33)])
+def test_scales_and_strides(ctx, q, kv, kw):
+    both(Setup(ctx, q, kv, 8, 2, 128, 16, "token", seed=11, pad=2, garbage=True), **kw)
+    if "window" not in kw:
+        both(Setup(ctx, q, kv, 6, 2, 64, 16, "token", seed=12, pad=2, garbage=True, prefix=150), **kw)
+
+
+def test_announced_maxima_may_be_larger(ctx):
+    """Launches are sized by the announcement: the same results where it is wide of the mark, and none where nothing is to be done."""
+    both(Setup(ctx, [1, 1], [100, 40], 8, 2, 128, pad=200, max_q=150, max_kv=5000, stride=320))
+    both(Setup(ctx, [0, 0, 0], [100, 0, 40], 8, 2, 128, pad=200, max_q=150, max_kv=5000, stride=320))
+    both(Setup(ctx, [0, 0], [100, 40], 8, 2, 64, pad=3, prefix=33))
+
+
+@pytest.mark.parametrize("q,D", [(3, 128), (100, 128), (100, 64), (3, 256)])
+def test_keys_that_are_not_finite(ctx, q, D):
+    """A NaN in K at one key: rows that do not see it are what they were, rows that see it are NaN."""
+    kv = q + 60
+    s = Setup(ctx, [q], [kv], 4, 2, D)
+    at = kv - (q + 1) // 2
+    s.k[s.table[0, at // 16], at % 16, 1, 7] = np.nan
+    s.close()
+    s.buffers = []
+    s.upload()
+    with np.errstate(invalid="ignore"):
+        want = s.want()
+    for f16 in (False, True):
+        got = s.attend(f16=f16)
+        for j in range(q):
+            assert np.array_equal(np.isnan(want[j]), np.isnan(got[j])) and np.isnan(got[j, 2:]).all() == (kv - q + j >= at), (f16, j)
+            assert np.nanmax(np.abs(want[j] - got[j])) <= (TOL16 if f16 else TOL32)
+    s.close()
+
+
+@pytest.mark.parametrize("q,kv,H,D", [(1, 200000, 4, 128), (128, 40000, 1, 128), (70, 40000, 1, 64), (2, 60000, 2, 256)])
+def test_long_sums(ctx, q, kv, H, D):
+    """The error of a 32-bit result does not grow with the keys: sums leave the matrix instructions, which cut them instead of rounding, every
+    256 keys or earlier. In there at most 32 instructions add to one sum, each off by less than 2^-23 of what the sum has grown to, half its
+    end on the average: 32 * 2^-24 = 1.9e-6 at most for values of one sign. The n ordinary additions behind them are rounded, sqrt(n) 2^-24 of
+    random sign: 7e-7 for 40000 keys at the most. Left in one accumulator, 40000 keys would be off by 5000 * 2^-24 = 3e-4."""
+    s = Setup(ctx, [q], [kv], H, 1, D, 64)
+    s.v[:] = np.abs(s.v)      # (sums of one sign: the cuts add up)
+    s.close()
+    s.buffers = []
+    s.upload()
+    want, got = s.want(), s.attend()
+    y = np.stack([want[j] for j in range(q)])
+    assert np.linalg.norm(got - y) <= 2.6e-6 * np.linalg.norm(y)
+    s.close()
+
+
+def test_recorded_batches_share_a_scratch(ctx):
+    """Two graphs whose launches use the same scratch and status words, replayed in turn, and one batch with the same call twice."""
+    a = Setup(ctx, [1] * 7, [3000, 5, 17, 900, 2000, 64, 1], 8, 2, 128, seed=1, pad=1)
+    b = Setup(ctx, [200, 3], [900, 2000], 8, 2, 128, seed=2, pad=1)
+    size = max(paged.scratch_bytes(ctx, s.seqs, heads=8, head_dim=128) for s in (a, b))
+    scratch, made = ctx.buffer(size), []
+    for s, twice in ((a, False), (b, True)):
+        dst = [s.own(np.full((s.held, 8, 128), 77.0, np.float32)) for _ in range(1 + twice)]
+        batch = ctx.batch(4)
+        for d in dst:
+            paged.record_attention(batch, s.cache, s.seqs, s.qb, d, scratch, a.status, heads=8, scale=128 ** -0.5)
+        batch.instantiate()
+        made.append((s, dst, batch))
+    for _ in range(3):
+        events = [batch.replay() for _, _, batch in made]
+        for ev in events:
+            ev.wait()
+            ev.destroy()
+        for s, dst, _ in made:
+            got = [d.read(np.float32) for d in dst]
+            assert all(x.tobytes() == got[0].tobytes() for x in got)
+            s.check(got[0].reshape(s.held, 8, 128), s.want(), False)
+            for d in dst:
+                d.write(np.full((s.held, 8, 128), 77.0, np.float32))
+    assert a.refused() == [0, 0xFFFFFFFF]
+    for _, _, batch in made:
+        batch.destroy()
+    for s, _, _ in made:
+        s.close()
+    scratch.destroy()
+
+
+def test_a_sequence_that_does_not_fit_is_counted_once(ctx):
+    s = Setup(ctx, [1, 90, 2], [50, 90, 60], 4, 2, 128)      # both kernels run
+    s.seqs.kv_len.write(np.array([50, 90, 10 ** 6], np.int32))
+    got = s.attend()
+    assert s.refused() == [1, 3] and np.all(got[91:] == 77.0) and np.all(np.isfinite(got[:91]))
+    s.close()
 
 
 @pytest.mark.parametrize("q,kv,prefix", [([1] * 5, [3000, 1, 500, 2000, 77], 0), ([400, 1, 20], [900, 3000, 20], 0), ([1] * 30, [40] * 30, 3000)])
