@@ -39,12 +39,14 @@ constexpr float kGrowth = 7.0f;   // probabilities stay below 2^7
 template <int D, bool EXACT>
 struct Tc {
     static constexpr uint32_t GROUPS = EXACT ? 1 : 2, ROWS = GROUPS * kGroupRows;
-    static constexpr uint32_t MMA = 4 * GROUPS, LOAD = MMA + GROUPS, QWARP = LOAD + 1, THREADS = EXACT ? 256 : 384;   // warps by role
+    static constexpr uint32_t PARTS = EXACT ? 2 : 1, KEYS = kTcKeys / PARTS, COLS = D / PARTS;   // threads of a row; a thread's share of keys and columns
+    static constexpr uint32_t MMA = 8, LOAD = MMA + GROUPS, QWARP = LOAD + 1, THREADS = 384;      // warps by role
     static constexpr uint32_t TMEM = EXACT && D == 64 ? 256 : 512;
-    static constexpr uint32_t A = D / 64, STAGES = EXACT || D == 64 ? 5 : 3;
+    static constexpr uint32_t A = D / 64, STAGES = D == 64 ? 5 : EXACT ? 4 : 3;
     static constexpr uint32_t Q = A * kGroupRows * 128u, TILE = A * kTcKeys * 128u;
-    static constexpr uint32_t STAGE_OUT = GROUPS * 4u * 32u * 64u;   // a warp's 32 rows x 16 columns on their way out
-    static constexpr uint32_t FIXED = 1024u + GROUPS * Q + 2u * STAGES * TILE + STAGE_OUT + 512u;
+    static constexpr uint32_t STAGE_OUT = MMA * 32u * 64u;   // a warp's 32 rows x 16 columns on their way out
+    static constexpr uint32_t PAIRS = EXACT ? 2u * 2u * kGroupRows * 8u : 0u;   // what the threads of a row tell one another
+    static constexpr uint32_t FIXED = 1024u + GROUPS * Q + 2u * STAGES * TILE + STAGE_OUT + PAIRS + 512u;
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
 constexpr uint32_t kFlush = 4;   // EXACT: key tiles that an accumulator takes before it is added to the row's sum
@@ -234,7 +236,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t *sQ = base, *sK = sQ + GROUPS * L::Q, *sV = sK + ST * L::TILE;
     uint8_t* s_out = sV + ST * L::TILE;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + L::STAGE_OUT);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_out + L::STAGE_OUT + L::PAIRS);
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST,
                    q_full = v_empty + 8u * ST, q_empty = q_full + 16u, s_full = q_empty + 16u, p_full = s_full + 32u, pv_done = p_full + 32u,
                    drain = pv_done + 32u;   // the last three: [group][tile & 1]
@@ -255,7 +257,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             mbar_init(q_empty + 8u * g, 1u);
             for (uint32_t b = 0; b < 2u; ++b) {
                 mbar_init(s_full + 16u * g + 8u * b, 1u);
-                mbar_init(p_full + 16u * g + 8u * b, 4u);
+                mbar_init(p_full + 16u * g + 8u * b, 4u * L::PARTS);
                 mbar_init(pv_done + 16u * g + 8u * b, 1u);   // two of them: a wait for tile j - 1's meets it at most one phase behind
             }
         }
@@ -280,7 +282,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     bool ok = true;
 
     if (warp >= L::MMA) {
-        if constexpr (!EXACT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == L::LOAD) {
             Ring kr(ST), vr(ST);
             uint32_t tiles = 0;     // of this CTA so far
@@ -509,25 +511,41 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             }
         }
     } else {
-        if constexpr (!EXACT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        const uint32_t g = warp >> 2, lanes = ((warp & 3u) * 32u) << 16, to = tmem + lanes + 2u * GROUPS * kTcKeys + g * D;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        constexpr uint32_t KEYS = L::KEYS, COLS = L::COLS;
+        const uint32_t g = EXACT ? 0u : warp >> 2, part = EXACT ? warp >> 2 : 0u, my = threadIdx.x & 127u;
+        const uint32_t lanes = ((warp & 3u) * 32u) << 16, to = tmem + lanes + 2u * GROUPS * kTcKeys + g * D + part * COLS;
+        // EXACT: the two threads of a row tell one another a value and whether all is well, so that both leave together. Two places in
+        // turn: a warp writes to one again behind the next barrier, which the other one passes after it has read.
+        float2* s_pair = reinterpret_cast<float2*>(s_out + L::STAGE_OUT);
+        uint32_t told = 0;
+        auto tell = [&](float v, bool& fine) {
+            s_pair[((told & 1u) * 2u + part) * kGroupRows + my] = make_float2(v, fine ? 1.0f : 0.0f);
+            tc_fence_before();
+            asm volatile("bar.sync %0, 64;" ::"r"(1u + (warp & 3u)) : "memory");
+            tc_fence_after();
+            const float2 y = s_pair[((told & 1u) * 2u + (part ^ 1u)) * kGroupRows + my];
+            ++told;
+            fine = __all_sync(0xffffffffu, fine && y.y != 0.0f);
+            return y.x;
+        };
         uint32_t j = 0, tiles = 0;   // key tiles of this group, of the CTA, so far
         bool cut = false;
         while (walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
             const Group x = group_of(pc, p, g);
-            const uint32_t my = threadIdx.x & 127u, row = x.r0 + my;
+            const uint32_t row = x.r0 + my;
             const bool valid = my < x.rows;
             const Span span = valid ? row_span(pc, p.q, row) : Span{0u, 0u};
             float m_run = neg_inf(), l_run = 0.0f;
-            float sum_o[EXACT ? D : 1];   // EXACT: the row's sum; the accumulators hold the last tiles
+            float sum_o[EXACT ? COLS : 1];   // EXACT: the row's sum; the accumulators hold the last tiles
             if (EXACT) {
 #pragma unroll
-                for (uint32_t c = 0; c < (uint32_t)D; ++c) sum_o[c] = 0.0f;
+                for (uint32_t c = 0; c < COLS; ++c) sum_o[c] = 0.0f;
             }
             auto add_up = [&](uint32_t acc) {
 #pragma unroll
-                for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
+                for (uint32_t c = 0; c < COLS; c += 32u) {
                     uint32_t v[32];
                     tmem_ld32_async(to + acc * (uint32_t)D + c, v);
                     tmem_wait_ld();
@@ -539,25 +557,26 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 const uint32_t key0 = t * kTcKeys, b = j & 1u, ts = tmem + lanes + (2u * g + b) * kTcKeys;
                 ok = ok && wait_on(s_full + 16u * g + 8u * b, (j >> 1) & 1u, ctl, pc.status, 0xDA0u);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (!EXACT && !ok) break;
                 tc_fence_after();
                 const uint32_t gone = s_bad[(tiles + (t - p.first - p.a)) & (kBadRing - 1u)];
-                float s[kTcKeys];
+                float s[KEYS];
 #pragma unroll
-                for (uint32_t c = 0; c < kTcKeys; c += 32u) tmem_ld32_async(ts + c, reinterpret_cast<uint32_t*>(s) + c);
+                for (uint32_t c = 0; c < KEYS; c += 32u) tmem_ld32_async(ts + part * KEYS + c, reinterpret_cast<uint32_t*>(s) + c);
                 tmem_wait_ld();
                 // the same for every thread of the group
                 const bool open = gone == 0u && key0 >= x.lo_all && key0 + kTcKeys <= x.hi_all, scaled = pc.softcap == 0.0f && pc.scale2 > 0.0f;
                 if (!scaled) {   // the cap, or a scale that is not positive
 #pragma unroll
-                    for (uint32_t k = 0; k < kTcKeys; ++k) s[k] = capped(pc, s[k]);
+                    for (uint32_t k = 0; k < KEYS; ++k) s[k] = capped(pc, s[k]);
                 }
                 if (!open) {     // hidden keys: a bit per key of 32
 #pragma unroll
-                    for (uint32_t c = 0; c < kTcKeys; c += 32u) {
-                        const uint32_t a = span.lo > key0 + c ? min(span.lo - key0 - c, 32u) : 0u, e = span.hi > key0 + c ? min(span.hi - key0 - c, 32u) : 0u;
+                    for (uint32_t c = 0; c < KEYS; c += 32u) {
+                        const uint32_t at = part * KEYS + c, first = key0 + at;
+                        const uint32_t a = span.lo > first ? min(span.lo - first, 32u) : 0u, e = span.hi > first ? min(span.hi - first, 32u) : 0u;
                         const uint32_t below = e >= 32u ? 0xffffffffu : (1u << e) - 1u, from = a >= 32u ? 0u : 0xffffffffu << a;
-                        const uint32_t there = ((gone >> (c >> 4) & 1u) ? 0u : 0xffffu) | ((gone >> ((c >> 4) + 1u) & 1u) ? 0u : 0xffff0000u);
+                        const uint32_t there = ((gone >> (at >> 4) & 1u) ? 0u : 0xffffu) | ((gone >> ((at >> 4) + 1u) & 1u) ? 0u : 0xffff0000u);
                         const uint32_t seen = below & from & there;
 #pragma unroll
                         for (uint32_t k = 0; k < 32u; ++k) s[c + k] = seen >> k & 1u ? s[c + k] : neg_inf();
@@ -567,8 +586,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
 #pragma unroll
                 for (uint32_t k = 0; k < 4u; ++k) m4[k] = fmaxf(s[2u * k], s[2u * k + 1u]);
 #pragma unroll
-                for (uint32_t k = 8u; k < kTcKeys; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
-                const float mul = scaled ? pc.scale2 : 1.0f, mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * mul;
+                for (uint32_t k = 8u; k < KEYS; k += 2u) m4[(k >> 1) & 3u] = max3(m4[(k >> 1) & 3u], s[k], s[k + 1u]);
+                const float mul = scaled ? pc.scale2 : 1.0f;
+                float mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * mul;
+                if (EXACT) {   // (both warps of the rows have read their scores behind this, and write P over them)
+                    mx = fmaxf(mx, tell(mx, ok));
+                    if (!ok) break;
+                }
                 // The accumulator that tile t - 2 completed is added up now: its P V is done, since S of this tile was issued behind it.
                 if (EXACT && t - x.t0 > kFlush && (t - x.t0) % kFlush == 1u) add_up((t - 2u - x.t0) / kFlush & 1u);
                 const bool grow = mx > m_run + kGrowth || (m_run == neg_inf() && mx != neg_inf());
@@ -578,16 +602,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     l_run *= f;
                     if (EXACT) {
 #pragma unroll
-                        for (uint32_t c = 0; c < (uint32_t)D; ++c) sum_o[EXACT ? c : 0u] *= f;
+                        for (uint32_t c = 0; c < COLS; ++c) sum_o[EXACT ? c : 0u] *= f;
                     }
                     if (t != x.t0) {
                         const uint32_t last = to + (EXACT ? ((t - 1u - x.t0) / kFlush & 1u) * (uint32_t)D : 0u);   // what tile t - 1 went to
                         ok = wait_on(pv_done + 16u * g + 8u * (b ^ 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDC8u);
                         ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
+                        if (!EXACT && !ok) break;
                         tc_fence_after();
 #pragma unroll 1
-                        for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
+                        for (uint32_t c = 0; c < COLS; c += 16u) {
                             uint32_t v[16];
                             tmem_ld16(last + c, v);
 #pragma unroll
@@ -600,23 +624,23 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 const uint64_t mul_2 = pack2(mul, mul), ref2 = pack2(-ref, -ref);
                 uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-                for (uint32_t part = 0; part < 2u; ++part) {
+                for (uint32_t h = 0; h < KEYS / 32u; ++h) {
                     uint32_t ph[16], pl[16];
 #pragma unroll
                     for (uint32_t k = 0; k < 16u; ++k) {
-                        const float2 e = unpack2(fma2(pack2(s[32u * part + 2u * k], s[32u * part + 2u * k + 1u]), mul_2, ref2));
+                        const float2 e = unpack2(fma2(pack2(s[32u * h + 2u * k], s[32u * h + 2u * k + 1u]), mul_2, ref2));
                         const float p0 = ex2(e.x), p1 = ex2(e.y);
                         sum2[k & 1u] = add2(sum2[k & 1u], pack2(p0, p1));
-                        const __half2 h = __floats2half2_rn(p0, p1);
-                        ph[k] = *reinterpret_cast<const uint32_t*>(&h);
+                        const __half2 hi = __floats2half2_rn(p0, p1);
+                        ph[k] = *reinterpret_cast<const uint32_t*>(&hi);
                         if (EXACT) {
-                            const float2 f2 = __half22float2(h);
+                            const float2 f2 = __half22float2(hi);
                             const __half2 low = __floats2half2_rn(p0 - f2.x, p1 - f2.y);
                             pl[k] = *reinterpret_cast<const uint32_t*>(&low);
                         }
                     }
-                    tmem_st16_async(ts + 16u * part, ph);   // over this tile's scores
-                    if (EXACT) tmem_st16_async(ts + 32u + 16u * part, pl);
+                    tmem_st16_async(ts + 16u * (part + h), ph);   // over this tile's scores
+                    if (EXACT) tmem_st16_async(ts + 32u + 16u * (part + h), pl);
                 }
                 const float2 sums = unpack2(add2(sum2[0], sum2[1]));
                 l_run += sums.x + sums.y;
@@ -629,6 +653,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const bool some = x.t1 > x.t0, whole = p.a == 0u && p.b == p.n;
             if (some) ok = ok && wait_on(pv_done + 16u * g + 8u * ((j - 1u) & 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDB0u) && !ctl->abort;
             ok = __all_sync(0xffffffffu, ok);
+            if (EXACT) l_run += tell(l_run, ok);
             if (!ok) break;
             tc_fence_after();
             tiles += p.b - p.a;
@@ -645,8 +670,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 if (valid) {
                     if (parts) {
                         float* r = whole ? reinterpret_cast<float*>(pc.dst) + dst_row(pc, token, head, D) : slot + (uint64_t)my * (D + 4u);
-                        *reinterpret_cast<float2*>(r) = make_float2(m_run, l_run);
-                        dst = r + 4;
+                        if (part == 0u) *reinterpret_cast<float2*>(r) = make_float2(m_run, l_run);
+                        dst = r + 4u + part * COLS;
                     } else {
                         float l = l_run, f = 1.0f;
                         if (pc.extra) {
@@ -661,7 +686,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                         own = f * inv;
                         other *= inv;
-                        const uint64_t e = dst_row(pc, token, head, D);
+                        const uint64_t e = dst_row(pc, token, head, D) + part * COLS;
                         dst = pc.out == OUT_F16 ? (void*)(reinterpret_cast<__half*>(pc.dst) + e) : (void*)(reinterpret_cast<float*>(pc.dst) + e);
                     }
                 }
@@ -680,8 +705,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     row_other[i] = __shfl_sync(0xffffffffu, other, 8u * i + sub);
                 }
                 const bool f16 = !parts && pc.out == OUT_F16;
-#pragma unroll(EXACT ? D / 16 : 1)
-                for (uint32_t c = 0; c < (uint32_t)D; c += 16u) {
+#pragma unroll(EXACT ? COLS / 16 : 1)
+                for (uint32_t c = 0; c < COLS; c += 16u) {
                     uint32_t v[16];
                     if (some) tmem_ld16(to_last + c, v);
 #pragma unroll
@@ -706,7 +731,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                      : "r"(mine + r * 64u + ((piece ^ ((r >> 1) & 3u)) << 4))
                                      : "memory");
                         if (row_extra[i]) {
-                            const float4 e = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row_extra[i]) + 4u + c + 4u * piece);
+                            const float4 e = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row_extra[i]) + 4u + part * COLS + c + 4u * piece);
                             y.x = fmaf(e.x, row_other[i], y.x);
                             y.y = fmaf(e.y, row_other[i], y.y);
                             y.z = fmaf(e.z, row_other[i], y.z);
@@ -722,8 +747,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     }
                     __syncwarp();
                 }
+                if (EXACT) check += tell(check, ok);   // (what the other warp has written of the rows is there)
                 // rows that are not finite although their sum is: over the keys they see, by the whole warp
-                for (uint32_t again = __ballot_sync(0xffffffffu, valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
+                for (uint32_t again = __ballot_sync(0xffffffffu, part == 0u && valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
                     const int i = __ffs(again) - 1;
                     const uint32_t r = x.r0 + (warp & 3u) * 32u + (uint32_t)i, tk = p.q.tok0 + r / pc.G, hd = p.group * pc.G + r % pc.G;
                     const float m = __shfl_sync(0xffffffffu, m_run, i), l = __shfl_sync(0xffffffffu, l_run, i);
