@@ -43,7 +43,7 @@ struct Args {
     uint32_t* status;           // the context's
     uint32_t max_own_q, max_own_kv;   // prefix launch: the maxima of the sequences
     uint32_t n_seqs, rows, max_q, max_kv, page_log2, n_pages, table_stride;
-    uint32_t n_head, n_head_kv, G;
+    uint32_t n_head, n_head_kv, G, g_mul, g_shift;   // x / G = x * g_mul >> g_shift for x < 2^31
     uint32_t c_ps, c_ts, c_hs;  // cache strides in elements: page, token, head
     uint32_t q_s, dst_s, out, node, window, min_rows, max_rows;   // a launch serves the sequences of min_rows .. max_rows rows
     float scale, softcap, scale2, cap_in, cap_out;                // scale2: scale * log2(e); 2 log2(e) scale / softcap, softcap * log2(e)
@@ -80,13 +80,17 @@ __device__ __forceinline__ Seq load_seq(const Args& pc, uint32_t s, bool report 
     return x;
 }
 
+// r / G without a division's instructions, which a CTA runs once and has to fetch: g_mul = ceil(2^g_shift / G) and g_shift = 31 + ceil(log2 G)
+// are off by less than 2^31 in r * g_mul, so that no quotient of r < 2^31 moves.
+__device__ __forceinline__ uint32_t query_of(const Args& pc, uint32_t r) { return (uint32_t)((uint64_t)r * pc.g_mul >> pc.g_shift); }
+
 // The keys that row r sees: [lo, hi)
 struct Span {
     uint32_t lo, hi;
 };
 __device__ __forceinline__ Span row_span(const Args& pc, const Seq& q, uint32_t r) {
     if (pc.prefix) return {0u, q.kv};
-    const int32_t end = (int32_t)q.kv - (int32_t)q.n_q + (int32_t)(r / pc.G) + 1;   // one past its own place
+    const int32_t end = (int32_t)q.kv - (int32_t)q.n_q + (int32_t)query_of(pc, r) + 1;   // one past its own place
     if (end <= 0) return {0u, 0u};
     const uint32_t hi = (uint32_t)end;
     return {pc.window && hi > pc.window ? hi - pc.window : 0u, hi};
@@ -189,8 +193,9 @@ __device__ __forceinline__ Stretch my_stretch(uint32_t total) {
     x.ctas = min(gridDim.x, total);
     x.begin = x.end = 0u;
     if (blockIdx.x < x.ctas) {
-        x.begin = (uint32_t)((uint64_t)blockIdx.x * total / x.ctas);
-        x.end = (uint32_t)((uint64_t)(blockIdx.x + 1u) * total / x.ctas);
+        const uint32_t q = total / x.ctas, r = total - q * x.ctas;   // floor(c total / ctas) in 32 bits
+        x.begin = blockIdx.x * q + blockIdx.x * r / x.ctas;
+        x.end = (blockIdx.x + 1u) * q + (blockIdx.x + 1u) * r / x.ctas;
     }
     return x;
 }
@@ -223,14 +228,21 @@ struct Walk {
                 p.q = load_seq(pc, lo);
                 p.R = p.q.n_q * pc.G;
             }
-            const uint32_t at = t - s_pref[seq], per_group = (s_pref[seq + 1u] - s_pref[seq]) / pc.groups;
-            p.group = at / per_group;
-            uint32_t rem = at - p.group * per_group;
+            uint32_t rem = t - s_pref[seq];
+            p.group = 0u;
+            if (pc.groups > 1u) {
+                const uint32_t per_group = (s_pref[seq + 1u] - s_pref[seq]) / pc.groups;
+                p.group = rem / per_group;
+                rem -= p.group * per_group;
+            }
             if (pc.prefix || p.R <= ROWS) {   // row tiles with the same number of key tiles, or a single one
                 tile_range(pc, p.q, 0u, p.R <= ROWS ? p.R - 1u : 0u, p.first, p.n);
-                const uint32_t i = rem / (p.n + pc.over);
-                p.r0 = i * ROWS;
-                rem -= i * (p.n + pc.over);
+                p.r0 = 0u;
+                if (p.R > ROWS) {
+                    const uint32_t i = rem / (p.n + pc.over);
+                    p.r0 = i * ROWS;
+                    rem -= i * (p.n + pc.over);
+                }
             } else {                          // counted 32 at a time
                 const uint32_t lane = threadIdx.x & 31u;
                 for (uint32_t base = 0;; base += 32u * ROWS) {

@@ -207,8 +207,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             const uint32_t r = p.r0 + g + 8u * h;
             valid[h] = mine && g + 8u * h < rows;
             span[h] = valid[h] ? row_span(pc, p.q, r) : Span{0u, 0u};
-            token[h] = p.q.tok0 + (valid[h] ? r / pc.G : 0u);
-            head[h] = valid[h] ? hkv * pc.G + r % pc.G : 0u;
+            const uint32_t query = query_of(pc, r);
+            token[h] = p.q.tok0 + (valid[h] ? query : 0u);
+            head[h] = valid[h] ? hkv * pc.G + r - query * pc.G : 0u;
             const __half* qrow = pc.q + (uint64_t)token[h] * pc.q_s + (uint64_t)head[h] * D;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -395,7 +396,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                 }
                 for (uint32_t bad = __ballot_sync(0xffffffffu, again && t4 == 0u); bad; bad &= bad - 1u) {   // by the whole warp
                     const int from = __ffs(bad) - 1;
-                    const uint32_t r = p.r0 + (uint32_t)from / 4u + 8u * h, tk = p.q.tok0 + r / pc.G, hd = hkv * pc.G + r % pc.G;
+                    const uint32_t r = p.r0 + (uint32_t)from / 4u + 8u * h, query = query_of(pc, r), tk = p.q.tok0 + query, hd = hkv * pc.G + r - query * pc.G;
                     const float m = __shfl_sync(0xffffffffu, m_run[h], from), l = __shfl_sync(0xffffffffu, l_run[h], from);
                     const Span s = row_span(pc, p.q, r);
                     float o[C];
@@ -570,8 +571,8 @@ __device__ __forceinline__ void merge_set(const MergeSet& set) {
             if (begin != 0u) continue;
         }
         if (have_row) {
-            const uint32_t row = note.z + r;
-            finish_row<C>(pc, note.y + row / pc.G, (group * pc.HB + hb) * pc.G + row % pc.G, m, l, o);
+            const uint32_t row = note.z + r, query = query_of(pc, row);
+            finish_row<C>(pc, note.y + query, (group * pc.HB + hb) * pc.G + row - query * pc.G, m, l, o);
         }
     }
     __syncthreads();   // (the memory is used again)
@@ -662,6 +663,8 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
         !pc.n_pages || !pc.table_stride || pc.out > OUT_F16 || !(pc.softcap >= 0.0f) || pc.scale != pc.scale)
         return AC_ERR_KERNEL_ARG_INVALID;
     pc.G = pc.n_head / pc.n_head_kv;
+    for (pc.g_shift = 31u; (1ull << (pc.g_shift - 31u)) < pc.G; ++pc.g_shift) {}
+    pc.g_mul = (uint32_t)(((1ull << pc.g_shift) + pc.G - 1u) / pc.G);
     if ((D != 64u && D != 128u && D != 256u) || P < 16u || P > 1024u) return AC_ERR_FEATURE_NOT_SUPPORTED;
     for (pc.page_log2 = 0; (1u << pc.page_log2) < P; ++pc.page_log2) {}
     if (pc.n_seqs > kMaxSeqs || pc.n_head > 65535u || pc.rows > 0x7FFFFFFFu || pc.max_kv > 0x7FFFFFFFu - 1024u || pc.n_pages > 0x7FFFFFFFu ||

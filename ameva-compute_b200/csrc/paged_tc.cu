@@ -480,14 +480,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                             mbar_arrive_expect_tx(q_full + 8u * g, L::Q);
                             for (uint32_t a = 0; a < A; ++a)
                                 tma_load_3d(smem_u32(sQ + g * L::Q + a * (kGroupRows * 128u)), &q_map, q_full + 8u * g, (int)(64u * a), (int)(p.group * pc.G),
-                                            (int)(p.q.tok0 + x.r0 / pc.G));
+                                            (int)(p.q.tok0 + query_of(pc, x.r0)));
                         }
                         __syncwarp();
                         continue;
                     }
                     constexpr uint32_t PIECES = D / 8, PER = 32u / PIECES;   // 16-byte pieces of a row; rows per load of a warp
                     const uint32_t c = lane % PIECES, at = smem_u32(sQ + g * L::Q + (c >> 3) * (kGroupRows * 128u));
-                    uint32_t r = lane / PIECES, token = (x.r0 + r) / pc.G, head = (x.r0 + r) % pc.G;
+                    uint32_t r = lane / PIECES, token = query_of(pc, x.r0 + r), head = x.r0 + r - token * pc.G;
                     const __half* q0 = pc.q + (uint64_t)p.q.tok0 * pc.q_s + (uint64_t)p.group * pc.G * D + 8u * c;
     #pragma unroll 4
                     for (uint32_t i = 0; i < kGroupRows / PER; ++i) {
@@ -661,7 +661,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const uint32_t n_tiles = x.t1 - x.t0, to_last = to + (EXACT && some ? ((n_tiles - 1u) / kFlush & 1u) * (uint32_t)D : 0u);
             if (EXACT && some && n_tiles > 1u && (n_tiles - 1u) % kFlush == 0u) add_up((n_tiles - 2u) / kFlush & 1u);
             if (x.rows) {
-                const uint32_t token = p.q.tok0 + row / pc.G, head = p.group * pc.G + row % pc.G;
+                const uint32_t query = query_of(pc, row), token = p.q.tok0 + query, head = p.group * pc.G + row - query * pc.G;
                 float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * L::ROWS + (x.r0 - p.r0)) * (D + 4u);
                 const bool parts = !whole || pc.out == OUT_PARTS;
                 float own = 1.0f, other = 0.0f;      // factors of the values here and of those over other keys
@@ -751,7 +751,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 // rows that are not finite although their sum is: over the keys they see, by the whole warp
                 for (uint32_t again = __ballot_sync(0xffffffffu, part == 0u && valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
                     const int i = __ffs(again) - 1;
-                    const uint32_t r = x.r0 + (warp & 3u) * 32u + (uint32_t)i, tk = p.q.tok0 + r / pc.G, hd = p.group * pc.G + r % pc.G;
+                    const uint32_t r = x.r0 + (warp & 3u) * 32u + (uint32_t)i, q_r = query_of(pc, r), tk = p.q.tok0 + q_r, hd = p.group * pc.G + r - q_r * pc.G;
                     const float m = __shfl_sync(0xffffffffu, m_run, i), l = __shfl_sync(0xffffffffu, l_run, i);
                     const Span sp = row_span(pc, p.q, r);
                     float o[C];
