@@ -14,6 +14,8 @@
 // probability would show in an f32 result, and makes an f16 one's error 1.25 times what its own rounding is; the second product costs 2 %
 // of the time above), and the matrix instruction's sums, which are cut rather than rounded, are added up per 32 keys by ordinary
 // additions: left in its accumulator from the first key to the last, 131072 keys are off by 2.3e-6 instead of 4e-7.
+// Bound by HBM, short calls by the instructions that a CTA fetches for the first time: those 96 sequences 119 us (659 MB, 5.5 TB/s; the copy
+// reaches 6.55), one of 131072 keys 103 us (537 MB, 5.2 TB/s), one of 500 keys 18 us (this kernel 8, the merge 5).
 #include <cstring>
 #include <type_traits>
 
@@ -423,7 +425,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 
 // Joins the cut row tiles. CTA x of the kernel in front notes a row tile that it begins and others end; its parts lie in slot 2 x + 1 and
 // in slots 2 y of the CTAs behind. The rows of a kernel's notes form one list that the warps of the grid share;
-// SHARE warps take the parts of a row in turn, the more the more parts there are.
+// `share` warps take the parts of a row in turn, the more the more parts there are (a long sequence alone has one per SM). Bound by latency:
+// 5 us for the 32 rows of one token, 16 us for 24 mixed sequences of 535 tokens.
 constexpr uint32_t kMergeWarps = 16, kMergeNotes = 512;
 struct MergeSet {
     Args pc;
@@ -698,10 +701,25 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
     return AC_SUCCESS;
 }
 
-// Which kernel a sequence of R rows per KV head runs in: up to kFewRows in paged_rows_kernel, more in paged_tc.cu's (D 64, 128).
-constexpr uint32_t kFewRows = 64;
-// What a row tile costs beside its key tiles, in key tiles (the line's allowance).
-constexpr uint32_t kFewOver = 1, kManyOver = 2;
+// Which kernel a sequence of R rows per KV head runs in (D 64, 128; D 256 knows one): paged_rows_kernel reads the keys once per 16 rows, the
+// kernel in paged_tc.cu takes the same time for 1 .. 128, but is one more launch where sequences of few rows are beside it. 8 sequences
+// of 4000 keys, 8 KV heads, f16 results, a pass in us, rows / tensor-core kernel: 32 rows 62 / 68, 64 rows 97 / 67, 128 rows 159 / 72;
+// 64 of 2000 keys: 191 / 165, 340 / 168, 620 / 178 (32-bit results: 192 / 185, 343 / 191, 620 / 203). 32 sequences of 7 to 42 rows, 2 KV
+// heads, 1024 keys: 21 / 46. So up to kFewRows; up to kFewRowsAlone while what the rows beyond add is below what the other launch costs:
+// 25 us, in which 360 thousand (row tile, KV head, key) are served.
+constexpr uint32_t kFewRows = 32, kFewRowsAlone = 64;
+constexpr uint64_t kLaunchWork = 360000;
+static uint32_t few_rows_of(const Args& pc, uint32_t D, uint64_t max_rows) {
+    if (D > 128u) return 0xFFFFFFFFu;
+    if (max_rows > kFewRowsAlone) return kFewRows;
+    const uint64_t keys = pc.window && (uint64_t)pc.window + pc.max_q < pc.max_kv ? (uint64_t)pc.window + pc.max_q : pc.max_kv;
+    const uint64_t beyond = max_rows > kFewRows ? (max_rows - kFewRows + kDecRows - 1u) / kDecRows : 0u;
+    return (pc.prefix ? 1u : pc.n_seqs) * keys * pc.n_head_kv * beyond > kLaunchWork ? kFewRows : kFewRowsAlone;
+}
+// What a row tile costs beside its key tiles, in key tiles (the line's allowance): Q and the first scores on their way, results written.
+// us with none / this: 96 sequences of 20 .. 8192 keys 126 / 119 (1: 121), 32 drafted ones 24.1 / 22.1 (1: 21.5); a prompt of 8192 737 / 648
+// (2: 700, 4: 665, 10: 653, 16: 664), 64 rows behind a prefix of 8192 keys 83.9 / 73.4.
+constexpr uint32_t kFewOver = 2, kManyOver = 6;
 // KV heads that paged_rows_kernel takes at once: all of them where its warps suffice, otherwise equal groups
 static uint32_t few_heads(uint32_t D, uint32_t n_head_kv) {
     const uint32_t W = D == 256u ? 4u : 8u, groups = (n_head_kv + W - 1u) / W;
@@ -733,11 +751,12 @@ struct Plan {
     uint32_t tc_rows;
 };
 static AcResult plan_set(const Args& pc, uint32_t D, uint64_t max_rows, Plan& x) {
-    const bool both = D <= 128u && max_rows > kFewRows;
+    const uint32_t few_max = few_rows_of(pc, D, max_rows);
+    const bool both = max_rows > few_max;
     x.few = x.many = pc;
     x.few.min_rows = 1u;
-    x.few.max_rows = both ? kFewRows : 0xFFFFFFFFu;
-    x.many.min_rows = pc.prefix ? 1u : kFewRows + 1u;   // (a prefix has one number of rows, and one kernel)
+    x.few.max_rows = both ? few_max : 0xFFFFFFFFu;
+    x.many.min_rows = pc.prefix ? 1u : few_max + 1u;   // (a prefix has one number of rows, and one kernel)
     x.many.max_rows = 0xFFFFFFFFu;
     x.use_few = !both || !pc.prefix;
     x.use_many = both;
@@ -754,7 +773,7 @@ static AcResult plan_set(const Args& pc, uint32_t D, uint64_t max_rows, Plan& x)
     x.many.over = kManyOver;
     x.tc_rows = pc.out == OUT_F16 ? kTcRows : kTcRows / 2u;   // (paged_tc.cu)
     // the line's length in 32 bits
-    const uint64_t few_rows = both ? kFewRows : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs;
+    const uint64_t few_rows = both ? few_max : max_rows, seqs = pc.prefix ? 1u : pc.n_seqs;
     auto too_long = [&](const Args& y, uint64_t row_tiles) {
         return seqs * y.groups * row_tiles * (((uint64_t)pc.max_kv >> y.keys_log2) + 2u + y.over) > 0xFFFFFFFFull;
     };
@@ -797,6 +816,7 @@ static AcResult cache_maps(const LaunchArgs& a, const Args& pc, uint32_t D, Maps
                     encode_cache(enc, &tc_maps.k, a.ptr[1], pc, D, tc_box, 1u) && encode_cache(enc, &tc_maps.v, a.ptr[2], pc, D, tc_box, 1u);
     if (!ok) return AC_ERR_INVALID_SHAPE;
     memset(&tc_maps.q, 0, sizeof(tc_maps.q));
+    // Q by TMA where whole tokens fill a group's 128 rows; otherwise by cp.async, 16 bytes a lane (a prompt of 8192, G = 4: 700 / 739 us)
     tc_maps.q_boxes = D <= 128u && (pc.G & (pc.G - 1u)) == 0u && pc.G <= 128u;
     if (tc_maps.q_boxes) {
         const cuuint64_t dims[3] = {D, pc.n_head, pc.rows}, strides[2] = {2ull * D, 2ull * (pc.rows > 1u ? pc.q_s : (uint64_t)pc.n_head * D)};

@@ -1,8 +1,8 @@
 // Attention over a paged KV cache for many rows per sequence (prompts, the shared prefix of a batch; D 64, 128) on the 5th-generation
 // tensor cores. Arguments, rows and the line of work: paged.cuh; launchers: paged_attn.cu.
 //
-// A CTA (one per SM) takes row tiles of 256 rows, two groups of 128 (f16 results; one group for 32-bit ones, EXACT, with the warps behind
-// the first four moved up), and walks key tiles of 64 for both:
+// A CTA (one per SM) takes row tiles of 256 rows, two groups of 128, and walks key tiles of 64 for both (f16 results; for 32-bit ones, EXACT,
+// below, one group of 128 rows):
 //   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 64 scores from tensor memory, online softmax to base 2, write P
 //                    over the scores as f16 (and, for a 32-bit result, what that rounding left beside it). The accumulator is rescaled
 //                    only when a row's maximum has grown by more than 2^kGrowth since its last rescale. They write the piece's results.
@@ -15,9 +15,14 @@
 //   warp 11          brings the Q rows in, those of the next piece as soon as the last S of this one has read them
 // Tensor memory: four S / P tiles of 64 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
 // steps of 16 keys that none sees; V rows behind the last key are zeroed before they are multiplied (a page holds anything there).
-// The tensor core's sums are cut rather than rounded, which an f16 result does not show and a 32-bit one would (2.2e-6 after 300 of them, in
-// proportion to their number): for those two accumulators take kFlush tiles each in turn and are added to a sum in registers, which takes
-// the registers of a second group's softmax.
+// EXACT. The tensor core's sums are cut rather than rounded, which an f16 result does not show and a 32-bit one would (2.2e-6 after 300 of
+// them, in proportion to their number): two accumulators take kFlush tiles each in turn and are added to a sum in registers (7.8e-7). Warps
+// 0-3 and 4-7 are two threads per row, each with half of a tile's keys and half of the columns, who exchange the row's maximum; warp 9
+// loads, warp 10 brings Q, warp 11 is idle. 24 mixed sequences, 512 new tokens in one: 115 us, 126 with a thread per row.
+// Bound by what the softmax warps do one after another in a tile (exponentials and conversions 770 clocks, maximum 220, waiting for scores
+// 280), in long runs by the power limit: a prompt of 8192, 32 heads of 128 over 8: 648 us, 850 TFLOP/s of the 1655 that the library's
+// product reaches (1408 sustained); 1080 tokens behind 30001 keys: 715 us. 1.7e4 clocks pass before a launch's second tile: the line of
+// work 3400, finding the first piece 5500, the first scores 1500, the first tile 7500, most of it instructions fetched for the first time.
 // Every wait on a barrier is bounded (paged.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
 #include <cstring>
 

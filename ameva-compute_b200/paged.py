@@ -11,8 +11,8 @@ within the announced maxima.
 
 All functions record dispatches into a `runtime.Batch`; arguments are checked by the library's launchers, which the batch reports when it is
 submitted or instantiated. What the device finds wrong in the step's numbers (a page that is none of the cache's, a length past the
-table) is left out and counted in `status`: two 32-bit words, the count (to be zeroed by the caller) and the lowest `node` number that
-met one (to be set to 0xFFFFFFFF).
+table) is left out and counted in `status`: two 32-bit words, the count (to be zeroed by the caller; a page counts for every tile that
+meets it) and the lowest `node` number that met one (to be set to 0xFFFFFFFF).
 """
 from __future__ import annotations
 
@@ -29,7 +29,7 @@ def _bits(v: float) -> int:
 
 @dataclass
 class Cache:
-    """One layer's keys and values, f16, in pages of `page_size` tokens. layout "token": [page][token][head][head_dim], a token's heads
+    """One layer's keys and values, f16, in pages of `page_size` tokens, two ranges that do not meet. layout "token": [page][token][head][head_dim], a token's heads
     beside one another; "head": [page][head][token][head_dim], a head's tokens beside one another (longer runs for the attention)."""
     k: rt.Buffer
     v: rt.Buffer
@@ -58,7 +58,7 @@ class Cache:
 @dataclass
 class Sequences:
     """A batch. table: i32 [n_seqs][table_stride], the pages of every sequence; q_start: i32 [n_seqs + 1], sequence s has the rows
-    q_start[s] .. q_start[s + 1] - 1 of the step; kv_len: i32 [n_seqs], the keys of every sequence, this step's among them. rows, max_q and
+    q_start[s] .. q_start[s + 1] - 1 of the step (not decreasing); kv_len: i32 [n_seqs], the keys of every sequence, this step's among them. rows, max_q and
     max_kv announce the most rows of a step, of one sequence, and the most keys of one: launches are sized by them."""
     table: rt.Buffer
     q_start: rt.Buffer
@@ -113,7 +113,8 @@ def record_attention(batch: rt.Batch, cache: Cache, seqs: Sequences, q: rt.Buffe
                      dst_stride: Optional[int] = None, node: int = 0) -> None:
     """q f16 [rows][heads x head_dim] -> dst f32 (f16_out: f16) [rows][heads x head_dim]. Query j of a sequence's n sees the keys up to its
     own place kv_len - n + j (window: that many of them); one that sees none is zero, rows behind the last sequence are left as they
-    are. scratch: see `scratch_bytes`; a smaller one means fewer CTAs, not another result than rounding makes."""
+    are. scratch: see `scratch_bytes`; a smaller one means fewer CTAs, not another result than rounding makes. Launches behind one another
+    may share it, batches that run at the same time may not."""
     push = _attention_push(cache, seqs, heads, scale, softcap, f16_out, q_stride, dst_stride) + [window, node]
     batch.dispatch(batch.ctx.kernel("ameva_paged_attn"), [q, cache.k, cache.v, seqs.table, seqs.q_start, seqs.kv_len, dst, scratch, status], push)
 
@@ -130,8 +131,8 @@ def record_prefix_attention(batch: rt.Batch, cache: Cache, seqs: Sequences, q: r
 
 
 def scratch_bytes(ctx: rt.Context, seqs: Sequences, *, heads: int, head_dim: int, prefix: bool = False, sms: int = 148) -> int:
-    """Bytes of scratch with which the attention of this batch takes the whole GPU: per SM two row tiles of 16 rows of eight KV heads and
-    two of 256 rows, and for a shared prefix the rows' results over their own keys."""
+    """Bytes of scratch with which the attention of this batch takes the whole GPU of `ctx` (every B200 has 148 SMs): per SM two row tiles of
+    16 rows of eight KV heads and two of 256 rows, and for a shared prefix the rows' results over their own keys."""
     row = (head_dim + 4) * 4
     own = seqs.rows * heads * row + 256 if prefix else 0
     return own + sms * (2 * (8 * 16 + 256) * row + 128) + 8192
