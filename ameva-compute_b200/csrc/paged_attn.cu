@@ -268,16 +268,16 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                         for (uint32_t kk = 0; kk < 2u; ++kk) ph[kk][1] = ph[kk][3] = pl[kk][1] = pl[kk][3] = 0u;
                         break;
                     }
-                    float x[4][2], mx = neg_inf();
+                    float x[8], mx = neg_inf();   // 2 nt + j
 #pragma unroll
-                    for (uint32_t nt = 0; nt < 4u; ++nt)
+                    for (uint32_t i = 0; i < 8u; ++i) x[i] = sc[i >> 1][2u * h + (i & 1u)];
+                    capped(pc, x);
 #pragma unroll
-                        for (uint32_t j = 0; j < 2u; ++j) {
-                            const uint32_t key = key0 + 8u * nt + 2u * t4 + j;
-                            const float v = capped(pc, sc[nt][2u * h + j]);
-                            x[nt][j] = plain || (key >= span[h].lo && key < span[h].hi && seen[nt >> 1]) ? v : neg_inf();
-                            mx = fmaxf(mx, x[nt][j]);
-                        }
+                    for (uint32_t i = 0; i < 8u; ++i) {
+                        const uint32_t key = key0 + 8u * (i >> 1) + 2u * t4 + (i & 1u);
+                        x[i] = plain || (key >= span[h].lo && key < span[h].hi && seen[i >> 2]) ? x[i] : neg_inf();
+                        mx = fmaxf(mx, x[i]);
+                    }
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                     const float m_new = fmaxf(m_run[h], mx);
@@ -295,7 +295,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                     float sum = 0.0f;
 #pragma unroll
                     for (uint32_t nt = 0; nt < 4u; ++nt) {
-                        const float p0 = ex2(x[nt][0] - ref), p1 = ex2(x[nt][1] - ref);
+                        const float p0 = ex2(x[2u * nt] - ref), p1 = ex2(x[2u * nt + 1u] - ref);
                         sum += p0 + p1;
                         const __half2 hi2 = __floats2half2_rn(p0, p1);
                         ph[nt >> 1][2u * (nt & 1u) + h] = *reinterpret_cast<const uint32_t*>(&hi2);
@@ -659,7 +659,7 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
     pc.softcap = word_f(w[17]);
     pc.scale2 = pc.scale * kLog2e;
     if (pc.softcap > 0.0f) {
-        pc.cap_in = 2.0f * kLog2e * pc.scale / pc.softcap;
+        pc.cap_in = pc.scale / pc.softcap;
         pc.cap_out = pc.softcap * kLog2e;
     }
     if (!D || !pc.n_head || !pc.n_head_kv || pc.n_head % pc.n_head_kv || !pc.n_seqs || !pc.rows || !pc.max_q || !pc.max_kv || !P || (P & (P - 1u)) ||

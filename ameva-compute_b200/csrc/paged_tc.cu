@@ -571,10 +571,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 tmem_wait_ld();
                 // the same for every thread of the group
                 const bool open = gone == 0u && key0 >= x.lo_all && key0 + kTcKeys <= x.hi_all, scaled = pc.softcap == 0.0f && pc.scale2 > 0.0f;
-                if (!scaled) {   // the cap, or a scale that is not positive
-#pragma unroll
-                    for (uint32_t k = 0; k < KEYS; ++k) s[k] = capped(pc, s[k]);
-                }
+                if (!scaled) capped(pc, s);   // the cap, or a scale that is not positive
                 if (!open) {     // hidden keys: a bit per key of 32
 #pragma unroll
                     for (uint32_t c = 0; c < KEYS; c += 32u) {

@@ -202,6 +202,9 @@ def test_scales_and_strides(ctx, q, kv, kw):
 def test_announced_maxima_may_be_larger(ctx):
     """Launches are sized by the announcement: the same results where it is wide of the mark, and none where nothing is to be done."""
     both(Setup(ctx, [1, 1], [100, 40], 8, 2, 128, pad=200, max_q=150, max_kv=5000, stride=320))
+    # 33 .. 64 rows: the tensor-core kernel where much work is announced, beside 32 and fewer in the other one
+    both(Setup(ctx, [10, 3, 16, 0, 8, 9], [100, 40, 300, 5, 8, 700], 8, 2, 128, pad=2, max_kv=200000, garbage=True))
+    both(Setup(ctx, [10, 3, 16, 0, 8, 9], [100, 40, 300, 5, 8, 700], 8, 2, 64, pad=2, max_kv=200000, garbage=True), window=90000)
     both(Setup(ctx, [0, 0, 0], [100, 0, 40], 8, 2, 128, pad=200, max_q=150, max_kv=5000, stride=320))
     both(Setup(ctx, [0, 0], [100, 40], 8, 2, 64, pad=3, prefix=33))
 
@@ -240,6 +243,20 @@ def test_long_sums(ctx, q, kv, H, D):
     want, got = s.want(), s.attend()
     y = np.stack([want[j] for j in range(q)])
     assert np.linalg.norm(got - y) <= 2.6e-6 * np.linalg.norm(y)
+    s.close()
+
+
+@pytest.mark.parametrize("q,D,H,Hkv", [(1, 128, 8, 2), (100, 128, 4, 1), (90, 64, 2, 1), (2, 256, 4, 2)])
+@pytest.mark.parametrize("softcap", [30.0, 3.0])
+def test_capped_scores_of_32_bits(ctx, q, D, H, Hkv, softcap):
+    """A score's error is a weight's relative one, and independent from key to key: a result is off by as much of itself as a score is on the
+    average. Scores of one: the sum's error (16 additions, 2^-24 each of partial sums below one) 2^-20 at most and 2^-22 on the average, the cap
+    2^-23 of the score for small ones and, above a quarter of the cap, 2^-22 of the cap at most: 7e-7 for a cap of 3, where all of it is rare
+    for a cap of 30. Twice their sum on the average: 1e-6."""
+    s = Setup(ctx, [q], [700], H, Hkv, D, seed=3)
+    want, got = s.want(softcap=softcap), s.attend(softcap=softcap)
+    y = np.stack([want[j] for j in range(q)])
+    assert np.linalg.norm(got - y) <= 1e-6 * np.linalg.norm(y)
     s.close()
 
 
