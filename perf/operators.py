@@ -296,18 +296,21 @@ def _attend_plain(s):
 
 
 # ---- the framework's calls ---------------------------------------------------------------------------------------------
-_context = None
+_context = _stream = None
 
 
 class _Plan:
-    """A call recorded once and replayed, as a serving loop does it; what it created is destroyed with it."""
+    """A call recorded once and replayed, as a serving loop does it; what it created is destroyed with it. The context's stream and torch's
+    know nothing of one another: events order a pass behind what torch has made of its inputs, and torch behind the pass."""
 
     def __init__(self, s):
-        global _context
+        global _context, _stream
         amv = importlib.import_module("ameva-compute_b200")
         if _context is None:
             _context = amv.runtime.init()
+            _stream = torch.cuda.ExternalStream(_context.stream)
         paged, ctx, c = amv.paged, _context, s.case
+        self.before, self.after = torch.cuda.Event(), torch.cuda.Event()
         self.owned, self.tensors, self.event = [], [], None
 
         def bind(t):
@@ -341,7 +344,12 @@ class _Plan:
     def run(self):
         if self.event is not None:
             self.event.destroy()      # of the pass before
+        torchs = torch.cuda.current_stream()
+        self.before.record(torchs)
+        _stream.wait_event(self.before)
         self.event = self.batch.replay()
+        self.after.record(_stream)
+        torchs.wait_event(self.after)
         return self.out
 
     def __del__(self):
