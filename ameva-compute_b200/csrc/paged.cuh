@@ -361,11 +361,13 @@ __device__ __forceinline__ float score2(const Args& pc, float s) {
     return pc.softcap != 0.0f ? pc.softcap * tanhf(s * pc.scale / pc.softcap) * kLog2e : s * pc.scale2;
 }
 
-// score2 of N scores a thread, by a converged warp, without tanhf's some 25 instructions. While all arguments are small (a cap of 30 and
-// scores below 7.5): the odd series y - y^3 / 3 + 2 y^5 / 15 - 17 y^7 / 315 + 62 y^9 / 2835, whose next term is below 1e-8 of it for |y| <= 1/4.
-// Otherwise 1 - 2 / (1 + e^2y) by two special functions, with an absolute error of 2^-22 where the largest tanh is at least 0.24 (alone, and
-// times a cap of 30, that is 7e-6 of a score: 1.4e-6 of a result that ordinary 32-bit operations leave with 2e-7). One branch for
-// all: a branch per score is slower than both forms (32 drafted sequences 24 us instead of 22.7).
+// score2 of N scores a thread, by a converged warp, without tanhf's some 25 instructions. Each score by its own size alone. Up to a quarter of
+// the cap (7.5 of 30): the odd series y - y^3 / 3 + 2 y^5 / 15 - 17 y^7 / 315 + 62 y^9 / 2835, whose next term is below 1e-8 of it for
+// |y| <= 1/4. Beyond: 1 - 2 / (1 + e^2y) by two special functions, with an absolute error of 2^-22 where tanh is at least 0.24 (times a cap of
+// 30, that is 7e-6 of a score: 1.4e-6 of a result that ordinary 32-bit operations leave with 2e-7). The warp's vote only spares it the second
+// form where nobody takes it; among its scores are hidden ones of any value (keys that nobody has written, shared memory of an earlier
+// kernel), which are not to decide how exact the others are. One branch for all: a branch per score is slower than both forms (32 drafted
+// sequences 24 us instead of 22.7).
 template <uint32_t N>
 __device__ __forceinline__ void capped(const Args& pc, float (&s)[N]) {
     if (pc.softcap == 0.0f) {
@@ -379,19 +381,20 @@ __device__ __forceinline__ void capped(const Args& pc, float (&s)[N]) {
         s[k] *= pc.cap_in;
         small = small && fabsf(s[k]) <= 0.25f;
     }
+    auto series = [&](float y) {
+        const float y2 = y * y, t = fmaf(y2, fmaf(y2, fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
+        return pc.cap_out * fmaf(y * y2, t, y);
+    };
     if (__all_sync(0xffffffffu, small)) {
 #pragma unroll
-        for (uint32_t k = 0; k < N; ++k) {
-            const float y = s[k], y2 = y * y, t = fmaf(y2, fmaf(y2, fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
-            s[k] = pc.cap_out * fmaf(y * y2, t, y);
-        }
+        for (uint32_t k = 0; k < N; ++k) s[k] = series(s[k]);
         return;
     }
 #pragma unroll
     for (uint32_t k = 0; k < N; ++k) {
         float r;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s[k] * (2.0f * kLog2e))));
-        s[k] = fmaf(-2.0f * pc.cap_out, r, pc.cap_out);
+        s[k] = fabsf(s[k]) <= 0.25f ? series(s[k]) : fmaf(-2.0f * pc.cap_out, r, pc.cap_out);
     }
 }
 // One row by a whole warp over keys [lo, hi), hidden keys left out instead of multiplied by zero: a lane's C columns of
