@@ -301,6 +301,26 @@ __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, ptx::Ctl*
     }
     return true;
 }
+// Waits for what the last stages of a ring were asked for: copy i of `issued` is the i / stages-th of stage i % stages. A copy that lands
+// after its CTA has left would write into the memory of the next one, so this goes by the copies alone, not by whether the CTA has given
+// up, and a warp that has asked for copies does it whenever it leaves: another one may give up later. They land within microseconds;
+// kDrainPolls polls of 64 ns or more bound the wait. arrived(stage, parity): whether the phase has completed.
+constexpr uint32_t kDrainPolls = 1u << 14;
+template <class Arrived>
+__host__ __device__ __forceinline__ bool drain_copies(uint32_t issued, uint32_t stages, Arrived arrived) {
+    for (uint32_t i = issued > stages ? issued - stages : 0u; i < issued; ++i)
+        for (uint32_t polls = 0; !arrived(i % stages, i / stages & 1u);)
+            if (++polls == kDrainPolls) return false;
+    return true;
+}
+__device__ __forceinline__ bool arrived_or_pause(uint32_t bar, uint32_t parity) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    __nanosleep(64);
+    return false;
+}
+__device__ __forceinline__ void drain_ring(uint32_t full, uint32_t issued, uint32_t stages) {
+    drain_copies(issued, stages, [&](uint32_t stage, uint32_t parity) { return arrived_or_pause(full + 8u * stage, parity); });
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

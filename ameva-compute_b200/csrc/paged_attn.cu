@@ -179,10 +179,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                 }
             }
         }
-        if (ctl->abort) {   // copies already requested finish before the CTA leaves
-            for (uint32_t i = issued > stages ? issued - stages : 0u; i < issued; ++i)
-                wait_on(full + 8u * (i % stages), (i / stages) & 1u, ctl, pc.status, 0xC10u);
-        }
+        drain_ring(full, issued, stages);
         return;
     }
 

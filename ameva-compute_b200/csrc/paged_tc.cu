@@ -23,7 +23,8 @@
 // 280), in long runs by the power limit: a prompt of 8192, 32 heads of 128 over 8: 648 us, 850 TFLOP/s of the 1655 that the library's
 // product reaches (1408 sustained); 1080 tokens behind 30001 keys: 715 us. 1.7e4 clocks pass before a launch's second tile: the line of
 // work 3400, finding the first piece 5500, the first scores 1500, the first tile 7500, most of it instructions fetched for the first time.
-// Every wait on a barrier is bounded (paged.cuh); a CTA that gives up drains its copies and MMAs, frees its tensor memory and returns.
+// Every wait on a barrier is bounded (paged.cuh). The warps that ask for copies and issue MMAs leave when these are done, in a CTA that gives
+// up, too; then its tensor memory is freed.
 #include <cstring>
 
 #include "paged.h"
@@ -342,10 +343,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     load_v = load;
                 }
             }
-            if (ctl->abort) {   // copies already requested finish before the CTA leaves
-                for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) wait_on(k_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD20u);
-                for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) wait_on(v_full + 8u * (i % ST), (i / ST) & 1u, ctl, pc.status, 0xD30u);
-            }
+            drain_ring(k_full, k_issued, ST);
+            drain_ring(v_full, v_issued, ST);
         } else if (warp < L::LOAD) {
             const uint32_t g = warp - L::MMA;
             const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
@@ -463,10 +462,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 }
                 tiles += p.b - p.a;
             }
-            if (__any_sync(0xffffffffu, ctl->abort != 0u)) {   // MMAs already issued finish before the CTA leaves
-                commit(drain + 8u * g);
-                for (uint32_t spins = 0; spins < 4096u && !mbar_try_wait(drain + 8u * g, 0u); ++spins) __nanosleep(64);
-            }
+            commit(drain + 8u * g);   // MMAs already issued finish before the CTA gives its memory back, whoever gives up, and when
+            drain_ring(drain + 8u * g, 1u, 1u);
         } else if (warp == L::QWARP) {
             // Q rows into the K-major 128-byte swizzle, idle rows zero
             uint32_t uses[2] = {0u, 0u};
@@ -476,10 +473,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 for (uint32_t g = 0; g < GROUPS; ++g) {
                     const Group x = group_of(pc, p, g);
                     if (x.t1 <= x.t0) continue;
-                    const uint32_t n = g ? uses[1]++ : uses[0]++;
+                    const uint32_t n = g ? uses[1] : uses[0];
                     if (n) ok = wait_on(q_empty + 8u * g, (n - 1u) & 1u, ctl, pc.status, 0xDC0u);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
+                    if (g) ++uses[1];
+                    else ++uses[0];
                     if (pc.q_boxes) {   // heads of a group in a power of two: 128 / G tokens by one copy per 64 columns (rows of others behind the last)
                         if (lane == 0u) {
                             mbar_arrive_expect_tx(q_full + 8u * g, L::Q);
@@ -514,6 +513,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (lane == 0u) mbar_arrive(q_full + 8u * g);
                 }
             }
+            drain_ring(q_full, uses[0], 1u);   // Q of a group is a ring of one stage
+            drain_ring(q_full + 8u, uses[1], 1u);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
