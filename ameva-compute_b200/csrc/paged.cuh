@@ -417,34 +417,281 @@ __device__ __forceinline__ void capped(const Args& pc, float (&s)[N]) {
         s[k] = fabsf(s[k]) <= 0.25f ? series(s[k]) : fmaf(-2.0f * pc.cap_out, r, pc.cap_out);
     }
 }
-// One row by a whole warp over keys [lo, hi), hidden keys left out instead of multiplied by zero: a lane's C columns of
-// sum 2^(score - ref) v. For rows whose accumulator is not finite: the matrix instructions multiply every key of a step with every
-// row, so a NaN or an infinity in V would reach rows that do not see its key, and an infinity would meet the remainder of its
-// probability, which may be zero or negative. Rare, so simple: a lane per key for the scores, all lanes on a key's columns.
-template <uint32_t C>
-__device__ __noinline__ void seen_keys_row(const Args& pc, const Seq& q, uint32_t hkv, const __half* qrow, uint32_t lo, uint32_t hi, float ref,
-                                           float (&o)[C]) {
-    constexpr uint32_t D = 32u * C;
-    const uint32_t lane = threadIdx.x & 31u, mask = (1u << pc.page_log2) - 1u;
+// A warp's rows once more, behind the last piece of its CTA, where one of them was not finite: the matrix instructions multiply every key of
+// a step with every row, so a NaN or an infinity in V reaches rows that do not see its key, and an infinity meets the remainder of its
+// probability, which may be zero or negative. The CTA's stretch is walked again, for rows first_row .. first_row + count - 1 of each row tile
+// (32 at most), head hb of a group, whose result of a piece, in dst or the piece's slot, is not finite. Nobody waits for this on a barrier
+// with a limit, so it may take its time.
+// Where Q and K are finite, a column in which a row sees values that are not is their sum: NaN, or one of the infinities, whatever their
+// weights are. So the keys are looked through, once for all rows where all see them. A row that is not finite in another column,
+// too, has it from a key that it does not see, and is formed anew, hidden keys left out instead of multiplied by zero: four rows and 32
+// keys at a time, in 32 bits; a score ends in the lane of its key's number.
+// For both, D / 8 lanes take a key, 16 bytes each; group g of them has keys g D / 8 .. of 32, one after another, and the groups meet at the end.
+// One infinity at the first key of every sequence, without / with it: a prompt of 2048, 8 heads of 128 over 2: 46 / 337 us, of 8192, 32 heads over
+// 8: 590 / 7300 us (32-bit results 1090 / 10100); 32 single tokens of 4000 keys 100 / 362 us. Each row's scores again: 17500 us for the first.
+template <uint32_t C, uint32_t ROWS>
+struct Again {
+    static constexpr uint32_t D = 32u * C, N = 4, LANES = D / 8u, AHEAD = 4, kNone = 0xFFFFFFFFu;
+    const Args& pc;
+    Piece p;
+    uint32_t hkv, lane, sub, lead;
+    bool whole;
+    float* slot;
+
+    static __device__ __forceinline__ void half8(const uint4& x, float (&y)[8]) {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (uint32_t c = 0; c < C; ++c) o[c] = 0.0f;
-    for (uint32_t key0 = lo; key0 < hi; key0 += 32u) {
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            y[2u * i] = f.x;
+            y[2u * i + 1u] = f.y;
+        }
+    }
+    static __device__ __forceinline__ bool odd(const uint4& x) {   // an exponent of ones in any of the eight
+        auto w = [](uint32_t v) { return (v & 0x7C007C00u) + 0x04000400u; };
+        return ((w(x.x) | w(x.y) | w(x.z) | w(x.w)) & 0x80008000u) != 0u;
+    }
+    static __device__ __forceinline__ void groups_meet(float (&x)[8]) {
+#pragma unroll
+        for (uint32_t w = LANES; w < 32u; w <<= 1)
+#pragma unroll
+            for (uint32_t c = 0; c < 8u; ++c) x[c] += __shfl_xor_sync(0xffffffffu, x[c], w);
+    }
+    __device__ __forceinline__ uint32_t token(uint32_t r) const { return p.q.tok0 + query_of(pc, r); }
+    __device__ __forceinline__ uint32_t head(uint32_t r) const { return hkv * pc.G + r - query_of(pc, r) * pc.G; }
+    __device__ __forceinline__ bool is_f16() const { return whole && pc.out == OUT_F16; }
+    __device__ __forceinline__ float* f32_row(uint32_t r) const {   // this lane's eight columns of what the first pass left
+        float* x = whole ? reinterpret_cast<float*>(pc.dst) + dst_row(pc, token(r), head(r), D) + (pc.out == OUT_PARTS ? 4u : 0u)
+                         : slot + (uint64_t)(r - p.r0) * (D + 4u) + 4u;
+        return x + 8u * sub;
+    }
+    __device__ __forceinline__ __half* f16_row(uint32_t r) const { return reinterpret_cast<__half*>(pc.dst) + dst_row(pc, token(r), head(r), D) + 8u * sub; }
+    __device__ __forceinline__ void read(uint32_t r, float (&x)[8]) const {
+        if (is_f16()) {
+            half8(*reinterpret_cast<const uint4*>(f16_row(r)), x);
+        } else {
+            const float4 *at = reinterpret_cast<const float4*>(f32_row(r)), u = at[0], v = at[1];
+            x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+        }
+    }
+    __device__ __forceinline__ bool finite(uint32_t r) const {
+        float x[8], sum = 0.0f;
+        read(r, x);
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) sum = fmaf(x[c], 0.0f, sum);
+        return __all_sync(0xffffffffu, sum == 0.0f) != 0;
+    }
+    // 32 keys from key0 on, below `last`: this lane's key's row in the caches, and which of them are there
+    __device__ __forceinline__ uint32_t keys_at(uint32_t key0, uint32_t last, uint64_t& at) const {
         const uint32_t key = key0 + lane;
-        const int32_t page = key < hi ? page_of(pc, q, key) : -1;
-        const uint64_t row = (uint64_t)(page < 0 ? 0 : page) * pc.c_ps + (uint64_t)(key & mask) * pc.c_ts + (uint64_t)hkv * pc.c_hs;
-        float p = 0.0f;
-        if (page >= 0) {
-            float s = 0.0f;
-            for (uint32_t c = 0; c < D; ++c) s = fmaf(__half2float(qrow[c]), __half2float(pc.k[row + c]), s);
-            p = ex2(score2(pc, s) - ref);
-        }
-        for (uint32_t seen = __ballot_sync(0xffffffffu, page >= 0); seen; seen &= seen - 1u) {
-            const int b = __ffs(seen) - 1;
-            const float pb = __shfl_sync(0xffffffffu, p, b);
-            const __half* vr = pc.v + __shfl_sync(0xffffffffu, (unsigned long long)row, b) + C * lane;
+        const int32_t page = key < last ? page_of(pc, p.q, key) : -1;
+        at = (uint64_t)(page < 0 ? 0 : page) * pc.c_ps + (uint64_t)(key & ((1u << pc.page_log2) - 1u)) * pc.c_ts + (uint64_t)hkv * pc.c_hs;
+        return __ballot_sync(0xffffffffu, page >= 0);
+    }
+    __device__ __forceinline__ uint4 load(const __half* cache, uint64_t at, uint32_t there, uint32_t i) const {   // this lane's columns of key lead + i
+        const uint64_t e = __shfl_sync(0xffffffffu, (unsigned long long)at, lead + i) + 8u * sub;
+        return there >> (lead + i) & 1u ? *reinterpret_cast<const uint4*>(cache + e) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    // Adds up this lane's columns of what is not finite in V; false: something of K is not.
+    __device__ __noinline__ bool look_through(uint32_t first, uint32_t last, float (&sum)[8]) const {
+        bool plain = true;
+#pragma unroll 1
+        for (uint32_t key0 = first; key0 < last; key0 += 32u) {
+            uint64_t at;
+            const uint32_t there = keys_at(key0, last, at);
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < LANES; i0 += AHEAD) {
+                uint4 x[AHEAD], y[AHEAD];
 #pragma unroll
-            for (uint32_t c = 0; c < C; ++c) o[c] = fmaf(pb, __half2float(vr[c]), o[c]);
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    x[i] = load(pc.v, at, there, i0 + i);
+                    y[i] = load(pc.k, at, there, i0 + i);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    plain = plain && !odd(y[i]);
+                    if (!odd(x[i])) continue;
+                    float v[8];
+                    half8(x[i], v);
+#pragma unroll
+                    for (uint32_t c = 0; c < 8u; ++c) sum[c] += v[c] * 0.0f == 0.0f ? 0.0f : v[c];
+                }
+            }
         }
+        return __all_sync(0xffffffffu, plain) != 0;
+    }
+    // Row r of what the rows see together, [a, b), its sum there and whether that tells all: whether the row is right now.
+    __device__ __forceinline__ bool from_sums(uint32_t r, uint32_t from, uint32_t to, uint32_t a, uint32_t b, const float (&common)[8], bool plain) const {
+        const Span s = row_span(pc, p.q, r);
+        float sum[8];
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) sum[c] = 0.0f;
+        plain = plain && !odd(*reinterpret_cast<const uint4*>(pc.q + (uint64_t)token(r) * pc.q_s + (uint64_t)head(r) * D + 8u * sub));
+        const uint32_t lo = max(s.lo, from), hi = min(s.hi, to);
+        if (lo < a) plain = look_through(lo, min(a, hi), sum) && plain;
+        if (b < hi) plain = look_through(max(b, lo), hi, sum) && plain;
+        groups_meet(sum);
+        float x[8];
+        read(r, x);
+        const float* extra = whole && pc.out != OUT_PARTS && pc.extra ? pc.extra + ((uint64_t)token(r) * pc.n_head + head(r)) * (D + 4u) + 4u + 8u * sub : nullptr;
+        bool known = plain;
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) {
+            if (x[c] * 0.0f == 0.0f) continue;
+            x[c] = sum[c] + common[c];
+            known = known && x[c] != 0.0f;
+            if (extra && extra[c] * 0.0f != 0.0f) x[c] += extra[c];
+        }
+        if (!__all_sync(0xffffffffu, known)) return false;
+        if (lead == 0u) {   // (finite columns are written as they were)
+            if (is_f16()) {
+#pragma unroll
+                for (uint32_t c = 0; c < 8u; ++c) f16_row(r)[c] = __float2half_rn(x[c]);
+            } else {
+#pragma unroll
+                for (uint32_t c = 0; c < 8u; ++c) f32_row(r)[c] = x[c];
+            }
+        }
+        return true;
+    }
+    // The first rows of a mask (bit b: row base + b), up to N of them, over the keys they see.
+    __device__ __noinline__ uint32_t from_keys(uint32_t mask, uint32_t base, uint32_t from, uint32_t to) const {
+        uint32_t row[N], lo[N], hi[N], first = kNone, last = 0u;
+        float m[N], l[N], qf[N][8], o[N][8];
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {   // (one that sees nothing where fewer than N are left)
+            const bool have = mask != 0u;
+            row[j] = have ? base + (uint32_t)__ffs(mask) - 1u : kNone;
+            mask &= mask - (have ? 1u : 0u);
+            const uint32_t r = have ? row[j] : p.r0;
+            half8(*reinterpret_cast<const uint4*>(pc.q + (uint64_t)token(r) * pc.q_s + (uint64_t)head(r) * D + 8u * sub), qf[j]);
+            const Span s = row_span(pc, p.q, r);
+            lo[j] = have ? max(s.lo, from) : kNone;
+            hi[j] = have ? min(s.hi, to) : 0u;
+            first = min(first, lo[j]);
+            last = max(last, hi[j]);
+            m[j] = neg_inf();
+            l[j] = 0.0f;
+#pragma unroll
+            for (uint32_t c = 0; c < 8u; ++c) o[j][c] = 0.0f;
+        }
+#pragma unroll 1
+        for (uint32_t key0 = first; key0 < last; key0 += 32u) {
+            uint64_t at;
+            const uint32_t there = keys_at(key0, last, at), key = key0 + lane;
+            float w[N];
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < LANES; i0 += AHEAD) {
+                uint4 x[AHEAD];
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) x[i] = load(pc.k, at, there, i0 + i);
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    float kf[8];
+                    half8(x[i], kf);
+#pragma unroll
+                    for (uint32_t j = 0; j < N; ++j) {
+                        float s = 0.0f;
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; ++c) s = fmaf(qf[j][c], kf[c], s);
+#pragma unroll
+                        for (uint32_t d = 1; d < LANES; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+                        w[j] = sub == i0 + i ? s : w[j];
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) {
+                const bool seen = (there >> lane & 1u) && key >= lo[j] && key < hi[j];
+                const float s = score2(pc, w[j]);
+                float top = seen ? s : neg_inf();
+#pragma unroll
+                for (uint32_t d = 1; d < 32u; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                if (top > m[j]) {
+                    const float f = weight(m[j], top);
+                    m[j] = top;
+                    l[j] *= f;
+#pragma unroll
+                    for (uint32_t c = 0; c < 8u; ++c) o[j][c] *= f;
+                }
+                // negative: not seen. A weight too small for 32 bits is one all the same: an infinity times it is infinite
+                const float e = ex2(s - (m[j] == neg_inf() ? 0.0f : m[j]));
+                w[j] = !seen ? -1.0f : e == 0.0f && s != neg_inf() ? 1.17549435e-38f : e;
+                l[j] += seen ? w[j] : 0.0f;
+            }
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < LANES; i0 += AHEAD) {
+                uint4 x[AHEAD];
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) x[i] = load(pc.v, at, there, i0 + i);
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    float vf[8];
+                    half8(x[i], vf);
+#pragma unroll
+                    for (uint32_t j = 0; j < N; ++j) {
+                        const float y = __shfl_sync(0xffffffffu, w[j], lead + i0 + i);
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; ++c) o[j][c] = y < 0.0f ? o[j][c] : fmaf(y, vf[c], o[j][c]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+            if (row[j] == kNone) continue;
+            groups_meet(o[j]);
+            float y[C];   // columns C lane ..: of those that lane C lane / 8 has
+#pragma unroll
+            for (uint32_t c = 0; c < 8u; ++c) {
+                const float x = __shfl_sync(0xffffffffu, o[j][c], C * lane / 8u);
+                if (c / C == C * lane % 8u / C) y[c % C] = x;
+            }
+#pragma unroll
+            for (uint32_t d = 1; d < 32u; d <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
+            if (whole) {
+                finish_row<C>(pc, token(row[j]), head(row[j]), m[j], l[j], y);
+            } else {
+                float* to_row = slot + (uint64_t)(row[j] - p.r0) * (D + 4u);
+                if (lane == 0u) *reinterpret_cast<float2*>(to_row) = make_float2(m[j], l[j]);
+#pragma unroll
+                for (uint32_t c = 0; c < C; ++c) to_row[4u + C * lane + c] = y[c];
+            }
+        }
+        return mask;
+    }
+};
+template <uint32_t C, uint32_t ROWS>
+__device__ __noinline__ void seen_keys_rows(const Args& pc, const Stretch& st, const uint32_t* s_pref, uint32_t hb, uint32_t first_row, uint32_t count) {
+    Walk<ROWS> walk(st);
+    while (walk.next(pc, s_pref)) {
+        const Piece& p = walk.p;
+        const uint32_t hkv = p.group * pc.HB + hb, lane = threadIdx.x & 31u, sub = lane % (4u * C);
+        if (hkv >= pc.n_head_kv) continue;
+        const Again<C, ROWS> x = {pc, p, hkv, lane, sub, lane - sub, p.a == 0u && p.b == p.n,
+                                  pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * pc.HB + hb) * ROWS * (32u * C + 4u)};
+        const uint32_t from = (p.first + p.a) << pc.keys_log2, to = (p.first + p.b) << pc.keys_log2;
+        const uint32_t base = p.r0 + first_row, end = min(p.R, base + count);
+        uint32_t mask = 0u, low = 0u, high = 0u;   // rows that are not finite, the first and the last of them
+        for (uint32_t r = base; r < end; ++r)
+            if (!x.finite(r)) {
+                low = mask ? low : r;
+                high = r;
+                mask |= 1u << (r - base);
+            }
+        if (!mask) continue;
+        const uint32_t a = max(row_span(pc, p.q, high).lo, from), b = max(a, min(row_span(pc, p.q, low).hi, to));   // seen by all of them
+        float common[8];
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) common[c] = 0.0f;
+        const bool plain = x.look_through(a, b, common);
+        x.groups_meet(common);
+        uint32_t anew = 0u;
+        for (uint32_t left = mask; left; left &= left - 1u) {
+            const uint32_t i = (uint32_t)__ffs(left) - 1u;
+            if (!plain || !x.from_sums(base + i, from, to, a, b, common, plain)) anew |= 1u << i;
+        }
+        while (anew) anew = x.from_keys(anew, base, from, to);
     }
 }
 

@@ -189,7 +189,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     const uint32_t g = lane >> 2, t4 = lane & 3u;
     const uint32_t lm_row = (lane & 7u) + ((lane >> 4) << 3), lm_hi = (lane >> 3) & 1u;   // K: key in the block, upper eight columns
     const uint32_t lv_row = (lane & 7u) + (((lane >> 3) & 1u) << 3), lv_nt = lane >> 4;    // V: key in the block, second n-tile
-    bool cut = false;
+    bool cut = false, again = false;   // again: rows that are not finite although their sum is
     while (walk.next(pc, s_pref)) {
         const Piece& p = walk.p;
         const uint32_t hkv = p.group * HB + hb;
@@ -386,29 +386,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                 check += __shfl_xor_sync(0xffffffffu, check, 1);
                 check += __shfl_xor_sync(0xffffffffu, check, 2);
                 // (a sum that is not finite says that the scores are not: the row is NaN either way)
-                const bool again = valid[h] && check != 0.0f && l_run[h] - l_run[h] == 0.0f;
-                if (valid[h] && !again) {
+                again = again || (valid[h] && check != 0.0f && l_run[h] - l_run[h] == 0.0f);
+                if (valid[h]) {
                     if (whole && pc.out != OUT_PARTS) finish_fragment<NT>(pc, token[h], head[h], t4, m_run[h], l_run[h], oc, h);
                     else
                         store_part<NT>(whole ? reinterpret_cast<float*>(pc.dst) + dst_row(pc, token[h], head[h], D) : slot + (uint64_t)(g + 8u * h) * (D + 4u),
                                        t4, m_run[h], l_run[h], oc, h);
-                }
-                for (uint32_t bad = __ballot_sync(0xffffffffu, again && t4 == 0u); bad; bad &= bad - 1u) {   // by the whole warp
-                    const int from = __ffs(bad) - 1;
-                    const uint32_t r = p.r0 + (uint32_t)from / 4u + 8u * h, query = query_of(pc, r), tk = p.q.tok0 + query, hd = hkv * pc.G + r - query * pc.G;
-                    const float m = __shfl_sync(0xffffffffu, m_run[h], from), l = __shfl_sync(0xffffffffu, l_run[h], from);
-                    const Span s = row_span(pc, p.q, r);
-                    float o[C];
-                    seen_keys_row<C>(pc, p.q, hkv, pc.q + (uint64_t)tk * pc.q_s + (uint64_t)hd * D, max(s.lo, (p.first + p.a) << pc.keys_log2),
-                                     min(s.hi, (p.first + p.b) << pc.keys_log2), m == neg_inf() ? 0.0f : m, o);
-                    if (whole) {
-                        finish_row<C>(pc, tk, hd, m, l, o);
-                    } else {
-                        float* to = slot + (uint64_t)(r - p.r0) * (D + 4u);
-                        if (lane == 0u) *reinterpret_cast<float2*>(to) = make_float2(m, l);
-#pragma unroll
-                        for (uint32_t c = 0; c < C; ++c) to[4u + C * lane + c] = o[c];
-                    }
                 }
             }
         }
@@ -418,6 +401,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         }
     }
     if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    if (__any_sync(0xffffffffu, again && ok)) {
+        __syncwarp();   // (the rows that other lanes have stored are read)
+        seen_keys_rows<C, kDecRows>(pc, st, s_pref, hb, 0u, kDecRows);
+    }
 }
 
 // Joins the cut row tiles. CTA x of the kernel in front notes a row tile that it begins and others end; its parts lie in slot 2 x + 1 and

@@ -536,7 +536,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             return y.x;
         };
         uint32_t j = 0, tiles = 0;   // key tiles of this group, of the CTA, so far
-        bool cut = false;
+        bool cut = false, again = false;   // again: rows that are not finite although their sum is
         while (walk.next(pc, s_pref)) {
             const Piece& p = walk.p;
             const Group x = group_of(pc, p, g);
@@ -751,23 +751,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     __syncwarp();
                 }
                 if (EXACT) check += tell(check, ok);   // (what the other warp has written of the rows is there)
-                // rows that are not finite although their sum is: over the keys they see, by the whole warp
-                for (uint32_t again = __ballot_sync(0xffffffffu, part == 0u && valid && check != 0.0f && l_run - l_run == 0.0f); again; again &= again - 1u) {
-                    const int i = __ffs(again) - 1;
-                    const uint32_t r = x.r0 + (warp & 3u) * 32u + (uint32_t)i, q_r = query_of(pc, r), tk = p.q.tok0 + q_r, hd = p.group * pc.G + r - q_r * pc.G;
-                    const float m = __shfl_sync(0xffffffffu, m_run, i), l = __shfl_sync(0xffffffffu, l_run, i);
-                    const Span sp = row_span(pc, p.q, r);
-                    float o[C];
-                    seen_keys_row<C>(pc, p.q, p.group, pc.q + (uint64_t)tk * pc.q_s + (uint64_t)hd * D, max(sp.lo, (p.first + p.a) * kTcKeys),
-                                     min(sp.hi, (p.first + p.b) * kTcKeys), m == neg_inf() ? 0.0f : m, o);
-                    if (whole) {
-                        finish_row<C>(pc, tk, hd, m, l, o);
-                    } else {
-                        float* to_row = slot + (uint64_t)(r - x.r0) * (D + 4u) + 4u + C * lane;
-#pragma unroll
-                        for (uint32_t c = 0; c < C; ++c) to_row[c] = o[c];
-                    }
-                }
+                again = again || (valid && check != 0.0f && l_run - l_run == 0.0f);
             }
             if (p.a == 0u && p.b < p.n) {
                 cut = true;
@@ -776,6 +760,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             tc_fence_before();   // (the next P V overwrites the accumulator behind an arrival of this thread)
         }
         if (!cut && threadIdx.x == 0u && pc.cut) pc.cut[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+        if (__any_sync(0xffffffffu, again && ok)) {   // (EXACT: both warps of the rows know, and take half of them each)
+            __syncwarp();
+            seen_keys_rows<C, L::ROWS>(pc, st, s_pref, 0u, g * kGroupRows + (warp & 3u) * 32u + part * 16u, 32u / L::PARTS);
+        }
     }
     tc_fence_before();
     __syncthreads();
