@@ -327,8 +327,9 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ float neg_inf() { return __uint_as_float(0xFF800000u); }
-// exp2(m - to) of a maximum m <= to, 0 where m is that of nothing
-__device__ __forceinline__ float weight(float m, float to) { return m == neg_inf() ? 0.0f : ex2(m - to); }
+// exp2(m - to) of a maximum m <= to, 0 where m is that of nothing. Of something it is never 0, but the smallest normal number at least, which
+// leaves no trace in a finite sum: an infinity or a NaN among the values is to show in the result however small its weight is.
+__device__ __forceinline__ float weight(float m, float to) { return m == neg_inf() ? 0.0f : fmaxf(ex2(m - to), 1.17549435e-38f); }
 
 __device__ __forceinline__ uint64_t dst_row(const Args& pc, uint32_t token, uint32_t head, uint32_t D) {
     return pc.out == OUT_PARTS ? ((uint64_t)token * pc.n_head + head) * (D + 4u) : (uint64_t)token * pc.dst_s + (uint64_t)head * D;

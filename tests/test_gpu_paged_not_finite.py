@@ -130,6 +130,31 @@ def test_a_weight_below_32_bits_is_one(ctx):  # noqa: F811
         s.close()
 
 
+@pytest.mark.parametrize("q,D,H,Hkv,prefix", [(1, 128, 2, 1, 0), (1, 64, 8, 8, 0), (100, 128, 2, 1, 0), (100, 64, 4, 2, 0), (2, 256, 2, 1, 0), (1, 128, 4, 2, 500),
+                                              (40, 64, 4, 1, 500)])
+@pytest.mark.parametrize("scratch", [None, 1])
+def test_parts_whose_weight_is_below_32_bits(ctx, q, D, H, Hkv, prefix, scratch):  # noqa: F811
+    """The same where the infinity and the score of 200 are seen by different warps, CTAs or launches, whose results are joined: it does not
+    depend on where the keys are cut."""
+    kv = 3000
+    s = Setup(ctx, [q], [kv], H, Hkv, D, seed=3, prefix=prefix)
+    s.q[:], s.k[:] = 1.0, 0.0
+    s.k[place(s, 0, 2500)][:] = 200.0 / D ** 0.5
+    s.v[place(s, 0, 7)][:, 3], s.v[place(s, 0, 1200)][:, 4], s.v[place(s, 0, 1900)][:, 5] = np.inf, -np.inf, np.nan
+    if prefix:
+        s.v[s.prefix[1], 9, :, 6] = np.inf
+    upload(s)
+    want, own = s.want(), s.held * H * (D + 4) * 4 + 256 if prefix else 0
+    y = np.stack([want[r] for r in range(q)])
+    assert np.isposinf(y[:, :, 3]).all() and np.isneginf(y[:, :, 4]).all() and np.isnan(y[:, :, 5]).all()
+    for f16 in (False, True):
+        got = s.attend(f16=f16, scratch=scratch and own + 256)[:q]
+        assert np.array_equal(np.isnan(got), np.isnan(y)) and np.array_equal(np.isposinf(got), np.isposinf(y)) and np.array_equal(np.isneginf(got), np.isneginf(y))
+        fine = np.isfinite(y)
+        assert np.max(np.abs(got[fine] - y[fine])) <= (TOL16 if f16 else TOL32)
+    s.close()
+
+
 @pytest.mark.parametrize("q,kv,H,Hkv,D", [(2048, 2048, 8, 2, 128), (2048, 2048, 8, 2, 64), (1, 60000, 8, 2, 128), (1, 30000, 4, 1, 256)])
 def test_a_sequence_that_is_not_finite_does_not_stall_its_batch(ctx, q, kv, H, Hkv, D):  # noqa: F811
     """One infinity that all rows see: the call takes some times as long as without, not hundreds of times (a row at a time, every key's
