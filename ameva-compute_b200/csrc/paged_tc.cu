@@ -4,8 +4,11 @@
 // A CTA (one per SM) takes row tiles of 256 rows, two groups of 128, and walks key tiles of 64 for both (f16 results; for 32-bit ones, EXACT,
 // below, one group of 128 rows):
 //   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 64 scores from tensor memory, online softmax to base 2, write P
-//                    over the scores as f16 (and, for a 32-bit result, what that rounding left beside it). The accumulator is rescaled
-//                    only when a row's maximum has grown by more than 2^kGrowth since its last rescale. They write the piece's results.
+//                    over the scores as f16, and what that rounding left beside it, so that a result has the 32 bits that it is computed in
+//                    until it is rounded itself (without the remainder an f16 one is off by 1.25 to 1.4 times what its own rounding leaves,
+//                    and a prompt of 8192 takes 640 us instead of 795). The accumulator is rescaled only when a row's maximum has
+//                    grown by more than 2^kGrowth since its last rescale, as attention kernels for this chip are known to do. They
+//                    write the piece's results.
 //   warps 8, 9       issue the MMAs of group 0 and 1: S = Q K^T (both in shared memory), O += P V (P in tensor memory, V MN-major). Each
 //                    group has two S / P tiles; P V of key tile j and S of tile j + 2, which takes its place, leave together, so that a
 //                    group's softmax finds the next scores there while the tensor core works on the other's. A warp per group, and the
@@ -20,8 +23,8 @@
 // 0-3 and 4-7 are two threads per row, each with half of a tile's keys and half of the columns, who exchange the row's maximum; warp 9
 // loads, warp 10 brings Q, warp 11 is idle. 24 mixed sequences, 512 new tokens in one: 115 us, 126 with a thread per row.
 // Bound by what the softmax warps do one after another in a tile (exponentials and conversions 770 clocks, maximum 220, waiting for scores
-// 280), in long runs by the power limit: a prompt of 8192, 32 heads of 128 over 8: 648 us, 850 TFLOP/s of the 1655 that the library's
-// product reaches (1408 sustained); 1080 tokens behind 30001 keys: 715 us. 1.7e4 clocks pass before a launch's second tile: the line of
+// 280; without the remainder) and the tensor core's P V of it: a prompt of 8192, 32 heads of 128 over 8: 795 us, 692 TFLOP/s of the 1655 that the
+// library's product reaches (1408 sustained); 1080 tokens behind 30001 keys: 870 us. 1.7e4 clocks pass before a launch's second tile: the line of
 // work 3400, finding the first piece 5500, the first scores 1500, the first tile 7500, most of it instructions fetched for the first time.
 // Every wait on a barrier is bounded (paged.cuh). The warps that ask for copies and issue MMAs leave when these are done, in a CTA that gives
 // up, too; then its tensor memory is freed.
@@ -111,8 +114,7 @@ __device__ __forceinline__ void commit(uint32_t bar) {
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
-// The MMAs of a whole tile and the commits behind them, one lane elected once. P V of 64 keys:
-template <bool EXACT>
+// The MMAs of a whole tile and the commits behind them, one lane elected once. P V of 64 keys, then its remainder's:
 __device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t bar0, uint32_t bar1) {
 #define AMV_TS(A, B, P) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [" A "], " B ", %3, " P ";\n\t"
 #define AMV_PV_HEAD                                                                                                                            \
@@ -122,16 +124,11 @@ __device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t b, uint3
 #define AMV_PV_TAIL                                                                                                                            \
     "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t"                                                       \
     "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t}"
-    if constexpr (EXACT)
-        asm volatile(AMV_PV_HEAD "add.u32 c0, %1, 32;\n\tadd.u32 c1, %1, 40;\n\tadd.u32 c2, %1, 48;\n\tadd.u32 c3, %1, 56;\n\t" AMV_TS("%1", "%2", "p")
-                         AMV_TS("a1", "b1", "t") AMV_TS("a2", "b2", "t") AMV_TS("a3", "b3", "t") AMV_TS("c0", "%2", "t") AMV_TS("c1", "b1", "t")
-                             AMV_TS("c2", "b2", "t") AMV_TS("c3", "b3", "t") AMV_PV_TAIL ::"r"(d),
-                     "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(bar0), "r"(bar1)
-                     : "memory");
-    else
-        asm volatile(AMV_PV_HEAD AMV_TS("%1", "%2", "p") AMV_TS("a1", "b1", "t") AMV_TS("a2", "b2", "t") AMV_TS("a3", "b3", "t") AMV_PV_TAIL ::"r"(d), "r"(a),
-                     "l"(b), "r"(idesc), "r"(acc), "r"(bar0), "r"(bar1)
-                     : "memory");
+    asm volatile(AMV_PV_HEAD "add.u32 c0, %1, 32;\n\tadd.u32 c1, %1, 40;\n\tadd.u32 c2, %1, 48;\n\tadd.u32 c3, %1, 56;\n\t" AMV_TS("%1", "%2", "p")
+                     AMV_TS("a1", "b1", "t") AMV_TS("a2", "b2", "t") AMV_TS("a3", "b3", "t") AMV_TS("c0", "%2", "t") AMV_TS("c1", "b1", "t")
+                         AMV_TS("c2", "b2", "t") AMV_TS("c3", "b3", "t") AMV_PV_TAIL ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(bar0), "r"(bar1)
+                 : "memory");
 #undef AMV_TS
 #undef AMV_PV_HEAD
 #undef AMV_PV_TAIL
@@ -165,7 +162,7 @@ __device__ __forceinline__ void mma_s(uint32_t d, uint64_t a, uint64_t b, uint32
 #undef AMV_S_TAIL
 }
 // P V of a tile and S of the one that takes its place, as mma_pv and mma_s.
-template <uint32_t A, bool EXACT>
+template <uint32_t A>
 __device__ __forceinline__ void mma_step(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t bar0, uint32_t bar1, uint64_t q, uint64_t k,
                                          uint32_t idesc_s, uint32_t bar2, uint32_t bar3) {
     constexpr uint64_t QA = kGroupRows * 128u / 16u, KA = kTcKeys * 128u / 16u;
@@ -188,10 +185,8 @@ __device__ __forceinline__ void mma_step(uint32_t d, uint32_t a, uint64_t b, uin
     AMV_SS("x4", "y4", "t") AMV_SS("x5", "y5", "t") AMV_SS("x6", "y6", "t") AMV_SS("x7", "y7", "t")
 #define AMV_TAIL AMV_COMMIT("%10") AMV_COMMIT("%11") "}"
 #define AMV_ARGS "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(bar0), "r"(bar1), "l"(q), "l"(k), "r"(idesc_s), "r"(bar2), "r"(bar3), "n"(QA), "n"(KA)
-    if constexpr (A == 2u && EXACT) asm volatile(AMV_HEAD AMV_LOW AMV_MID AMV_MORE AMV_TAIL ::AMV_ARGS : "memory");
-    else if constexpr (A == 2u) asm volatile(AMV_HEAD AMV_MID AMV_MORE AMV_TAIL ::AMV_ARGS : "memory");
-    else if constexpr (EXACT) asm volatile(AMV_HEAD AMV_LOW AMV_MID AMV_TAIL ::AMV_ARGS : "memory");
-    else asm volatile(AMV_HEAD AMV_MID AMV_TAIL ::AMV_ARGS : "memory");
+    if constexpr (A == 2u) asm volatile(AMV_HEAD AMV_LOW AMV_MID AMV_MORE AMV_TAIL ::AMV_ARGS : "memory");
+    else asm volatile(AMV_HEAD AMV_LOW AMV_MID AMV_TAIL ::AMV_ARGS : "memory");
 #undef AMV_TS
 #undef AMV_SS
 #undef AMV_COMMIT
@@ -371,7 +366,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         if (!ok) break;
                         tc_fence_after();
                         if (EXACT && (t - 2u - x.t0) % kFlush == 0u) started = 0u;
-                        mma_step<A, EXACT>(t_o + acc_of(t - 2u - x.t0), t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
+                        mma_step<A>(t_o + acc_of(t - 2u - x.t0), t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
                                            dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
                         started = 1u;
                         if (t + 1u == x.t1) commit(q_empty + 8u * g);
@@ -398,7 +393,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                             const uint32_t steps = ~bad_2 & 0xFu;   // 16 keys whose page is there
                             const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
                             if (steps == 0xFu && key0 >= x.lo && key0 + kTcKeys <= x.hi) {
-                                mma_pv<EXACT>(t_acc, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
+                                mma_pv(t_acc, t_s + b * kTcKeys, dvt, idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx);
                                 started = 1u;
                             } else {
                                 if (hi_all < key0 + kTcKeys) {   // the rest of the step of the last key
@@ -416,7 +411,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                 for (uint32_t k = s0; k < s1; ++k) {   // 16 keys a step: 8 columns of P, two groups of eight V rows
                                     if (!(steps >> k & 1u)) continue;
                                     mma_ts(t_acc, t_s + b * kTcKeys + 8u * k, dvt + 128u * k, idesc_o, started);
-                                    if (EXACT) mma_ts(t_acc, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
+                                    mma_ts(t_acc, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
                                     started = 1u;
                                 }
                                 if (EXACT && !started) {   // no page of the tile is there, and the accumulator is to begin anew: with zeros
@@ -636,14 +631,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         sum2[k & 1u] = add2(sum2[k & 1u], pack2(p0, p1));
                         const __half2 hi = __floats2half2_rn(p0, p1);
                         ph[k] = *reinterpret_cast<const uint32_t*>(&hi);
-                        if (EXACT) {
-                            const float2 f2 = __half22float2(hi);
-                            const __half2 low = __floats2half2_rn(p0 - f2.x, p1 - f2.y);
-                            pl[k] = *reinterpret_cast<const uint32_t*>(&low);
-                        }
+                        const float2 f2 = __half22float2(hi);
+                        const __half2 low = __floats2half2_rn(p0 - f2.x, p1 - f2.y);
+                        pl[k] = *reinterpret_cast<const uint32_t*>(&low);
                     }
                     tmem_st16_async(ts + 16u * (part + h), ph);   // over this tile's scores
-                    if (EXACT) tmem_st16_async(ts + 32u + 16u * (part + h), pl);
+                    tmem_st16_async(ts + 32u + 16u * (part + h), pl);
                 }
                 const float2 sums = unpack2(add2(sum2[0], sum2[1]));
                 l_run += sums.x + sums.y;
