@@ -14,7 +14,10 @@ struct Maps {
 constexpr uint32_t kDecRows = 16;                        // paged_attn.cu: rows per tile
 constexpr uint32_t kTcRows = 256, kTcKeys = 64;          // paged_tc.cu: rows (half as many for a 32-bit result) and keys per tile
 
-bool launch_tc(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t head_dim, uint32_t ctas);
+constexpr uint32_t kRenew = 128;                         // key tiles that an accumulator of two row groups takes before it is added to the piece's slot
+
+// exact: one row group, sums added up in registers (32-bit results; also writes f16 ones)
+bool launch_tc(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t head_dim, uint32_t ctas, bool exact);
 
 }  // namespace paged
 }  // namespace amv

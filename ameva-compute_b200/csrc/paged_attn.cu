@@ -733,6 +733,7 @@ struct Plan {
     Args few, many;
     bool use_few, use_many;
     uint32_t tc_rows;
+    bool short_line;   // the tensor-core kernel's line also fits 32 bits with half the rows a tile
 };
 static AcResult plan_set(const Args& pc, uint32_t D, uint64_t max_rows, Plan& x) {
     const uint32_t few_max = few_rows_of(pc, D, max_rows);
@@ -763,6 +764,7 @@ static AcResult plan_set(const Args& pc, uint32_t D, uint64_t max_rows, Plan& x)
     };
     if (x.use_few && too_long(x.few, (few_rows + kDecRows - 1u) / kDecRows)) return AC_ERR_INVALID_SHAPE;
     if (x.use_many && too_long(x.many, (max_rows + x.tc_rows - 1u) / x.tc_rows)) return AC_ERR_INVALID_SHAPE;
+    x.short_line = !too_long(x.many, (max_rows + kTcRows / 2u - 1u) / (kTcRows / 2u));
     return AC_SUCCESS;
 }
 // The sequences of few rows, those of many, and the join of what both cut.
@@ -782,10 +784,12 @@ static AcResult launch_set(const LaunchArgs& a, const Plan& x, uint32_t D, Scrat
     if (use_many) {
         n_many = ctas_for(scratch.left, tc_rows * row, sms);
         many.cut = (uint4*)scratch.take(n_many * 16ull);
-        many.slots = (float*)scratch.take(n_many > 1u ? 2ull * n_many * tc_rows * row : 0u);
+        many.slots = (float*)scratch.take(2ull * n_many * tc_rows * row);
         if (!many.cut || !many.slots) n_many = 1u, many.cut = nullptr, many.slots = nullptr;
     }
-    if (use_many && !launch_tc(a, many, tc_maps, D, n_many)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
+    // f16 results of more keys than one accumulator is to take need a slot to add it to; without, the kernel of 32-bit results rounds them
+    const bool exact = many.out != OUT_F16 || (!many.slots && many.max_kv > kRenew * kTcKeys && x.short_line);
+    if (use_many && !launch_tc(a, many, tc_maps, D, n_many, exact)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
     if (use_few && !launch_rows(a, few, rows_maps, D, n_few)) return AC_ERR_INVALID_WORK_GROUP_SIZE;
     const uint32_t merge_few = n_few > 1u ? n_few : 0u, merge_many = n_many > 1u ? n_many : 0u;
     if (merge_few + merge_many && !launch_merge(a, few, many, D, merge_few, merge_many, kDecRows, tc_rows)) return AC_ERR_INVALID_WORK_GROUP_SIZE;

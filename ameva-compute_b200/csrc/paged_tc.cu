@@ -6,7 +6,7 @@
 //   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 64 scores from tensor memory, online softmax to base 2, write P
 //                    over the scores as f16, and what that rounding left beside it, so that a result has the 32 bits that it is computed in
 //                    until it is rounded itself (without the remainder an f16 one is off by 1.25 to 1.4 times what its own rounding leaves,
-//                    and a prompt of 8192 takes 640 us instead of 795). The accumulator is rescaled only when a row's maximum has
+//                    and a prompt of 8192 takes 640 us instead of 808). The accumulator is rescaled only when a row's maximum has
 //                    grown by more than 2^kGrowth since its last rescale, as attention kernels for this chip are known to do. They
 //                    write the piece's results.
 //   warps 8, 9       issue the MMAs of group 0 and 1: S = Q K^T (both in shared memory), O += P V (P in tensor memory, V MN-major). Each
@@ -18,13 +18,17 @@
 //   warp 11          brings the Q rows in, those of the next piece as soon as the last S of this one has read them
 // Tensor memory: four S / P tiles of 64 columns, two O of D. Key tiles that no row of a group sees are left out for it, and of a tile the
 // steps of 16 keys that none sees; V rows behind the last key are zeroed before they are multiplied (a page holds anything there).
-// EXACT. The tensor core's sums are cut rather than rounded, which an f16 result does not show and a 32-bit one would (2.2e-6 after 300 of
-// them, in proportion to their number): two accumulators take kFlush tiles each in turn and are added to a sum in registers (7.8e-7). Warps
+// The tensor core's sums are cut rather than rounded: 7e-9 of a sum per MMA, whatever it is small against, and always downwards. An f16 result
+// (its rounding leaves 2.1e-4) shows that from some ten thousand keys on (131072 keys in one accumulator, values around 1: 6.8e-4, 500000: 2.3e-3).
+// So an accumulator takes kRenew tiles, 8192 keys; then the group's softmax warps add it to their piece's slot in the scratch, and it
+// begins anew (4e-5 at most; 12 us each time for both groups, 4 % of the 30001 keys below).
+// EXACT. A 32-bit result shows it at once (2.2e-6 after 300 MMAs): two accumulators take kFlush tiles each in turn and are added to a sum in
+// registers (7.8e-7). This form writes f16 results, too, where the scratch holds no slot and there may be more than kRenew tiles. Warps
 // 0-3 and 4-7 are two threads per row, each with half of a tile's keys and half of the columns, who exchange the row's maximum; warp 9
 // loads, warp 10 brings Q, warp 11 is idle. 24 mixed sequences, 512 new tokens in one: 115 us, 126 with a thread per row.
 // Bound by what the softmax warps do one after another in a tile (exponentials and conversions 770 clocks, maximum 220, waiting for scores
-// 280; without the remainder) and the tensor core's P V of it: a prompt of 8192, 32 heads of 128 over 8: 795 us, 692 TFLOP/s of the 1655 that the
-// library's product reaches (1408 sustained); 1080 tokens behind 30001 keys: 870 us. 1.7e4 clocks pass before a launch's second tile: the line of
+// 280; without the remainder) and the tensor core's P V of it: a prompt of 8192, 32 heads of 128 over 8: 808 us, 680 TFLOP/s of the 1655 that the
+// library's product reaches (1408 sustained); 1080 tokens behind 30001 keys: 908 us. 1.7e4 clocks pass before a launch's second tile: the line of
 // work 3400, finding the first piece 5500, the first scores 1500, the first tile 7500, most of it instructions fetched for the first time.
 // Every wait on a barrier is bounded (paged.cuh). The warps that ask for copies and issue MMAs leave when these are done, in a CTA that gives
 // up, too; then its tensor memory is freed.
@@ -58,7 +62,7 @@ struct Tc {
     static constexpr uint32_t FIXED = 1024u + GROUPS * Q + 2u * STAGES * TILE + STAGE_OUT + PAIRS + 512u;
     static constexpr uint32_t smem(uint32_t n_seqs) { return FIXED + (n_seqs + 1u) * 4u; }
 };
-constexpr uint32_t kFlush = 4;   // EXACT: key tiles that an accumulator takes before it is added to the row's sum
+constexpr uint32_t kFlush = 4;     // EXACT: key tiles that an accumulator takes before it is added to the row's sum
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int page) {
     asm volatile(
@@ -204,6 +208,83 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t smem_addr) {
     return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(kTcKeys * 128u >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// 32 rows x 16 columns of 32 bits through 2048 bytes of shared memory, so that a row leaves 64 bytes at a time (a lane per row and 16 bytes: 32
+// lines per store, 10 us a piece): lane 4 k + c takes columns 4 c .. 4 c + 3 of rows 8 i + k.
+struct Staging {
+    uint32_t base, lane, piece;
+    __device__ __forceinline__ Staging(uint32_t at, uint32_t lane_) : base(at), lane(lane_), piece(lane_ & 3u) {}
+    __device__ __forceinline__ uint32_t row(uint32_t i) const { return 8u * i + (lane >> 2); }
+    __device__ __forceinline__ void put(const uint32_t (&v)[16]) const {   // this lane's row
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + lane * 64u + ((k ^ (lane >> 1 & 3u)) << 4)), "r"(v[4 * k]), "r"(v[4 * k + 1]),
+                         "r"(v[4 * k + 2]), "r"(v[4 * k + 3])
+                         : "memory");
+        __syncwarp();
+    }
+    __device__ __forceinline__ float4 get(uint32_t r) const {
+        float4 y;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
+                     : "r"(base + r * 64u + ((piece ^ (r >> 1 & 3u)) << 4))
+                     : "memory");
+        return y;
+    }
+};
+__device__ __forceinline__ void add4(float4& y, const float4& e, float f) {
+    y.x = fmaf(e.x, f, y.x);
+    y.y = fmaf(e.y, f, y.y);
+    y.z = fmaf(e.z, f, y.z);
+    y.w = fmaf(e.w, f, y.w);
+}
+
+// The accumulator of a warp's rows goes to the piece's slot (f32 [row of the group][D + 4]: the maximum it refers to, values from column 4 on), with
+// what the slot holds already unless this is the first time. Returns whether a column of this thread's row is not finite. What the
+// slot holds is read a round ahead. A function of its own, so that the loop over key tiles keeps its registers.
+template <int D>
+__device__ __noinline__ bool add_to_slot(float* slot, uint32_t n_rows, uint32_t acc, uint32_t s_out, bool first, float m) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, r0 = (warp & 3u) * 32u;
+    const Staging stage(s_out + warp * 2048u, lane);
+    float* own = slot + (uint64_t)(r0 + lane) * (D + 4u);
+    const bool mine = r0 + lane < n_rows;
+    const float f = first || !mine ? 0.0f : weight(*own, m);
+    if (mine) *own = m;
+    float check = 0.0f, f_row[4];
+    float4 held[4];
+    float* at[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t r = stage.row(i);
+        f_row[i] = __shfl_sync(0xffffffffu, f, r);
+        at[i] = r0 + r < n_rows ? slot + (uint64_t)(r0 + r) * (D + 4u) + 4u + 4u * stage.piece : nullptr;
+        held[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (f_row[i] != 0.0f) held[i] = *reinterpret_cast<const float4*>(at[i]);
+    }
+#pragma unroll 1
+    for (uint32_t c = 0; c < D; c += 16u) {
+        float4 now[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            now[i] = held[i];
+            if (f_row[i] != 0.0f && c + 16u < D) held[i] = *reinterpret_cast<const float4*>(at[i] + c + 16u);
+        }
+        uint32_t v[16];
+        tmem_ld16(acc + c, v);
+#pragma unroll
+        for (uint32_t k = 0; k < 16u; ++k) check = fmaf(__uint_as_float(v[k]), 0.0f, check);
+        stage.put(v);
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            if (!at[i]) continue;
+            float4 y = stage.get(stage.row(i));
+            if (f_row[i] != 0.0f) add4(y, now[i], f_row[i]);
+            *reinterpret_cast<float4*>(at[i] + c) = y;
+        }
+        __syncwarp();
+    }
+    return mine && check != 0.0f;
+}
+
 // A group's share of a piece: its rows, the keys any of them sees and those all of them see, its key tiles [t0, t1).
 struct Group {
     uint32_t r0, rows, lo, hi, lo_all, hi_all, t0, t1;
@@ -346,6 +427,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             const uint32_t t_s = tmem + 2u * g * kTcKeys, t_o = tmem + 2u * GROUPS * kTcKeys + g * D;
             // EXACT: the accumulator of the group's tile i of a piece, two in turn
             auto acc_of = [](uint32_t i) { return EXACT ? (i / kFlush & 1u) * (uint32_t)D : 0u; };
+            const uint32_t takes = EXACT ? kFlush : pc.slots ? kRenew : 1u << 31;   // key tiles that an accumulator takes
+            auto anew = [&](uint32_t i) { return (i & (takes - 1u)) == 0u; };
             const uint64_t dq = make_smem_desc(smem_u32(sQ + g * L::Q)), dk = make_smem_desc(smem_u32(sK)), dv = v_desc(smem_u32(sV));
             const uint32_t my_s = s_full + 16u * g, my_p = p_full + 16u * g, my_pv = pv_done + 16u * g;
             Ring kr(ST), vr(ST);
@@ -365,7 +448,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         tc_fence_after();
-                        if (EXACT && (t - 2u - x.t0) % kFlush == 0u) started = 0u;
+                        if (anew(t - 2u - x.t0)) started = 0u;
                         mma_step<A>(t_o + acc_of(t - 2u - x.t0), t_s + b * kTcKeys, dv + vr.idx * (L::TILE / 16u), idesc_o, started, my_pv + 8u * b, v_empty + 8u * vr.idx, dq,
                                            dk + kr.idx * (L::TILE / 16u), idesc_s, my_s + 8u * b, k_empty + 8u * kr.idx);
                         started = 1u;
@@ -388,7 +471,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         if (mine) {
                             ++p_tiles;
                             tc_fence_after();
-                            if (EXACT && (u - x.t0) % kFlush == 0u) started = 0u;
+                            if (anew(u - x.t0)) started = 0u;
                             const uint32_t t_acc = t_o + acc_of(u - x.t0);
                             const uint32_t steps = ~bad_2 & 0xFu;   // 16 keys whose page is there
                             const uint64_t dvt = dv + vr.idx * (L::TILE / 16u);
@@ -414,7 +497,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                                     mma_ts(t_acc, t_s + b * kTcKeys + 32u + 8u * k, dvt + 128u * k, idesc_o, 1u);
                                     started = 1u;
                                 }
-                                if (EXACT && !started) {   // no page of the tile is there, and the accumulator is to begin anew: with zeros
+                                if (!started) {   // no page of the tile is there, and the accumulator is to begin anew: with zeros
                                     for (uint32_t j = lane; j < 16u * (D / 8u); j += 32u) {
                                         const uint32_t r = 16u * s0 + j / (D / 8u), c = j % (D / 8u);
                                         *reinterpret_cast<uint4*>(sV + vr.idx * L::TILE + (c >> 3) * (kTcKeys * 128u) + r * 128u + ((c & 7u) << 4)) =
@@ -520,6 +603,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
         // turn: a warp writes to one again behind the next barrier, which the other one passes after it has read.
         float2* s_pair = reinterpret_cast<float2*>(s_out + L::STAGE_OUT);
         uint32_t told = 0;
+        auto slot_rows = [&](const Piece& p, const Group& x) {
+            return pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * L::ROWS + (x.r0 - p.r0)) * (D + 4u);
+        };
         auto tell = [&](float v, bool& fine) {
             s_pair[((told & 1u) * 2u + part) * kGroupRows + my] = make_float2(v, fine ? 1.0f : 0.0f);
             tc_fence_before();
@@ -556,6 +642,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             };
             for (uint32_t t = x.t0; t < x.t1; ++t, ++j) {
                 const uint32_t key0 = t * kTcKeys, b = j & 1u, ts = tmem + lanes + (2u * g + b) * kTcKeys;
+                if (!EXACT && t != x.t0 && (t - x.t0) % kRenew == 0u && pc.slots) {   // the accumulator goes to the slot, and begins anew
+                    ok = ok && wait_on(pv_done + 16u * g + 8u * (b ^ 1u), ((j - 1u) >> 1) & 1u, ctl, pc.status, 0xDC4u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    again = add_to_slot<D>(slot_rows(p, x), x.rows, to, smem_u32(s_out), t - x.t0 == kRenew, m_run) || again;
+                }
                 ok = ok && wait_on(s_full + 16u * g + 8u * b, (j >> 1) & 1u, ctl, pc.status, 0xDA0u);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!EXACT && !ok) break;
@@ -658,9 +751,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             if (EXACT && some && n_tiles > 1u && (n_tiles - 1u) % kFlush == 0u) add_up((n_tiles - 2u) / kFlush & 1u);
             if (x.rows) {
                 const uint32_t query = query_of(pc, row), token = p.q.tok0 + query, head = p.group * pc.G + row - query * pc.G;
-                float* slot = pc.slots + ((uint64_t)(2u * blockIdx.x + (p.a == 0u ? 1u : 0u)) * L::ROWS + (x.r0 - p.r0)) * (D + 4u);
+                float* slot = slot_rows(p, x);
                 const bool parts = !whole || pc.out == OUT_PARTS;
                 float own = 1.0f, other = 0.0f;      // factors of the values here and of those over other keys
+                // what the slot holds of this piece
+                const float m_slot = !EXACT && pc.slots && valid && x.t1 - x.t0 > kRenew ? slot[(uint64_t)my * (D + 4u)] : neg_inf();
                 const float* extra = nullptr;
                 void* dst = nullptr;
                 if (valid) {
@@ -686,19 +781,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         dst = pc.out == OUT_F16 ? (void*)(reinterpret_cast<__half*>(pc.dst) + e) : (void*)(reinterpret_cast<float*>(pc.dst) + e);
                     }
                 }
-                const bool nothing = l_run == 0.0f;   // nothing was accumulated, or only what zeros made
                 float check = 0.0f;
-                // Through shared memory, so that a row leaves 64 bytes at a time (a lane per row and 16 bytes: 32 lines per store, 10 us a
-                // piece): lane 4 i + j of a round has columns 4 j .. 4 j + 3 of row i.
-                const uint32_t mine = smem_u32(s_out) + warp * 2048u, my_at = mine + lane * 64u, sub = lane >> 2, piece = lane & 3u;
-                const uint32_t swz = (lane >> 1) & 3u;
+                const bool nothing = l_run == 0.0f;   // nothing was accumulated, or only what zeros made
                 unsigned long long row_dst[4], row_extra[4];
-                float row_other[4];
+                float row_other[4], row_slot[4];   // row_slot: the factor of what the slot holds of this piece
+                const float held = nothing ? 0.0f : weight(m_slot, m_run) * own;
+                const Staging stage(smem_u32(s_out) + warp * 2048u, lane);
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i) {
-                    row_dst[i] = __shfl_sync(0xffffffffu, (unsigned long long)dst, 8u * i + sub);
-                    row_extra[i] = __shfl_sync(0xffffffffu, (unsigned long long)extra, 8u * i + sub);
-                    row_other[i] = __shfl_sync(0xffffffffu, other, 8u * i + sub);
+                    row_dst[i] = __shfl_sync(0xffffffffu, (unsigned long long)dst, stage.row(i));
+                    row_extra[i] = __shfl_sync(0xffffffffu, (unsigned long long)extra, stage.row(i));
+                    row_other[i] = __shfl_sync(0xffffffffu, other, stage.row(i));
+                    row_slot[i] = __shfl_sync(0xffffffffu, held, stage.row(i));
                 }
                 const bool f16 = !parts && pc.out == OUT_F16;
 #pragma unroll(EXACT ? COLS / 16 : 1)
@@ -711,34 +805,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                         check = fmaf(o, 0.0f, check);
                         v[j] = __float_as_uint(own == 0.0f ? 0.0f : o * own);
                     }
-#pragma unroll
-                    for (uint32_t j = 0; j < 4u; ++j)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(my_at + ((j ^ swz) << 4)), "r"(v[4 * j]), "r"(v[4 * j + 1]),
-                                     "r"(v[4 * j + 2]), "r"(v[4 * j + 3])
-                                     : "memory");
-                    __syncwarp();
+                    stage.put(v);
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; ++i) {
                         if (!row_dst[i]) continue;
-                        const uint32_t r = 8u * i + sub;
-                        float4 y;
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
-                                     : "r"(mine + r * 64u + ((piece ^ ((r >> 1) & 3u)) << 4))
-                                     : "memory");
-                        if (row_extra[i]) {
-                            const float4 e = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row_extra[i]) + 4u + part * COLS + c + 4u * piece);
-                            y.x = fmaf(e.x, row_other[i], y.x);
-                            y.y = fmaf(e.y, row_other[i], y.y);
-                            y.z = fmaf(e.z, row_other[i], y.z);
-                            y.w = fmaf(e.w, row_other[i], y.w);
-                        }
+                        float4 y = stage.get(stage.row(i));
+                        if (!EXACT && row_slot[i] != 0.0f)
+                            add4(y, *reinterpret_cast<const float4*>(slot + (uint64_t)((warp & 3u) * 32u + stage.row(i)) * (D + 4u) + 4u + c + 4u * stage.piece), row_slot[i]);
+                        if (row_extra[i])
+                            add4(y, *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row_extra[i]) + 4u + part * COLS + c + 4u * stage.piece), row_other[i]);
                         if (f16) {
                             const __half2 h0 = __floats2half2_rn(y.x, y.y), h1 = __floats2half2_rn(y.z, y.w);
-                            *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(row_dst[i]) + c + 4u * piece) =
+                            *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(row_dst[i]) + c + 4u * stage.piece) =
                                 make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
                         } else {
-                            *reinterpret_cast<float4*>(reinterpret_cast<float*>(row_dst[i]) + c + 4u * piece) = y;
+                            *reinterpret_cast<float4*>(reinterpret_cast<float*>(row_dst[i]) + c + 4u * stage.piece) = y;
                         }
                     }
                     __syncwarp();
@@ -770,8 +851,7 @@ static bool launch_tc_t(const LaunchArgs& a, const Args& pc, const Maps& maps, u
     return true;
 }
 
-bool launch_tc(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t head_dim, uint32_t ctas) {
-    const bool exact = pc.out != OUT_F16;
+bool launch_tc(const LaunchArgs& a, const Args& pc, const Maps& maps, uint32_t head_dim, uint32_t ctas, bool exact) {
     return head_dim == 64u ? (exact ? launch_tc_t<64, true>(a, pc, maps, ctas) : launch_tc_t<64, false>(a, pc, maps, ctas))
                            : (exact ? launch_tc_t<128, true>(a, pc, maps, ctas) : launch_tc_t<128, false>(a, pc, maps, ctas));
 }
