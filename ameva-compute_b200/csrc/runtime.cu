@@ -952,6 +952,14 @@ AcResult ac_b200_context_get_stream(const AcContext* ctx, void** out_stream) {
     return AC_SUCCESS;
 }
 
+AcResult ac_b200_context_get_sm_count(const AcContext* ctx, uint32_t* out_count) {
+    if (!out_count) return AC_ERR_NULL_POINTER;
+    *out_count = 0;
+    if (!ctx_ok(ctx)) return AC_ERR_INVALID_CONTEXT;
+    *out_count = (uint32_t)ctx->prop.multiProcessorCount;
+    return AC_SUCCESS;
+}
+
 AcResult ac_b200_context_synchronize(AcContext* ctx) {
     if (!ctx_ok(ctx)) return AC_ERR_INVALID_CONTEXT;
     DeviceGuard g(ctx->device);

@@ -130,9 +130,10 @@ def record_prefix_attention(batch: rt.Batch, cache: Cache, seqs: Sequences, q: r
                    [q, cache.k, cache.v, seqs.table, seqs.q_start, seqs.kv_len, dst, scratch, status, prefix], push)
 
 
-def scratch_bytes(ctx: rt.Context, seqs: Sequences, *, heads: int, head_dim: int, prefix: bool = False, sms: int = 148) -> int:
-    """Bytes of scratch with which the attention of this batch takes the whole GPU of `ctx` (every B200 has 148 SMs): per SM two row tiles of
-    16 rows of eight KV heads and two of 256 rows, and for a shared prefix the rows' results over their own keys."""
+def scratch_bytes(ctx: rt.Context, seqs: Sequences, *, heads: int, head_dim: int, prefix: bool = False, sms: Optional[int] = None) -> int:
+    """Bytes of scratch with which the attention of this batch takes the whole GPU of `ctx` (or `sms` SMs): per SM two row tiles of 16 rows of
+    eight KV heads and two of 256 rows, and for a shared prefix the rows' results over their own keys."""
+    sms = ctx.sm_count if sms is None else sms
     row = (head_dim + 4) * 4
     own = seqs.rows * heads * row + 256 if prefix else 0
     return own + sms * (2 * (8 * 16 + 256) * row + 128) + 8192

@@ -130,7 +130,7 @@ EXPORTED_SYMBOLS = [
     "ac_runtime_get_generation", "ac_runtime_reset_error_state", "ac_runtime_set_error_ctx",
     "ac_runtime_get_error_state_ctx", "ac_runtime_consume_error_ctx", "ac_runtime_advance_generation_ctx",
     "ac_runtime_get_generation_ctx", "ac_runtime_reset_error_state_ctx", "ac_runtime_kernel_create_builtin",
-    "ac_b200_kernel_count", "ac_b200_kernel_name", "ac_b200_kernel_register", "ac_b200_weight_upload", "ac_b200_context_get_stream", "ac_b200_buffer_import",
+    "ac_b200_kernel_count", "ac_b200_kernel_name", "ac_b200_kernel_register", "ac_b200_weight_upload", "ac_b200_context_get_stream", "ac_b200_context_get_sm_count", "ac_b200_buffer_import",
     "ac_b200_buffer_export_ipc", "ac_b200_buffer_open_ipc", "ac_b200_buffer_write_async", "ac_b200_buffer_read_async", "ac_b200_context_synchronize", "ac_b200_batch_instantiate", "ac_b200_batch_replay", "ac_b200_batch_get_launches", "ac_b200_gemm_last_k_ranges",
     "ac_b200_device_layout", "ac_b200_device_type", "ac_b200_repack_to_device", "ac_b200_repack_from_device", "ac_b200_mul_mat_plan",
     "ac_b200_weight_exponent",
@@ -209,6 +209,7 @@ def load_library() -> C.CDLL:
         "ac_b200_kernel_register": (C.c_int, [C.c_char_p, u32, u32, C.c_void_p]),
         "ac_b200_weight_upload": (C.c_int, [vp, sz, u32, vp, u64, u64]),
         "ac_b200_context_get_stream": (C.c_int, [vp, P(vp)]),
+        "ac_b200_context_get_sm_count": (C.c_int, [vp, P(C.c_uint32)]),
         "ac_b200_buffer_import": (C.c_int, [vp, vp, sz, P(vp)]),
         "ac_b200_buffer_export_ipc": (C.c_int, [vp, vp]),
         "ac_b200_buffer_open_ipc": (C.c_int, [vp, vp, sz, P(vp)]),
@@ -455,6 +456,12 @@ class Context:
         out = C.c_void_p()
         _check(load_library().ac_b200_context_get_stream(self._h, C.byref(out)))
         return out.value or 0
+
+    @property
+    def sm_count(self) -> int:
+        out = C.c_uint32(0)
+        _check(load_library().ac_b200_context_get_sm_count(self._h, C.byref(out)))
+        return out.value
 
     def limits(self) -> AcDeviceLimits:
         lim = AcDeviceLimits(AC_ABI_VERSION, C.sizeof(AcDeviceLimits))

@@ -354,6 +354,8 @@ typedef AcResult (*AcB200LaunchFn)(const AcB200Launch* launch);
 AcResult ac_b200_kernel_register(const char* name, uint32_t binding_count, uint32_t push_constant_size, AcB200LaunchFn fn);
 /* The context's CUDA stream (a cudaStream_t), for callers that time or order their own work against it. */
 AcResult ac_b200_context_get_stream(const AcContext* ctx, void** out_stream);
+/* Streaming multiprocessors of the context's device: what launches that deal their work to one CTA per SM are sized by. */
+AcResult ac_b200_context_get_sm_count(const AcContext* ctx, uint32_t* out_count);
 /* Wrap device memory owned by the caller (e.g. a framework allocator) as a buffer; destroy does not free it. */
 AcResult ac_b200_buffer_import(AcContext* ctx, void* device_ptr, size_t size_bytes, AcBuffer** out_buf);
 /* Sharing a buffer between the ranks of one box (one process per GPU): the owner exports a 64-byte handle
