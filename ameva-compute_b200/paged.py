@@ -88,7 +88,8 @@ def record_append(batch: rt.Batch, cache: Cache, seqs: Sequences, q: rt.Buffer, 
                   q_stride: Optional[int] = None, k_stride: Optional[int] = None, v_stride: Optional[int] = None,
                   q_out_stride: Optional[int] = None, node: int = 0) -> None:
     """q f32 [rows][heads x head_dim], k and v f32 [rows][kv_heads x head_dim] (strides in floats: the three may be column ranges of one
-    product) -> q_out f16 rotated, k rotated and v in the cache. positions: i32 [rows] instead of the keys' places; factors: f32
+    product) -> q_out f16 rotated, k rotated and v in the cache. positions: i32 [rows] instead of the keys' places, which are counted from
+    a sequence's first own key: behind a shared prefix they have to be given, the prefix's number of keys added. factors: f32
     [n_dims / 2]. Rows behind the last sequence are left as they are; tokens whose place has no page are not written, and counted."""
     D, w, kw = cache.head_dim, heads * cache.head_dim, cache.kv_heads * cache.head_dim
     flags = (1 if positions is not None else 0) | (2 if factors is not None else 0)
@@ -123,7 +124,8 @@ def record_prefix_attention(batch: rt.Batch, cache: Cache, seqs: Sequences, q: r
                             status: rt.Buffer, *, prefix: rt.Buffer, max_prefix: int, heads: int, scale: float, softcap: float = 0.0,
                             f16_out: bool = False, q_stride: Optional[int] = None, dst_stride: Optional[int] = None, node: int = 0) -> None:
     """`record_attention` for sequences whose keys begin with a prefix that all of them share. prefix: i32 [1 + pages], its number of keys
-    (at most max_prefix) and its pages; `seqs` describes the keys behind it. The rows begin at 0, and a batch with a sequence that does not
+    (at most max_prefix) and its pages; `seqs` describes the keys behind it, which are appended with the positions that they have behind
+    it (`record_append`: positions). The rows begin at 0, and a batch with a sequence that does not
     fit its numbers is left out altogether."""
     push = _attention_push(cache, seqs, heads, scale, softcap, f16_out, q_stride, dst_stride) + [max_prefix, node]
     batch.dispatch(batch.ctx.kernel("ameva_paged_prefix_attn"),
