@@ -80,15 +80,21 @@ __device__ __forceinline__ Seq load_seq(const Args& pc, uint32_t s, bool report 
     return x;
 }
 
+// Query heads that share a KV head, and what query_of divides by them with.
+inline void set_group(Args& pc, uint32_t G) {
+    pc.G = G;
+    for (pc.g_shift = 31u; (1ull << (pc.g_shift - 31u)) < G; ++pc.g_shift) {}
+    pc.g_mul = (uint32_t)(((1ull << pc.g_shift) + G - 1u) / G);
+}
 // r / G without a division's instructions, which a CTA runs once and has to fetch: g_mul = ceil(2^g_shift / G) and g_shift = 31 + ceil(log2 G)
 // are off by less than 2^31 in r * g_mul, so that no quotient of r < 2^31 moves.
-__device__ __forceinline__ uint32_t query_of(const Args& pc, uint32_t r) { return (uint32_t)((uint64_t)r * pc.g_mul >> pc.g_shift); }
+__host__ __device__ __forceinline__ uint32_t query_of(const Args& pc, uint32_t r) { return (uint32_t)((uint64_t)r * pc.g_mul >> pc.g_shift); }
 
 // The keys that row r sees: [lo, hi)
 struct Span {
     uint32_t lo, hi;
 };
-__device__ __forceinline__ Span row_span(const Args& pc, const Seq& q, uint32_t r) {
+__host__ __device__ __forceinline__ Span row_span(const Args& pc, const Seq& q, uint32_t r) {
     if (pc.prefix) return {0u, q.kv};
     const int32_t end = (int32_t)q.kv - (int32_t)q.n_q + (int32_t)query_of(pc, r) + 1;   // one past its own place
     if (end <= 0) return {0u, 0u};
@@ -96,7 +102,7 @@ __device__ __forceinline__ Span row_span(const Args& pc, const Seq& q, uint32_t 
     return {pc.window && hi > pc.window ? hi - pc.window : 0u, hi};
 }
 // The first key tile of rows r0 .. r1 and how many there are: at least one, so that rows that see nothing are written, too.
-__device__ __forceinline__ void tile_range(const Args& pc, const Seq& q, uint32_t r0, uint32_t r1, uint32_t& first, uint32_t& count) {
+__host__ __device__ __forceinline__ void tile_range(const Args& pc, const Seq& q, uint32_t r0, uint32_t r1, uint32_t& first, uint32_t& count) {
     const uint32_t lo = row_span(pc, q, r0).lo, hi = row_span(pc, q, r1).hi;
     first = lo >> pc.keys_log2;
     count = hi > lo ? ((hi + (1u << pc.keys_log2) - 1u) >> pc.keys_log2) - first : 1u;
@@ -187,20 +193,21 @@ __device__ __forceinline__ uint32_t build_line(const Args& pc, uint32_t* s_pref,
 struct Stretch {
     uint32_t begin, end, ctas, total;
 };
-__device__ __forceinline__ Stretch my_stretch(uint32_t total) {
+__host__ __device__ __forceinline__ Stretch stretch_of(uint32_t total, uint32_t cta, uint32_t grid) {
     Stretch x;
     x.total = total;
-    x.ctas = min(gridDim.x, total);
+    x.ctas = grid < total ? grid : total;
     x.begin = x.end = 0u;
-    if (blockIdx.x < x.ctas) {
+    if (cta < x.ctas) {
         const uint32_t q = total / x.ctas, r = total - q * x.ctas;   // floor(c total / ctas) in 32 bits
-        x.begin = blockIdx.x * q + blockIdx.x * r / x.ctas;
-        x.end = (blockIdx.x + 1u) * q + (blockIdx.x + 1u) * r / x.ctas;
+        x.begin = cta * q + cta * r / x.ctas;
+        x.end = (cta + 1u) * q + (cta + 1u) * r / x.ctas;
     }
     return x;
 }
+__device__ __forceinline__ Stretch my_stretch(uint32_t total) { return stretch_of(total, blockIdx.x, gridDim.x); }
 // the last CTA whose stretch has a tile in front of tile e (e > 0)
-__device__ __forceinline__ uint32_t last_cta(const Stretch& x, uint32_t e) {
+__host__ __device__ __forceinline__ uint32_t last_cta(const Stretch& x, uint32_t e) {
     return (uint32_t)(((uint64_t)e * x.ctas + x.total - 1u) / x.total) - 1u;
 }
 

@@ -649,9 +649,7 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
     if (!D || !pc.n_head || !pc.n_head_kv || pc.n_head % pc.n_head_kv || !pc.n_seqs || !pc.rows || !pc.max_q || !pc.max_kv || !P || (P & (P - 1u)) ||
         !pc.n_pages || !pc.table_stride || pc.out > OUT_F16 || !(pc.softcap >= 0.0f) || pc.scale != pc.scale)
         return AC_ERR_KERNEL_ARG_INVALID;
-    pc.G = pc.n_head / pc.n_head_kv;
-    for (pc.g_shift = 31u; (1ull << (pc.g_shift - 31u)) < pc.G; ++pc.g_shift) {}
-    pc.g_mul = (uint32_t)(((1ull << pc.g_shift) + pc.G - 1u) / pc.G);
+    set_group(pc, pc.n_head / pc.n_head_kv);
     if ((D != 64u && D != 128u && D != 256u) || P < 16u || P > 1024u) return AC_ERR_FEATURE_NOT_SUPPORTED;
     for (pc.page_log2 = 0; (1u << pc.page_log2) < P; ++pc.page_log2) {}
     if (pc.n_seqs > kMaxSeqs || pc.n_head > 65535u || pc.rows > 0x7FFFFFFFu || pc.max_kv > 0x7FFFFFFFu - 1024u || pc.n_pages > 0x7FFFFFFFu ||
