@@ -11,7 +11,7 @@
 // read together because in a cache with a token's heads beside one another they are one run of memory: a head at a time (a warp per
 // 16 keys of a tile of 128) took 195 us for 96 sequences of 20 to 8192 keys, 8 KV heads of 128, 160 k keys, as against 100 us for the
 // bytes, and 8 us per (sequence, head). P enters the second product as an f16 value and its remainder (rounded once, 2^-12 of every
-// probability would show in an f32 result, and makes an f16 one's error 1.25 times what its own rounding is; the second product costs 2 %
+// probability would show in an f32 result, and makes an f16 one's error 1.25 to 1.4 times what its own rounding is; the second product costs 2 %
 // of the time above), and the matrix instruction's sums, which are cut rather than rounded, are added up per 32 keys by ordinary
 // additions: left in its accumulator from the first key to the last, 131072 keys are off by 2.3e-6 instead of 4e-7.
 // Bound by HBM, short calls by the instructions that a CTA fetches for the first time: those 96 sequences 119 us (659 MB, 5.5 TB/s; the copy
@@ -685,8 +685,8 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
 
 // Which kernel a sequence of R rows per KV head runs in (D 64, 128; D 256 knows one): paged_rows_kernel reads the keys once per 16 rows, the
 // kernel in paged_tc.cu takes the same time for 1 .. 128, but is one more launch where sequences of few rows are beside it. 8 sequences
-// of 4000 keys, 8 KV heads, f16 results, a pass in us, rows / tensor-core kernel: 32 rows 62 / 68, 64 rows 97 / 67, 128 rows 159 / 72;
-// 64 of 2000 keys: 191 / 165, 340 / 168, 620 / 178 (32-bit results: 192 / 185, 343 / 191, 620 / 203). 32 sequences of 7 to 42 rows, 2 KV
+// of 4000 keys, 8 KV heads, f16 results, a pass in us, rows / tensor-core kernel: 64 rows 97 / 74, 128 rows 159 / 78; 64 of 2000 keys:
+// 340 / 189, 620 / 196 (32-bit results: 32 rows 192 / 185, 343 / 191, 620 / 201). 32 sequences of 7 to 42 rows, 2 KV
 // heads, 1024 keys: 21 / 46. So up to kFewRows; up to kFewRowsAlone while what the rows beyond add is below what the other launch costs:
 // 25 us, in which 360 thousand (row tile, KV head, key) are served.
 constexpr uint32_t kFewRows = 32, kFewRowsAlone = 64;
@@ -699,8 +699,8 @@ static uint32_t few_rows_of(const Args& pc, uint32_t D, uint64_t max_rows) {
     return (pc.prefix ? 1u : pc.n_seqs) * keys * pc.n_head_kv * beyond > kLaunchWork ? kFewRows : kFewRowsAlone;
 }
 // What a row tile costs beside its key tiles, in key tiles (the line's allowance): Q and the first scores on their way, results written.
-// us with none / this: 96 sequences of 20 .. 8192 keys 126 / 119 (1: 121), 32 drafted ones 24.1 / 22.1 (1: 21.5); a prompt of 8192 737 / 648
-// (2: 700, 4: 665, 10: 653, 16: 664), 64 rows behind a prefix of 8192 keys 83.9 / 73.4.
+// us with none / this: 96 sequences of 20 .. 8192 keys 126 / 119 (1: 121), 32 drafted ones 24.1 / 22.1 (1: 21.5); f16 results before P had its
+// remainder: a prompt of 8192 737 / 648 (2: 700, 4: 665, 10: 653, 16: 664), 64 rows behind a prefix of 8192 keys 83.9 / 73.4.
 constexpr uint32_t kFewOver = 2, kManyOver = 6;
 // KV heads that paged_rows_kernel takes at once: all of them where its warps suffice, otherwise equal groups
 static uint32_t few_heads(uint32_t D, uint32_t n_head_kv) {
@@ -802,7 +802,7 @@ static AcResult cache_maps(const LaunchArgs& a, const Args& pc, uint32_t D, Maps
                     encode_cache(enc, &tc_maps.k, a.ptr[1], pc, D, tc_box, 1u) && encode_cache(enc, &tc_maps.v, a.ptr[2], pc, D, tc_box, 1u);
     if (!ok) return AC_ERR_INVALID_SHAPE;
     memset(&tc_maps.q, 0, sizeof(tc_maps.q));
-    // Q by TMA where whole tokens fill a group's 128 rows; otherwise by cp.async, 16 bytes a lane (a prompt of 8192, G = 4: 700 / 739 us)
+    // Q by TMA where whole tokens fill a group's 128 rows; otherwise by cp.async, 16 bytes a lane (a prompt of 8192, G = 4, before P had its remainder: 700 / 739 us)
     tc_maps.q_boxes = D <= 128u && (pc.G & (pc.G - 1u)) == 0u && pc.G <= 128u;
     if (tc_maps.q_boxes) {
         const cuuint64_t dims[3] = {D, pc.n_head, pc.rows}, strides[2] = {2ull * D, 2ull * (pc.rows > 1u ? pc.q_s : (uint64_t)pc.n_head * D)};
@@ -841,7 +841,8 @@ AcResult launch_paged_attn(const LaunchArgs& a) {
     return launch_set(a, plan, D, {(uint8_t*)a.ptr[7], a.range[7]}, rows_maps, tc_maps);
 }
 
-// ameva_paged_prefix_attn: the same for sequences that share a prefix, whose pages are read once for all of them. Binding 9: prefix i32
+// ameva_paged_prefix_attn: the same for sequences that share a prefix, whose pages are read once for all of them (D 64, 128; once per 16 rows,
+// D 256). Binding 9: prefix i32
 // [1 + pages], its number of keys and its pages; kv_len and the tables are those of the sequences' own keys behind it. push words 18, 19:
 // most keys of the prefix, node; no window. The scratch holds rows x n_head x (D + 4) floats at least.
 AcResult launch_paged_prefix_attn(const LaunchArgs& a) {

@@ -2,7 +2,8 @@
 
     append            the projected rows of a step: queries and keys rotated to their positions, keys and values stored in the pages
     attention         of a ragged batch over its pages: single tokens, drafts, prompts, all of them in one call
-    prefix attention  the same for a batch that shares the pages of a long prefix, which are read once for all of it
+    prefix attention  the same for a batch that shares the pages of a long prefix, which are read once for all of it (head_dim 64 and 128; 256: once
+                      per 16 rows)
 
 The reference keeps one contiguous cache per sequence (its ROPE, SET_ROWS and FLASH_ATTN_EXT nodes, adapters/llama/ggml-ameva/ggml-ameva.cpp:
 4008-4111, 5140-5285); a server of several users needs their keys in pages that are handed out one at a time. Everything that changes from
@@ -112,7 +113,7 @@ def _attention_push(cache: Cache, seqs: Sequences, heads, scale, softcap, f16_ou
 def record_attention(batch: rt.Batch, cache: Cache, seqs: Sequences, q: rt.Buffer, dst: rt.Buffer, scratch: rt.Buffer, status: rt.Buffer, *,
                      heads: int, scale: float, softcap: float = 0.0, window: int = 0, f16_out: bool = False, q_stride: Optional[int] = None,
                      dst_stride: Optional[int] = None, node: int = 0) -> None:
-    """q f16 [rows][heads x head_dim] -> dst f32 (f16_out: f16) [rows][heads x head_dim]. Query j of a sequence's n sees the keys up to its
+    """q f16 [rows][heads x head_dim] -> dst f32 (f16_out: the same, rounded to f16 once) [rows][heads x head_dim]. Query j of a sequence's n sees the keys up to its
     own place kv_len - n + j (window: that many of them); one that sees none is zero, rows behind the last sequence are left as they
     are. scratch: see `scratch_bytes`; a smaller one means fewer CTAs, not another result than rounding makes. Launches behind one another
     may share it, batches that run at the same time may not."""
