@@ -435,8 +435,8 @@ __device__ __forceinline__ void capped(const Args& pc, float (&s)[N]) {
 // too, has it from a key that it does not see, and is formed anew, hidden keys left out instead of multiplied by zero: four rows and 32
 // keys at a time, in 32 bits; a score ends in the lane of its key's number.
 // For both, D / 8 lanes take a key, 16 bytes each; group g of them has keys g D / 8 .. of 32, one after another, and the groups meet at the end.
-// One infinity at the first key of every sequence, without / with it: a prompt of 2048, 8 heads of 128 over 2: 46 / 337 us, of 8192, 32 heads over
-// 8: 590 / 7300 us (32-bit results 1090 / 10100); 32 single tokens of 4000 keys 100 / 362 us. Each row's scores again: 17500 us for the first.
+// One infinity at the first key of every sequence, without / with it: a prompt of 2048, 8 heads of 128 over 2: 49 / 350 us, of 8192, 32 heads over
+// 8: 706 / 7700 us (32-bit results 1086 / 9970); 32 single tokens of 4000 keys 98 / 364 us. Each row's scores again: 17500 us for the first.
 template <uint32_t C, uint32_t ROWS>
 struct Again {
     static constexpr uint32_t D = 32u * C, N = 4, LANES = D / 8u, AHEAD = 4, kNone = 0xFFFFFFFFu;
@@ -547,8 +547,9 @@ struct Again {
         for (uint32_t c = 0; c < 8u; ++c) {
             if (x[c] * 0.0f == 0.0f) continue;
             x[c] = sum[c] + common[c];
-            known = known && x[c] != 0.0f;
-            if (extra && extra[c] * 0.0f != 0.0f) x[c] += extra[c];
+            const bool theirs = extra && extra[c] * 0.0f != 0.0f;
+            known = known && (x[c] != 0.0f || (theirs && pc.prefix));   // (of a prefix, no key is hidden)
+            if (theirs) x[c] += extra[c];
         }
         if (!__all_sync(0xffffffffu, known)) return false;
         if (lead == 0u) {   // (finite columns are written as they were)

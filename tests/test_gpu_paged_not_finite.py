@@ -185,3 +185,18 @@ def test_a_sequence_that_is_not_finite_does_not_stall_its_batch(ctx, q, kv, H, H
     assert times[1] <= 40 * times[0], times
     batch.destroy()
     s.close()
+
+
+def test_a_prefix_that_is_not_finite_behind_sequences_that_are_not(ctx):  # noqa: F811
+    """Columns whose only such values are among a row's own keys, others of the prefix, others of both: in every row of the batch."""
+    for D, f in ((128, 300), (64, 900), (256, 100)):
+        q = [1, 3, 40]
+        s = Setup(ctx, q, [n + 30 for n in q], 8, 2, D, 16, "token", seed=D, pad=1, garbage=True, prefix=f)
+        s.v[s.prefix[1], 2, :, 3], s.v[s.prefix[1], 3, :, 4], s.v[s.prefix[2], 5, :, 9] = np.inf, np.nan, np.inf
+        for i in range(3):
+            s.v[place(s, i, 0)][:, 5], s.v[place(s, i, 1)][:, 6] = np.inf, np.nan
+            s.v[place(s, i, 4)][:, 9], s.v[place(s, i, 2)][:, 3] = -np.inf, np.inf
+        upload(s)
+        y = check(s)
+        assert np.isposinf(y[:, :, 3]).all() and np.isposinf(y[:, :, 5]).all() and all(np.isnan(y[:, :, c]).all() for c in (4, 6, 9))
+        s.close()
