@@ -16,6 +16,7 @@
 // additions: left in its accumulator from the first key to the last, 131072 keys are off by 2.3e-6 instead of 4e-7.
 // Bound by HBM, short calls by the instructions that a CTA fetches for the first time: those 96 sequences 119 us (659 MB, 5.5 TB/s; the copy
 // reaches 6.55), one of 131072 keys 103 us (537 MB, 5.2 TB/s), one of 500 keys 18 us (this kernel 8, the merge 5).
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -647,8 +648,11 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
         pc.cap_out = pc.softcap * kLog2e;
     }
     if (!D || !pc.n_head || !pc.n_head_kv || pc.n_head % pc.n_head_kv || !pc.n_seqs || !pc.rows || !pc.max_q || !pc.max_kv || !P || (P & (P - 1u)) ||
-        !pc.n_pages || !pc.table_stride || pc.out > OUT_F16 || !(pc.softcap >= 0.0f) || pc.scale != pc.scale)
+        !pc.n_pages || !pc.table_stride || pc.out > OUT_F16 || !(pc.softcap >= 0.0f))
         return AC_ERR_KERNEL_ARG_INVALID;
+    // what scores are multiplied by is finite (a score of 0 would be NaN otherwise)
+    for (float x : {pc.scale, pc.scale2, pc.softcap, pc.cap_in, pc.cap_out})
+        if (!std::isfinite(x)) return AC_ERR_KERNEL_ARG_INVALID;
     set_group(pc, pc.n_head / pc.n_head_kv);
     if ((D != 64u && D != 128u && D != 256u) || P < 16u || P > 1024u) return AC_ERR_FEATURE_NOT_SUPPORTED;
     for (pc.page_log2 = 0; (1u << pc.page_log2) < P; ++pc.page_log2) {}
