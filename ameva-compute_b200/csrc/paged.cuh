@@ -436,7 +436,7 @@ __device__ __forceinline__ void capped(const Args& pc, float (&s)[N]) {
 // keys at a time, in 32 bits; a score ends in the lane of its key's number.
 // For both, D / 8 lanes take a key, 16 bytes each; group g of them has keys g D / 8 .. of 32, one after another, and the groups meet at the end.
 // One infinity at the first key of every sequence, without / with it: a prompt of 2048, 8 heads of 128 over 2: 49 / 350 us, of 8192, 32 heads over
-// 8: 706 / 7700 us (32-bit results 1086 / 9970); 32 single tokens of 4000 keys 98 / 364 us. Each row's scores again: 17500 us for the first.
+// 8: 714 / 7500 us (32-bit results 974 / 9800); 32 single tokens of 4000 keys 98 / 364 us. Each row's scores again: 17500 us for the first.
 template <uint32_t C, uint32_t ROWS>
 struct Again {
     static constexpr uint32_t D = 32u * C, N = 4, LANES = D / 8u, AHEAD = 4, kNone = 0xFFFFFFFFu;

@@ -690,7 +690,7 @@ static AcResult read_args(const LaunchArgs& a, Args& pc, uint32_t& D) {
 // Which kernel a sequence of R rows per KV head runs in (D 64, 128; D 256 knows one): paged_rows_kernel reads the keys once per 16 rows, the
 // kernel in paged_tc.cu takes the same time for 1 .. 128, but is one more launch where sequences of few rows are beside it. 8 sequences
 // of 4000 keys, 8 KV heads, f16 results, a pass in us, rows / tensor-core kernel: 64 rows 97 / 74, 128 rows 159 / 78; 64 of 2000 keys:
-// 340 / 189, 620 / 196 (32-bit results: 32 rows 192 / 185, 343 / 191, 620 / 201). 32 sequences of 7 to 42 rows, 2 KV
+// 340 / 185, 620 / 195 (32-bit results: 32 rows 192 / 185, 343 / 186, 620 / 196). 32 sequences of 7 to 42 rows, 2 KV
 // heads, 1024 keys: 21 / 46. So up to kFewRows; up to kFewRowsAlone while what the rows beyond add is below what the other launch costs:
 // 25 us, in which 360 thousand (row tile, KV head, key) are served.
 constexpr uint32_t kFewRows = 32, kFewRowsAlone = 64;

@@ -6,7 +6,7 @@
 //   warps 0-3, 4-7   softmax of group 0 and 1, a row per thread: read 64 scores from tensor memory, online softmax to base 2, write P
 //                    over the scores as f16, and what that rounding left beside it, so that a result has the 32 bits that it is computed in
 //                    until it is rounded itself (without the remainder an f16 one is off by 1.25 to 1.4 times what its own rounding leaves,
-//                    and a prompt of 8192 takes 640 us instead of 808). The accumulator is rescaled only when a row's maximum has
+//                    and a prompt of 8192 takes 640 us instead of 810). The accumulator is rescaled only when a row's maximum has
 //                    grown by more than 2^kGrowth since its last rescale, as attention kernels for this chip are known to do. They
 //                    write the piece's results.
 //   warps 8, 9       issue the MMAs of group 0 and 1: S = Q K^T (both in shared memory), O += P V (P in tensor memory, V MN-major). Each
@@ -27,8 +27,8 @@
 // 0-3 and 4-7 are two threads per row, each with half of a tile's keys and half of the columns, who exchange the row's maximum; warp 9
 // loads, warp 10 brings Q, warp 11 is idle. 24 mixed sequences, 512 new tokens in one: 115 us, 126 with a thread per row.
 // Bound by what the softmax warps do one after another in a tile (exponentials and conversions 770 clocks, maximum 220, waiting for scores
-// 280; without the remainder) and the tensor core's P V of it: a prompt of 8192, 32 heads of 128 over 8: 808 us, 680 TFLOP/s of the 1655 that the
-// library's product reaches (1408 sustained); 1080 tokens behind 30001 keys: 908 us. 1.7e4 clocks pass before a launch's second tile: the line of
+// 280; without the remainder) and the tensor core's P V of it: a prompt of 8192, 32 heads of 128 over 8: 810-830 us, 670 TFLOP/s of the 1655 that the
+// library's product reaches (1408 sustained); 1080 tokens behind 30001 keys: 910-930 us. 1.7e4 clocks pass before a launch's second tile: the line of
 // work 3400, finding the first piece 5500, the first scores 1500, the first tile 7500, most of it instructions fetched for the first time.
 // Every wait on a barrier is bounded (paged.cuh). The warps that ask for copies and issue MMAs leave when these are done, in a CTA that gives
 // up, too; then its tensor memory is freed.
@@ -362,6 +362,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
     Walk<L::ROWS> walk(st);
     const uint32_t P = 1u << pc.page_log2, box = P < kTcKeys ? P : kTcKeys, boxes = kTcKeys / box;
     bool ok = true;
+    uint32_t bar0 = 0, asked0 = 0, bar1 = 0, asked1 = 0, depth = 1;   // two rings of copies (or the MMAs) that this warp waits for before it leaves
 
     if (warp >= L::MMA) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -419,8 +420,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     load_v = load;
                 }
             }
-            drain_ring(k_full, k_issued, ST);
-            drain_ring(v_full, v_issued, ST);
+            bar0 = k_full, asked0 = k_issued, bar1 = v_full, asked1 = v_issued, depth = ST;
         } else if (warp < L::LOAD) {
             const uint32_t g = warp - L::MMA;
             const uint32_t idesc_s = make_idesc(1u, 0u, kTcKeys, kGroupRows), idesc_o = make_idesc(1u, 0u, (uint32_t)D, kGroupRows) | (1u << 16);
@@ -541,7 +541,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                 tiles += p.b - p.a;
             }
             commit(drain + 8u * g);   // MMAs already issued finish before the CTA gives its memory back, whoever gives up, and when
-            drain_ring(drain + 8u * g, 1u, 1u);
+            bar0 = drain + 8u * g, asked0 = 1u;
         } else if (warp == L::QWARP) {
             // Q rows into the K-major 128-byte swizzle, idle rows zero
             uint32_t uses[2] = {0u, 0u};
@@ -591,8 +591,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
                     if (lane == 0u) mbar_arrive(q_full + 8u * g);
                 }
             }
-            drain_ring(q_full, uses[0], 1u);   // Q of a group is a ring of one stage
-            drain_ring(q_full + 8u, uses[1], 1u);
+            bar0 = q_full, asked0 = uses[0], bar1 = q_full + 8u, asked1 = uses[1];   // Q of a group is a ring of one stage
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -839,6 +838,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant
             seen_keys_rows<C, L::ROWS>(pc, st, s_pref, 0u, g * kGroupRows + (warp & 3u) * 32u + part * 16u, 32u / L::PARTS);
         }
     }
+    // (one place for all roles: copies of it in each made a prompt of 4096 with 32-bit results 200 us instead of 164)
+    drain_ring(bar0, asked0, depth);
+    drain_ring(bar1, asked1, depth);
     tc_fence_before();
     __syncthreads();
     if (warp == L::MMA) tmem_dealloc<false>(tmem, L::TMEM);
